@@ -384,5 +384,47 @@ int hbk_attn_decode(const void* q, int ldq, const void* k_cache, const void* v_c
 size_t hbk_attn_decode_workspace_floats(int B, int Hq, int D, int num_splits) {
   return hb::attn_decode_workspace_floats(B, Hq, D, num_splits);
 }
+int hbk_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int max_pages, int32_t* free_pages,
+                    const int32_t* free_count, int32_t* free_left, int num_pages, int32_t* cu_seqlens, int32_t* kv_lens, int32_t* positions,
+                    int32_t* slot_mapping, int T, int page_size, void* stream) {
+  return kret(hb::page_tables((cudaStream_t)stream, hb::PageTableArgs{ctx_lens, new_lens, B, page_table, max_pages, free_pages, free_count, free_left, num_pages,
+                                                                      cu_seqlens, kv_lens, positions, slot_mapping, T, page_size}));
+}
+size_t hbk_kv_q4_plane_bytes(int num_pages, int Hkv, int D) { return hb::kv_q4_plane_bytes(num_pages, Hkv, D); }
+int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_t* slot_mapping, void* k_cache, void* v_cache, void* k_seen, int ldks,
+                    void* v_seen, int ldvs, int T, int Hkv, int D, int page_size, int num_pages, void* stream) {
+  return kret(hb::kv_write_q4((cudaStream_t)stream,
+                              hb::CacheWriteQ4Args{(const hb::bf16*)k, ldk, (const hb::bf16*)v, ldv, slot_mapping, (uint8_t*)k_cache, (uint8_t*)v_cache,
+                                                   (hb::bf16*)k_seen, ldks, (hb::bf16*)v_seen, ldvs, T, Hkv, D, page_size, num_pages}));
+}
+int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
+                      const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
+                      int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream) {
+  hb::AttnQ4Args a{};
+  a.q = (const hb::bf16*)q; a.ldq = ldq;
+  a.k_cache = (const uint8_t*)k_cache; a.v_cache = (const uint8_t*)v_cache;
+  a.page_table = page_table; a.max_pages = max_pages; a.kv_lens = kv_lens; a.cu_seqlens = cu_seqlens;
+  a.out = (hb::bf16*)out; a.ldo = ldo; a.workspace = workspace;
+  a.B = B; a.T = T; a.max_q_len = max_q_len; a.max_kv_len = max_kv_len; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page_size = page_size;
+  a.split_pages = split_pages; a.scale = scale; a.num_pages = num_pages; a.window = window; a.softcap = softcap; a.sink = (const hb::bf16*)sink;
+  return kret(hb::attn_q4((cudaStream_t)stream, a));
+}
+int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms) {
+  return hb::attn_q4_split(B, max_q_len, max_kv_len, Hq, Hkv, window, sms);
+}
+size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window) {
+  return hb::attn_q4_workspace_floats(B, T, max_q_len, max_kv_len, Hq, Hkv, D, split_pages, window);
+}
+size_t hbk_gemm_q4_bytes(int N, int K) { return hb::gemm_q4_bytes(N, K); }
+int hbk_gemm_q4_pack(const void* blocks, void* packed, int N, int K, void* stream) {
+  return kret(hb::gemm_q4_pack((cudaStream_t)stream, blocks, packed, N, K));
+}
+int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, const void* R, int ldr, const void* bias, int M, int N, int K, int epi,
+                void* stream) {
+  const bool with_bias = epi == hb::EPI_BIAS || epi == hb::EPI_BIAS_RESID, with_r = epi == hb::EPI_RESID || epi == hb::EPI_BIAS_RESID;
+  if ((epi != hb::EPI_NONE && epi != hb::EPI_F32 && !with_bias && !with_r) || (with_bias && !bias) || (with_r && !R)) return kret(cudaErrorInvalidValue);
+  return kret(hb::gemm_q4((cudaStream_t)stream, hb::GemmQ4Args{(const hb::bf16*)X, ldx, (const uint8_t*)W4, out, ldo, epi == hb::EPI_F32,
+                                                               with_r ? (const hb::bf16*)R : nullptr, ldr, with_bias ? (const hb::bf16*)bias : nullptr, M, N, K}));
+}
 
 }  // extern "C"

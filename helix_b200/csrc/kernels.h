@@ -244,6 +244,64 @@ cudaError_t attn_decode(cudaStream_t stream, const AttnDecodeArgs& a);
 size_t attn_decode_workspace_floats(int B, int Hq, int D, int num_splits);
 
 
+// ---- a step whose cache and weights are held in 4 bits (layouts: quant4.cuh; contracts: include/helix_b200_kernels.h) ----
+struct PageTableArgs {
+  const int32_t *ctx_lens, *new_lens;  // [B]
+  int B;
+  int32_t* page_table; int max_pages;  // [B][max_pages]
+  int32_t* free_pages;                 // stack of num_pages entries
+  const int32_t* free_count; int32_t* free_left;
+  int num_pages;
+  int32_t *cu_seqlens, *kv_lens;       // [B + 1], [B]
+  int32_t *positions, *slot_mapping;   // [T]
+  int T, page_size;
+};
+cudaError_t page_tables(cudaStream_t stream, const PageTableArgs& a);
+
+struct CacheWriteQ4Args {
+  const bf16* k; int ldk;              // [T, >= Hkv * D] (post-RoPE)
+  const bf16* v; int ldv;
+  const int32_t* slots;                // [T]
+  uint8_t *k_cache, *v_cache;          // [num_pages][Hkv][block]
+  bf16* k_seen; int ldks;              // optional: what the cache now stands for (may be k, v themselves)
+  bf16* v_seen; int ldvs;
+  int T, Hkv, D, page_size, num_pages;
+};
+cudaError_t kv_write_q4(cudaStream_t stream, const CacheWriteQ4Args& a);
+size_t kv_q4_plane_bytes(int num_pages, int Hkv, int D);
+
+struct AttnQ4Args {
+  const bf16* q; int ldq;              // [T, >= Hq * D] (post-RoPE)
+  const uint8_t *k_cache, *v_cache;
+  const int32_t* page_table; int max_pages;
+  const int32_t* kv_lens;              // [B]
+  const int32_t* cu_seqlens;           // [B + 1], or NULL: row b is sequence b's
+  bf16* out; int ldo;
+  float* workspace;                    // attn_q4_workspace_floats
+  int B, T, max_q_len, max_kv_len, Hq, Hkv, D, page_size;
+  int split_pages;                     // pages of a block's share; 0: by the rule
+  float scale;
+  int num_pages, window;
+  float softcap;
+  const bf16* sink;                    // [Hq] or NULL
+  int max_splits, kv_bound;            // filled in by the launcher
+};
+cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a);
+int attn_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
+size_t attn_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
+
+struct GemmQ4Args {
+  const bf16* x; int ldx;              // [M, K]
+  const uint8_t* w;                    // gemm_q4_pack's tiles
+  void* out; int ldo; bool out_f32;    // [M, N]
+  const bf16* r; int ldr;              // optional residual [M, N]
+  const bf16* bias;                    // optional [N]
+  int M, N, K;
+};
+cudaError_t gemm_q4(cudaStream_t stream, const GemmQ4Args& a);
+cudaError_t gemm_q4_pack(cudaStream_t stream, const void* blocks, void* out, int N, int K);
+size_t gemm_q4_bytes(int N, int K);
+
 // ---- decode-step GEMM (M <= 256): swap-AB + deterministic stream-K, fp32 partial slabs ----
 struct SkinnyPlan {
   int grid;                  // CTAs (== SMs unless the problem is tiny)

@@ -96,6 +96,54 @@ int hbk_attn_decode(const void* q, int ldq, const void* k_cache, const void* v_c
                     int D, int page_size, int num_splits, float scale, int num_pages);
 size_t hbk_attn_decode_workspace_floats(int B, int Hq, int D, int num_splits);
 
+/* ---- a step whose cache and weights are held in 4 bits.  32 neighbouring entries share a scale d and a code c in 0..15 stands for d (c - 8); with m the
+ * entry of largest magnitude (the first of equals) d = m / -8 rounded, c = clamp(floor(x / d + 1/2) + 8, 0, 15), 8 where d = 0.  These calls take the
+ * stream they run on (NULL: the legacy default stream), allocate nothing, never wait, and can be captured into a graph; a call's buffers must be on the
+ * current device.  Row strides count entries and are multiples of 8, rows of bf16 read in whole begin on 16 bytes.
+ *
+ * Page tables, slot maps and packed-row indices from lengths, in one launch.  Request b has ctx_lens[b] cached positions in the first ceil(ctx / 64) pages of
+ * its row of page_table [B][max_pages].  new_lens[b] >= 0: it has that many more tokens in this step and takes the pages that they need from the top
+ * of the stack free_pages[0 .. *free_count), in request order; new_lens[b] < 0: it has ended, its pages go on top of the stack first.
+ * Out: the new entries of page_table; the stack and its height *free_left; cu_seqlens [B + 1], rows of the packed batch (capped at T); kv_lens [B] = ctx + new,
+ * 0 for a request that has ended; positions [T] and slot_mapping [T] (page * 64 + place), 0 and -1 behind the last token.
+ * A request that does not fit (more than max_pages pages, rows past T, or the first that finds too few pages and every later one that needs some) takes no page:
+ * kv_lens[b] = ctx_lens[b] says so, and its rows have slot -1.  free_left may be free_count and kv_lens may be ctx_lens; nothing else may overlap.
+ * free_pages has room for num_pages entries.  1 <= B <= 2048, page_size 64.  Lengths below 0 in ctx_lens count as 0. */
+int hbk_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int max_pages, int32_t* free_pages,
+                    const int32_t* free_count, int32_t* free_left, int num_pages, int32_t* cu_seqlens, int32_t* kv_lens, int32_t* positions,
+                    int32_t* slot_mapping, int T, int page_size, void* stream);
+/* A 4-bit cache plane (one of K, one of V): [num_pages][Hkv][block], block = 64 rows of D / 2 bytes of codes, then 64 rows of D / 32 bf16 scales (D 64 or 128).
+ * K codes: position p's row at p D / 2; word j (4 bytes) of its quarter t (D / 8 bytes) holds entries 32 j + 8 t + i, i = 0..7, even i in nibble i / 2, odd i in
+ * nibble 4 + i / 2.  V codes: positions 2 n and 2 n + 1 share the D bytes at n D; chunk g (D / 8 bytes, at place g ^ 2 (n mod 4) for D = 128, g ^ 4 (n / 2 mod 2) for
+ * D = 64) holds in word j entries 32 j + 4 g + r, r = 0..3, of the even position in nibble r, of the odd one in nibble 4 + r. */
+size_t hbk_kv_q4_plane_bytes(int num_pages, int Hkv, int D); /* 0: refused sizes */
+/* Rows k, v [T][>= Hkv * D] (bf16, k rotated) into the planes at slot_mapping [T] (a slot that is none, -1 say: the row is not stored; no slot may occur twice).
+ * k_seen / v_seen (or NULL; may be k / v): the rows as the cache now stands for them, rounded to bf16: what a prompt's own attention reads
+ * if it shall see what later steps will.  A group with an infinity or a NaN reads as NaN. */
+int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_t* slot_mapping, void* k_cache, void* v_cache, void* k_seen, int ldks,
+                    void* v_seen, int ldvs, int T, int Hkv, int D, int page_size, int num_pages, void* stream);
+/* Attention over such planes: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q are the last positions of the kv_lens[b]-long sequence b (at most max_q_len of them;
+ * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv.  window, softcap and sink as in
+ * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
+ * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  split_pages: pages that one block reads of a
+ * sequence, counted from position 0 (a row's bits depend on its sequence and on it alone); 0: hbk_attn_paged_q4_split's.  workspace: as many floats as
+ * hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL); launches that may run at the same time need one each. */
+int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
+                      const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
+                      int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream);
+/* pages per block by the rule for `sms` SMs (0: the current device's); host arithmetic, -1 for refused sizes */
+int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
+size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
+/* 4-bit weights: N rows of K / 32 GGUF Q4_0 blocks (18 bytes: fp16 d, then byte i with entries i and i + 16; device memory) laid out as the product reads them, in
+ * hbk_gemm_q4_bytes(N, K) bytes (K a multiple of 32): tiles [ceil(N / 16)][ceil(K / 128)] of 16 rows of 64 bytes as K codes above with D = 128, then
+ * [16 rows][4 groups] fp16 scales. */
+size_t hbk_gemm_q4_bytes(int N, int K); /* 0: refused sizes */
+int hbk_gemm_q4_pack(const void* blocks, void* packed, int N, int K, void* stream);
+/* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 64 rows hbk_gemm with bf16 weights is quicker); epi as in hbk_gemm: 0, 1, 3, 4
+ * (bf16 out) or 6 (fp32 out); R may be out itself */
+int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, const void* R, int ldr, const void* bias, int M, int N, int K, int epi,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
