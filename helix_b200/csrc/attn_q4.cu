@@ -4,13 +4,16 @@
 //
 // The columns of a block are (row, query head) pairs of one kv head, eight per product: S^T[16 positions x 8 columns] = K q^T and
 // O^T[16 entries x 8 columns] += V^T P^T as warp-wide 16 x 8 x 16 products.  Both operands that come from the cache are then the 16-row one, the
-// codes go straight from their words to its registers as the integers c - 8 (fp16, exact), and no cached byte passes through shared memory twice.
-// The tensor-memory path would need the widened entries in shared memory: four times the cache's bytes written there and read again.
-//   S: the products of a group of 32 entries are summed as integers times q, then times the key group's scale in fp32.
-//   O: the value group's scale depends on the position, which is summed over: it goes into P^T, one operand per group, rounded to fp16 once
-//      (bf16 would add as much error as the output's own rounding).  A group's scales are brought near 1 by a power of two that follows
-//      their largest finite one so far, as the running maximum does for the scores: what falls below 2^-36 of a sequence's largest
-//      weight of that group is lost, and only there fp16's range is felt.
+// codes go straight from their words to its registers, and no cached byte passes through shared memory twice.  The tensor-memory path would need
+// the widened entries in shared memory: four times the cache's bytes written there and read again.
+// Instructions bound it (HBM gives a position of a kv head of 128 entries 25 issue slots), the products least of all.
+//   c - 8 is exact in fp16.  (Codes as they are, numbers below fp16's smallest normal one, with the 8 taken off by a further product, save four
+//      of nine instructions per word, but such products are summed to some 14 bits only: results whose codes are near 8 were off by 2^-15 of a group's weight.)
+//   S: the products of a group of 32 entries are summed by themselves, then times the key group's scale in fp32.
+//   O: the value group's scale depends on the position, which is summed over: it goes into P^T, one operand per group, fp16 (bf16 would add as much
+//      error as the output's own rounding; here two roundings of at most 2^-11 each).  A group's scales are brought near 1 by a power of two that
+//      follows their largest finite one so far, as the running maximum does for the scores: what falls below 2^-36 of a sequence's
+//      largest weight of that group is lost, and only there fp16's range is felt.
 //   q: fp16 after a power of two per column (bf16 has fewer bits; entries 2^-27 of the column's largest and below lose some).
 // Softmax statistics and sums are fp32.  A warp takes every fourth page of the block's share by itself; the four meet at the end.
 //
@@ -20,6 +23,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kernels.h"
 #include "launch.h"
@@ -108,7 +112,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* p, float (&s)[D / 32]
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(const AttnQ4Args a) {
   using C = Cfg<D, NT>;
   constexpr int J = C::J;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -133,31 +137,41 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
 
   uint8_t* ring = smem + warp * (STAGES * 2 * C::BLOCK);
   const int32_t* table = a.page_table + (size_t)b * a.max_pages;
-  const size_t block0 = (size_t)kvh * C::BLOCK, page_stride = (size_t)a.Hkv * C::BLOCK;
-  auto page_of = [&](int p) {  // a page number that is none: its positions are not seen
-    const int id = table[p];
-    return id >= 0 && id < a.num_pages ? id : -1;
+  const size_t block0 = (size_t)kvh * C::BLOCK + lane * 16, page_stride = (size_t)a.Hkv * C::BLOCK;
+  // the warp's pages are p_begin + warp + 4 i; lane i % 32 holds the number of page i, -1 for one that is none: its positions are not seen
+  const int n_mine = (p_end - p_begin - warp + kWarps - 1) / kWarps;
+  int ids = -1;
+  auto look_up = [&](int i) {
+    ids = -1;
+    if (i + lane < n_mine) {
+      const int id = table[p_begin + warp + kWarps * (i + lane)];
+      if (id >= 0 && id < a.num_pages) ids = id;
+    }
   };
-  auto fetch = [&](int p, int stage) {
-    if (p < p_end) {
-      const int id = page_of(p);
-      if (id >= 0) {
-        const size_t at = (size_t)id * page_stride + block0;
-        uint8_t* dst = ring + stage * 2 * C::BLOCK;
-        for (int i = lane; i < C::BLOCK / 16; i += 32) {
-          copy16(dst + i * 16, a.k_cache + at + i * 16);
-          copy16(dst + C::BLOCK + i * 16, a.v_cache + at + i * 16);
-        }
-      }
+  auto fetch = [&](int i, int stage) {  // all lanes; returns the page's number
+    if ((i & 31) == 0) look_up(i);
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    if (i < n_mine && id >= 0) {
+      const uint8_t *k = a.k_cache + (size_t)id * page_stride + block0, *v = a.v_cache + (size_t)id * page_stride + block0;
+      uint8_t* dst = ring + stage * 2 * C::BLOCK + lane * 16;
+#pragma unroll
+      for (int c = 0; c < C::BLOCK; c += 512)
+        if (c + 512 <= C::BLOCK || c + lane * 16 < C::BLOCK) copy16(dst + c, k + c);
+      copy_commit();
+#pragma unroll
+      for (int c = 0; c < C::BLOCK; c += 512)
+        if (c + 512 <= C::BLOCK || c + lane * 16 < C::BLOCK) copy16(dst + C::BLOCK + c, v + c);
+    } else {
+      copy_commit();
     }
     copy_commit();
+    return i < n_mine ? id : -1;
   };
-  fetch(p_begin + warp, 0);
+  int id = fetch(0, 0);
 
   // q as the 8-column operand: lane (g, t) holds entries 32 j + 8 t .. + 7 of column g
   uint32_t qr[NT][J][4];
-  float f_in[NT][2];          // scale (and log2 e) of the lane's two columns 2 t, 2 t + 1
-  int first[NT][2], last[NT][2];  // positions they see: first <= j <= last
+  float mul[NT][2];               // what brings a column's sums to log2 of its weights (to scores, where they are capped)
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int c = n * 8 + g;
@@ -185,30 +199,34 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
     mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
     // the largest becomes [2^10, 2^11): exponent field e -> factor 2^(137 - e), kept a normal number at both ends
     const int e = max((int)(mag >> 7), 20);
-    const float up = __uint_as_float((uint32_t)(264 - e) << 23);
-    const float down = __uint_as_float((uint32_t)(e - 10) << 23);
+    const float up = __uint_as_float((uint32_t)(264 - e) << 23), down = __uint_as_float((uint32_t)(e - 10) << 23);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) qr[n][j][i] = q4::pack_f16x2(q4::bf16_lo(w[i]) * up, q4::bf16_hi(w[i]) * up);
     }
+    // the sign of the scale goes into q, so that the largest sum is the largest score
+    const float scale = a.softcap > 0.f ? fabsf(a.scale) : fabsf(a.scale) * kLog2e;
+    if (a.scale < 0.f) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f_in[n][i] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + i)) * a.scale;
-      const int col = n * 8 + 2 * t + i;
-      last[n][i] = col < tile.cols ? tile.pos0 + (tile.col0 + col) / G : -1;
-      first[n][i] = a.window > 0 ? last[n][i] - a.window + 1 : 0;
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qr[n][j][i] ^= 0x80008000u;
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      mul[n][i] = fmaxf(__shfl_sync(0xffffffffu, down, 4 * (2 * t + i)) * scale, 1e-37f);  // (a scale of 0 still leaves what is not seen at -inf)
   }
-  const float cap_in = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
+  auto last_of = [&](int c) { return c < tile.cols ? tile.pos0 + (tile.col0 + c) / G : -1; };  // positions a column sees: first_of <= j <= last_of
+  auto first_of = [&](int last) { return a.window > 0 ? last - a.window + 1 : 0; };
   // every column sees a page whole that lies in [all_lo, all_hi]
   const int all_hi = tile.pos0 + tile.col0 / G;
   const int all_lo = a.window > 0 ? tile.pos0 + (tile.col0 + tile.cols - 1) / G - a.window + 1 : 0;
 
   float o[J][2][NT][4];
-  float m[NT][2], l[NT][2];
-  int ex[J];  // exponent field of a value group's largest scale so far
+  float m[NT][2], l[NT][2];  // running maximum (log2 of a weight) and sum of weights times 16
+  int ex[J];                 // exponent field of a value group's largest scale so far
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     ex[j] = 12;
@@ -227,180 +245,197 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
       l[n][i] = 0.f;
     }
 
-  int stage = 0;
-  for (int p = p_begin + warp; p < p_end; p += kWarps, stage ^= 1) {
-    fetch(p + kWarps, stage ^ 1);
-    copy_wait<1>();
-    __syncwarp();
-    if (page_of(p) >= 0) {
-      const uint8_t* kb = ring + stage * 2 * C::BLOCK;
-      const uint8_t* vb = kb + C::BLOCK;
-      const int pos = p * PAGE;
-      const bool whole = pos >= all_lo && pos + PAGE - 1 <= all_hi;
-
-      // scores
-      float s[4][NT][4];
+  // One page; `whole`: every column sees all of it
+  auto page = [&](uint8_t* kb, const int pos, auto whole_t) {
+    constexpr bool whole = decltype(whole_t)::value;
+    uint8_t* vb = kb + C::BLOCK;
+    float s[4][NT][4];
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk) {
-        const int r0 = blk * 16 + g;
-        uint32_t k0[J], k1[J];
-        float d0[J], d1[J];
-        load_words<D>(kb + r0 * (D / 2) + t * (D / 8), k0);
-        load_words<D>(kb + (r0 + 8) * (D / 2) + t * (D / 8), k1);
-        load_scales<D>(kb + q4::code_bytes(D) + r0 * J * 2, d0);
-        load_scales<D>(kb + q4::code_bytes(D) + (r0 + 8) * J * 2, d1);
+    for (int blk = 0; blk < 4; ++blk) {
+      const int r0 = blk * 16 + g;
+      uint32_t k0[J], k1[J];
+      float d0[J], d1[J];
+      load_words<D>(kb + r0 * (D / 2) + t * (D / 8), k0);
+      load_words<D>(kb + (r0 + 8) * (D / 2) + t * (D / 8), k1);
+      load_scales<D>(kb + q4::code_bytes(D) + r0 * J * 2, d0);
+      load_scales<D>(kb + q4::code_bytes(D) + (r0 + 8) * J * 2, d1);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int j = 0; j < J; ++j) {
+        uint32_t a0[4], a1[4];
+        q4::codes_f16(k0[j], a0);
+        q4::codes_f16(k1[j], a1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[blk][n][i] = 0.f;
+        for (int n = 0; n < NT; ++n) {
+          float c[4];
+          q4::mma_f16_first(c, a0[0], a1[0], a0[1], a1[1], qr[n][j][0], qr[n][j][1]);
+          q4::mma_f16(c, a0[2], a1[2], a0[3], a1[3], qr[n][j][2], qr[n][j][3]);
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          uint32_t a0[4], a1[4];
-          q4::codes_f16(k0[j], a0);
-          q4::codes_f16(k1[j], a1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            q4::mma_f16(c, a0[0], a1[0], a0[1], a1[1], qr[n][j][0], qr[n][j][1]);
-            q4::mma_f16(c, a0[2], a1[2], a0[3], a1[3], qr[n][j][2], qr[n][j][3]);
-            s[blk][n][0] = fmaf(d0[j], c[0], s[blk][n][0]);
-            s[blk][n][1] = fmaf(d0[j], c[1], s[blk][n][1]);
-            s[blk][n][2] = fmaf(d1[j], c[2], s[blk][n][2]);
-            s[blk][n][3] = fmaf(d1[j], c[3], s[blk][n][3]);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[blk][n][i] * f_in[n][i & 1];
-            if (a.softcap > 0.f)  // cap tanh(x / cap) in the exp2 domain, tanh(y) = 1 - 2 / (e^2y + 1)
-              x = fmaf(-2.f * cap_out, __fdividef(1.f, exp2_fast(x * cap_in) + 1.f), cap_out);
-            else
-              x *= kLog2e;
-            if (!whole) {
-              const int at = pos + blk * 16 + g + 8 * (i >> 1);
-              if (at > last[n][i & 1] || at < first[n][i & 1]) x = -INFINITY;
-            }
-            s[blk][n][i] = x;
-          }
-      }
-      // running maximum
-      bool moved = false;
-      float up[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float x = m[n][i];
-#pragma unroll
-          for (int blk = 0; blk < 4; ++blk) x = fmaxf(x, fmaxf(s[blk][n][i], s[blk][n][i + 2]));
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-          up[n][i] = x > m[n][i] ? exp2_fast(m[n][i] - x) : 1.f;  // (-inf before: 0)
-          moved |= x > m[n][i];
-          m[n][i] = x;
-        }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            l[n][i] *= up[n][i];
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                o[j][h][n][i] *= up[n][i];
-                o[j][h][n][i + 2] *= up[n][i];
-              }
-          }
-      }
-      // the largest exponent of each value group's scales: a lane looks at positions 2 lane, 2 lane + 1
-      {
-        uint32_t w[J];  // J 16-bit scales of each of the two positions
-        load_words<D>(vb + q4::code_bytes(D) + lane * (J * 4), w);
-        const int at = pos + 2 * lane;
-        auto finite = [](uint32_t x) {  // halves that are infinities or NaN: 0 (they reach their columns through the weights)
-          return (x & 0xffffu) < 0x7f80u ? ((x >> 16) < 0x7f80u ? x : x & 0xffffu) : ((x >> 16) < 0x7f80u ? x & 0xffff0000u : 0u);
-        };
-#pragma unroll
-        for (int i = 0; i < J / 2; ++i) {
-          uint32_t x = 0, y = 0;
-          if (whole || (at >= tile.lo && at < tile.hi)) x = w[i] & 0x7fff7fffu;
-          if (whole || (at + 1 >= tile.lo && at + 1 < tile.hi)) y = w[J / 2 + i] & 0x7fff7fffu;
-          const uint32_t both = __vmaxu2(x, y);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int j = 2 * i + h;
-            uint32_t most = __reduce_max_sync(0xffffffffu, h ? both >> 16 : both & 0xffffu);
-            if (most >= 0x7f80u) {
-              const uint32_t z = __vmaxu2(finite(x), finite(y));
-              most = __reduce_max_sync(0xffffffffu, h ? z >> 16 : z & 0xffffu);
-            }
-            const int e = (int)(most >> 7);
-            if (e > ex[j]) {
-              const float dn = exp2f((float)(ex[j] - e));
-              ex[j] = e;
-#pragma unroll
-              for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int i2 = 0; i2 < 4; ++i2) o[j][q][n][i2] *= dn;
-            }
-          }
-        }
-      }
-      // weights and sums
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float mm = m[n][i] == -INFINITY ? 0.f : m[n][i];
-#pragma unroll
-          for (int blk = 0; blk < 4; ++blk)
-#pragma unroll
-            for (int h = 0; h < 4; h += 2) {
-              s[blk][n][i + h] = exp2_fast(s[blk][n][i + h] - mm);
-              l[n][i] += s[blk][n][i + h];
-            }
-        }
-#pragma unroll
-      for (int blk = 0; blk < 4; ++blk) {
-        const int r0 = blk * 16 + g, pair = blk * 8 + t;
-        uint32_t v0[J], v1[J];
-        float d0[J], d1[J];
-        load_words<D>(vb + pair * D + (g ^ q4::place_xor(D, pair)) * (D / 8), v0);
-        load_words<D>(vb + (pair + 4) * D + (g ^ q4::place_xor(D, pair + 4)) * (D / 8), v1);
-        load_scales<D>(vb + q4::code_bytes(D) + r0 * J * 2, d0);
-        load_scales<D>(vb + q4::code_bytes(D) + (r0 + 8) * J * 2, d1);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const float near1 = __uint_as_float((uint32_t)(265 - ex[j]) << 23);  // 2^(138 - ex): the largest scale becomes [2^11, 2^12)
-          const float e0 = d0[j] * near1, e1 = d1[j] * near1;
-          uint32_t a0[4], a1[4];
-          q4::codes_f16(v0[j], a0);
-          q4::codes_f16(v1[j], a1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              w[i] = s[blk][n][i] * (i < 2 ? e0 : e1);
-              if (!whole) {  // what a column does not see has no part in it, whatever its bytes say
-                const int at = pos + r0 + 8 * (i >> 1);
-                if (at > last[n][i & 1] || at < first[n][i & 1]) w[i] = 0.f;
-              }
-            }
-            const uint32_t b0 = q4::transpose8(q4::pack_f16x2(w[0], w[1])), b1 = q4::transpose8(q4::pack_f16x2(w[2], w[3]));
-            q4::mma_f16(o[j][0][n], a0[0], a0[1], a1[0], a1[1], b0, b1);
-            q4::mma_f16(o[j][1][n], a0[2], a0[3], a1[2], a1[3], b0, b1);
-          }
+          for (int i = 0; i < 4; ++i) s[blk][n][i] = j == 0 ? (i < 2 ? d0 : d1)[j] * c[i] : fmaf((i < 2 ? d0 : d1)[j], c[i], s[blk][n][i]);
         }
       }
     }
+    if (a.softcap > 0.f) {  // cap tanh(x / cap) as log2 of a weight, tanh(y) = 1 - 2 / (e^2y + 1)
+      const float in = 2.f * kLog2e / a.softcap, out = a.softcap * kLog2e;
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[blk][n][i] = fmaf(-2.f * out, __fdividef(1.f, exp2_fast(s[blk][n][i] * mul[n][i & 1] * in) + 1.f), out);
+    }
+    if constexpr (!whole) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int hi = last_of(n * 8 + 2 * t + i), lo = first_of(hi);
+#pragma unroll
+          for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int at = pos + blk * 16 + g + 8 * h;
+              if (at > hi || at < lo) s[blk][n][i + 2 * h] = -INFINITY;
+            }
+        }
+    }
+    // running maximum
+    bool moved = false;
+    float keep[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = fmaxf(s[0][n][i], s[0][n][i + 2]);
+#pragma unroll
+        for (int blk = 1; blk < 4; ++blk) x = fmaxf(x, fmaxf(s[blk][n][i], s[blk][n][i + 2]));
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+        if (!(a.softcap > 0.f)) x *= mul[n][i];
+        keep[n][i] = x > m[n][i] ? exp2_fast(m[n][i] - x) : 1.f;  // (-inf before: 0)
+        moved |= x > m[n][i];
+        m[n][i] = fmaxf(m[n][i], x);
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l[n][i] *= keep[n][i];
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              o[j][h][n][i] *= keep[n][i];
+              o[j][h][n][i + 2] *= keep[n][i];
+            }
+        }
+    }
+    // value scales: a lane takes those of positions 2 lane and 2 lane + 1, follows each group's largest exponent, and puts them back as
+    // fp16 pairs of the two positions with the largest in [2^10, 2^11)
+    {
+      uint32_t w[J];
+      uint8_t* mine = vb + q4::code_bytes(D) + lane * (J * 4);
+      load_words<D>(mine, w);
+      const int at = pos + 2 * lane;
+      auto finite = [](uint32_t x) {  // halves that are infinities or NaN: 0 (they reach their columns through the weights)
+        return (x & 0xffffu) < 0x7f80u ? ((x >> 16) < 0x7f80u ? x : x & 0xffffu) : ((x >> 16) < 0x7f80u ? x & 0xffff0000u : 0u);
+      };
+      uint32_t pair[J];
+#pragma unroll
+      for (int i = 0; i < J / 2; ++i) {
+        uint32_t x = 0, y = 0;
+        if (whole || (at >= tile.lo && at < tile.hi)) x = w[i] & 0x7fff7fffu;
+        if (whole || (at + 1 >= tile.lo && at + 1 < tile.hi)) y = w[J / 2 + i] & 0x7fff7fffu;
+        const uint32_t both = __vmaxu2(x, y);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = 2 * i + h;
+          uint32_t most = __reduce_max_sync(0xffffffffu, h ? both >> 16 : both & 0xffffu);
+          if (most >= 0x7f80u) {
+            const uint32_t z = __vmaxu2(finite(x), finite(y));
+            most = __reduce_max_sync(0xffffffffu, h ? z >> 16 : z & 0xffffu);
+          }
+          const int e = (int)(most >> 7);
+          if (e > ex[j]) {
+            const float less = exp2f((float)(ex[j] - e));
+            ex[j] = e;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[j][q][n][k] *= less;
+          }
+          const float near1 = __uint_as_float((uint32_t)(264 - ex[j]) << 23);  // 2^(137 - ex)
+          pair[j] = q4::pack_f16x2((h ? q4::bf16_hi(w[i]) : q4::bf16_lo(w[i])) * near1, (h ? q4::bf16_hi(w[J / 2 + i]) : q4::bf16_lo(w[J / 2 + i])) * near1);
+        }
+      }
+      if constexpr (J == 4) *reinterpret_cast<uint4*>(mine) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+      else *reinterpret_cast<uint2*>(mine) = make_uint2(pair[0], pair[1]);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) {
+      const int p0 = blk * 8 + t;
+      uint32_t v0[J], v1[J], s0[J], s1[J], b0[NT], b1[NT];
+      load_words<D>(vb + p0 * D + (g ^ q4::place_xor(D, p0)) * (D / 8), v0);
+      load_words<D>(vb + (p0 + 4) * D + (g ^ q4::place_xor(D, p0 + 4)) * (D / 8), v1);
+      load_words<D>(vb + q4::code_bytes(D) + p0 * (J * 4), s0);
+      load_words<D>(vb + q4::code_bytes(D) + (p0 + 4) * (J * 4), s1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float base = 4.f - (m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1]);  // weights times 16: fp16 holds them better
+          w[i] = exp2_fast(a.softcap > 0.f ? s[blk][n][i] + base : fmaf(s[blk][n][i], mul[n][i & 1], base));
+          l[n][i & 1] += w[i];
+        }
+        b0[n] = q4::transpose8(q4::pack_f16x2(w[0], w[1]));
+        b1[n] = q4::transpose8(q4::pack_f16x2(w[2], w[3]));
+      }
+      uint32_t see0[NT], see1[NT];  // what a column does not see has no part in it, whatever its bytes say
+      if constexpr (!whole) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int hi = last_of(n * 8 + g), lo = first_of(hi);
+          auto seen = [&](int at) { return (at >= lo && at <= hi ? 0xffffu : 0u) | (at + 1 >= lo && at + 1 <= hi ? 0xffff0000u : 0u); };
+          see0[n] = seen(pos + 2 * p0);
+          see1[n] = seen(pos + 2 * p0 + 8);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        uint32_t a0[4], a1[4];
+        q4::codes_f16(v0[j], a0);
+        q4::codes_f16(v1[j], a1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t w0 = q4::hmul2(b0[n], s0[j]), w1 = q4::hmul2(b1[n], s1[j]);
+          if constexpr (!whole) {
+            w0 &= see0[n];
+            w1 &= see1[n];
+          }
+          q4::mma_f16(o[j][0][n], a0[0], a0[1], a1[0], a1[1], w0, w1);
+          q4::mma_f16(o[j][1][n], a0[2], a0[3], a1[2], a1[3], w0, w1);
+        }
+      }
+    }
+  };
+
+  for (int i = 0; i < n_mine; ++i) {
+    const int next = fetch(i + 1, (i + 1) & 1);
+    copy_wait<2>();
+    __syncwarp();
+    if (id >= 0) {
+      uint8_t* kb = ring + (i & 1) * 2 * C::BLOCK;
+      const int pos = (p_begin + warp + kWarps * i) * PAGE;
+      if (pos >= all_lo && pos + PAGE - 1 <= all_hi) page(kb, pos, std::true_type{});
+      else page(kb, pos, std::false_type{});
+    }
     __syncwarp();  // the stage is free for the fetch after next
+    id = next;
   }
   copy_wait<0>();
   __syncthreads();
@@ -418,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
       for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const float back = __uint_as_float((uint32_t)(ex[j] - 11) << 23);  // 2^(ex - 138)
+        const float back = __uint_as_float((uint32_t)(ex[j] - 10) << 23);  // 2^(ex - 137)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           dst[32 * j + 4 * g + 2 * h] = o[j][h][n][i] * back;
@@ -444,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_kernel(const AttnQ4Args a) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* src = sm + (size_t)(w * C::COLS + c) * (D + 2);
-      const float f = exp2_fast(src[D] - ref);
+      const float f = exp2_fast(src[D] - ref - 4.f);  // (sums are 16 times what they stand for)
       acc = fmaf(src[d], f, acc);
       sum = fmaf(src[D + 1], f, sum);
     }

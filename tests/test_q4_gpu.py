@@ -270,9 +270,10 @@ def cache(seed, lens, hkv, d, spread=1.0, spare=2, width=0):
 
 
 def check_attn(out, want, mass, hq, d):
-    """bf16 rounding of the result (2^-8 of it), fp16 rounding of the weights (2^-11 of the sum of p |v|) and as much again for all that is done in fp32."""
+    """bf16 rounding of the result (2^-8 of it); every weight is rounded to fp16 by itself and again times its value scale, each by 2^-11 of it at most, so
+    (1 + 2^-11)^2 - 1 < 2^-10 + 2^-21 of the sum of p |v|; 2^-12 of that sum for all that is done in fp32."""
     got = out[:, :hq * d].view(-1, hq, d).double()
-    off = (got - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -12) * mass + 1e-30)
+    off = (got - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -12) * mass + 1e-30)
     assert not torch.isnan(got).any() and (off <= 0).all(), (off.max().item(), (got - want).norm().item() / want.norm().item())
 
 
