@@ -284,7 +284,8 @@ struct AttnQ4Args {
   int num_pages, window;
   float softcap;
   const bf16* sink;                    // [Hq] or NULL
-  int max_splits, kv_bound;            // filled in by the launcher
+  int max_splits, kv_bound, group;     // filled in by the launcher
+  unsigned long long inv_group;
 };
 cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a);
 int attn_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);

@@ -123,11 +123,11 @@ size_t hbk_kv_q4_plane_bytes(int num_pages, int Hkv, int D); /* 0: refused sizes
 int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_t* slot_mapping, void* k_cache, void* v_cache, void* k_seen, int ldks,
                     void* v_seen, int ldvs, int T, int Hkv, int D, int page_size, int num_pages, void* stream);
 /* Attention over such planes: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q are the last positions of the kv_lens[b]-long sequence b (at most max_q_len of them;
- * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv.  window, softcap and sink as in
+ * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096.  window, softcap and sink as in
  * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
- * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  split_pages: pages that one block reads of a
- * sequence, counted from position 0 (a row's bits depend on its sequence and on it alone); 0: hbk_attn_paged_q4_split's.  workspace: as many floats as
- * hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL); launches that may run at the same time need one each. */
+ * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  split_pages: pages that one block
+ * reads of a sequence at most (a row's bits depend on its sequence and on it alone); 0: hbk_attn_paged_q4_split's.  workspace: as many floats as
+ * hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL; on 16 bytes); launches that may run at the same time need one each. */
 int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
                       const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
                       int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream);

@@ -44,7 +44,7 @@ def attn(q=OK, ldq=1024, kc=OK, vc=OK, table=OK, max_pages=8, kv=OK, cu=OK, out=
                                 dict(vc=OK + 2), dict(ldq=1016), dict(ldq=1028), dict(ldo=1016), dict(out=OK + 1), dict(B=0), dict(B=65536), dict(T=-1), dict(most=0), dict(longest=-1),
                                 dict(hq=7), dict(hkv=0), dict(hkv=3), dict(d=32), dict(d=256), dict(page=128), dict(split=-1), dict(split=2 ** 25), dict(pages=0),
                                 dict(pages=2 ** 26), dict(max_pages=-1), dict(window=-1), dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("nan")), dict(cu=None, T=3),
-                                dict(cu=None, most=2), dict(hq=2 ** 20, hkv=2 ** 20, ldq=2 ** 27, ldo=2 ** 27)])
+                                dict(cu=None, most=2), dict(hq=2 ** 20, hkv=2 ** 20, ldq=2 ** 27, ldo=2 ** 27), dict(hq=4097, hkv=1, ldq=2 ** 20, ldo=2 ** 20), dict(work=OK + 4)])
 def test_attention_refusals(kw):
     assert attn(**kw) == 1
 
@@ -77,19 +77,19 @@ def test_sizes():
                                                          (3, 97, 5000, 12, 2, 0), (1, 300, 70000, 9, 3, 100), (65535, 1, 100, 8, 8, 0), (1, 1, 0, 8, 8, 0)])
 def test_shares_cover_what_is_seen_and_fit_the_workspace(B, most, longest, hq, hkv, window):
     split = L.hbk_attn_paged_q4_split(B, most, longest, hq, hkv, window, 148)
-    assert split >= 4 and split % 4 == 0
     group = hq // hkv
     cols = 16 if group * most > 8 else 8
+    assert 4 <= split <= 40
     n = L.hbk_attn_paged_q4_workspace_floats(B, B * most, most, longest, hq, hkv, 128, split, window)
-    shares = n // (B * most * hq * 130) if n else 1
-    assert n == (0 if shares == 1 else B * most * hq * 130 * shares)
+    shares = n // (B * most * hq * 132) if n else 1
+    assert n == (0 if shares == 1 else B * most * hq * 132 * shares)
     for length in {longest, longest - 1, longest // 2, 65 % (longest + 1), min(longest, split * 64 + 1)}:
         for c0 in range(0, group * most, cols):
             first, last = c0 // group, (min(c0 + cols, group * most) - 1) // group
             hi = max(length - most + last + 1, 0)
             lo = max(length - most + first - window + 1, 0) if window else 0
             if hi > lo:
-                assert (-(-hi // 64) + split - 1) // split - lo // 64 // split <= shares
+                assert -(-(-(-hi // 64) - lo // 64) // split) <= shares
 
 
 def test_split_refusals():
