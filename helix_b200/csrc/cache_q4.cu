@@ -16,52 +16,82 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Eight entries and their group's scale: the eight codes as bytes of two words (entry i in byte i), the scale, and the entries as the cache stands for them
 struct Coded {
-  uint32_t code[8];
+  uint32_t lo, hi;
   bf16 scale;
 };
 
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {  // NaN if either is
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float add_down(float a, float b) {
+  float r;
+  asm("add.rz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // All four lanes of a group call it with their eight entries
-__device__ __forceinline__ Coded encode(const uint4 raw, int quarter) {
+template <bool SEEN>
+__device__ __forceinline__ Coded encode(const uint4 raw, int quarter, uint4& seen) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  // magnitude | 31 - place | sign: the largest key names the first entry of largest magnitude (an entry's 15 magnitude bits order as integers)
-  uint32_t key = 0;
+  // the largest of the entries and of their negatives, as two halves
+  const uint32_t p = max_bf16x2(max_bf16x2(w[0], w[1]), max_bf16x2(w[2], w[3]));
+  const uint32_t q = max_bf16x2(max_bf16x2(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), max_bf16x2(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+  uint32_t pq = max_bf16x2(__byte_perm(p, q, 0x5410), __byte_perm(p, q, 0x7632));
+  pq = max_bf16x2(pq, __shfl_xor_sync(0xffffffffu, pq, 1));
+  pq = max_bf16x2(pq, __shfl_xor_sync(0xffffffffu, pq, 2));
+  const float up = __uint_as_float(pq << 16), dn = __uint_as_float(pq & 0xffff0000u);
+  float m = up > dn ? up : -dn;
+  if (up == dn) {  // both signs reach it (or all is zero): the first entry says which; the other lanes of the group are here too
+    uint32_t key = 0;  // 31 - place | sign
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-    key = max(key, (u & 0x7fffu) << 6 | (uint32_t)(31 - 8 * quarter - i) << 1 | u >> 15);
+    for (int i = 7; i >= 0; --i) {
+      const uint32_t u = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+      if ((u & 0x7fffu) == (pq & 0x7fffu)) key = (uint32_t)(31 - 8 * quarter - i) << 1 | u >> 15;
+    }
+    const uint32_t four = 0xfu << (threadIdx.x & 28);
+    key = max(key, __shfl_xor_sync(four, key, 1));
+    key = max(key, __shfl_xor_sync(four, key, 2));
+    m = key & 1 ? -up : up;
   }
-  key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
-  key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
-  const uint32_t mag = key >> 6;
-  const float m = __uint_as_float(mag << 16 | (key & 1u) << 31);
   Coded c;
   c.scale = __float2bfloat16(m * -0.125f);
   const float d = __bfloat162float(c.scale);
   // x / d as x (1 / d).  With eight bits each, a quotient that is no half integer is at least 2^-9 from one, while product and sum are off by less
-  // than 2^-18: 2^-16 more puts every half integer itself on its upper side and moves nothing else.  1 / d of a tiny d would overflow: both are raised first.
-  const float up = fabsf(d) < 1e-30f ? 1.8446744e19f : 1.f;  // 2^64
-  const float inv = 1.f / (d * up);
-  const bool zero = d == 0.f;
+  // than 2^-18: 2^-16 more puts every half integer itself on its upper side and moves nothing else.  1 / d of a tiny d would overflow: both are
+  // raised first.  x / d + 8.5 is above 0 where the scale is rounded by 2^-8 at most, so that only subnormal ones need the lower end; adding 2^23
+  // towards zero leaves the whole part in the low bits.
+  const bool tiny = fabsf(d) < 1e-30f;
+  const float raise = tiny ? 1.8446744e19f : 1.f;  // 2^64
+  const float inv = 1.f / (d * raise);
+  uint32_t b[8];
+  float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t u = (w[i >> 1] >> (16 * (i & 1))) << 16;
-    const float x = __uint_as_float(u) * up;
-    const float f = fminf(fmaxf(floorf(fmaf(x, inv, 8.5f + 1.52587890625e-5f)), 0.f), 15.f);
-    c.code[i] = zero ? 8u : (uint32_t)f;
+    float x = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    if (tiny) x *= raise;
+    float f = fminf(fmaf(x, inv, 8.5f + 1.52587890625e-5f), 15.5f);
+    if (tiny) f = fmaxf(f, 0.f);
+    f = add_down(f, 8388608.f);
+    b[i] = __float_as_uint(f);
+    if (SEEN) y[i] = (f - 8388616.f) * d;
   }
-  if (mag >= 0x7f80u) c.scale = __ushort_as_bfloat16(0x7fffu);
+  c.lo = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  c.hi = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+  if (SEEN) seen = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+  const bool none = !(fabsf(m) < INFINITY);
+  if (d == 0.f || none) {
+    c.lo = c.hi = 0x08080808u;
+    if (SEEN) seen = none ? make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu) : make_uint4(0, 0, 0, 0);
+    if (none) c.scale = __ushort_as_bfloat16(0x7fffu);
+  }
   return c;
 }
-__device__ __forceinline__ uint4 decoded(const Coded& c) {
-  const float d = __bfloat162float(c.scale);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(d * (float)((int)c.code[2 * i] - 8), d * (float)((int)c.code[2 * i + 1] - 8));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
-template <int D>
+template <int D, bool SEEN>
 __global__ void __launch_bounds__(kThreads) kv_write_q4_kernel(const CacheWriteQ4Args a) {
   constexpr int LANES = D / 8, J = D / q4::kGroup, PART = D / 8;  // threads per row, groups, bytes of a quarter or chunk
   pdl_wait();
@@ -76,30 +106,33 @@ __global__ void __launch_bounds__(kThreads) kv_write_q4_kernel(const CacheWriteQ
   const uint4 kraw = *reinterpret_cast<const uint4*>(a.k + (size_t)t * a.ldk + col);
   const uint4 vraw = *reinterpret_cast<const uint4*>(a.v + (size_t)t * a.ldv + col);
   const int slot = a.slots[t];
-  const Coded k = encode(kraw, quarter), v = encode(vraw, quarter);
+  uint4 k_seen, v_seen;
+  const Coded k = encode<SEEN>(kraw, quarter, k_seen), v = encode<SEEN>(vraw, quarter, v_seen);
   if (!live) return;
   if (slot >= 0 && slot < a.num_pages * q4::kPage) {
     const int page = slot / q4::kPage, pos = slot % q4::kPage;
     const size_t block = ((size_t)page * a.Hkv + h) * q4::block_bytes(D);
-    uint32_t kw = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) kw |= k.code[i] << (4 * (i / 2 + 4 * (i & 1)));
-    *reinterpret_cast<uint32_t*>(a.k_cache + block + pos * (D / 2) + quarter * PART + j * 4) = kw;
+    // keys: even entries in nibbles 0..3, odd ones in 4..7
+    const uint32_t even = __byte_perm(k.lo, k.hi, 0x6420), odd = __byte_perm(k.lo, k.hi, 0x7531);
+    const uint32_t e2 = even | even >> 4, o2 = odd | odd >> 4;  // bytes 0 and 2: two codes each
+    *reinterpret_cast<uint32_t*>(a.k_cache + block + pos * (D / 2) + quarter * PART + j * 4) = __byte_perm(e2, o2, 0x6420);
+    // values: entries 4 c + r in nibble r
+    const uint32_t v2 = v.lo | v.lo >> 4, v3 = v.hi | v.hi >> 4;
     const int pair = pos >> 1;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int place = (2 * quarter + c) ^ q4::place_xor(D, pair);
-      const uint32_t hw = v.code[4 * c] | v.code[4 * c + 1] << 4 | v.code[4 * c + 2] << 8 | v.code[4 * c + 3] << 12;
-      *reinterpret_cast<uint16_t*>(a.v_cache + block + pair * D + place * PART + j * 4 + (pos & 1) * 2) = (uint16_t)hw;
-    }
+    uint8_t* row = a.v_cache + block + pair * D + j * 4 + (pos & 1) * 2;
+    const int x = q4::place_xor(D, pair);
+    *reinterpret_cast<uint16_t*>(row + ((2 * quarter) ^ x) * PART) = (uint16_t)__byte_perm(v2, 0, 0x4420);
+    *reinterpret_cast<uint16_t*>(row + ((2 * quarter + 1) ^ x) * PART) = (uint16_t)__byte_perm(v3, 0, 0x4420);
     if (quarter == 0) {
       const size_t at = block + q4::code_bytes(D) + (pos * J + j) * 2;
       *reinterpret_cast<bf16*>(a.k_cache + at) = k.scale;
       *reinterpret_cast<bf16*>(a.v_cache + at) = v.scale;
     }
   }
-  if (a.k_seen) *reinterpret_cast<uint4*>(a.k_seen + (size_t)t * a.ldks + col) = decoded(k);
-  if (a.v_seen) *reinterpret_cast<uint4*>(a.v_seen + (size_t)t * a.ldvs + col) = decoded(v);
+  if (SEEN) {
+    if (a.k_seen) *reinterpret_cast<uint4*>(a.k_seen + (size_t)t * a.ldks + col) = k_seen;
+    if (a.v_seen) *reinterpret_cast<uint4*>(a.v_seen + (size_t)t * a.ldvs + col) = v_seen;
+  }
 }
 
 bool rows_ok(const void* p, int ld, int need) { return ((uintptr_t)p & 15) == 0 && ld >= need && ld % 8 == 0; }
@@ -120,7 +153,9 @@ cudaError_t kv_write_q4(cudaStream_t stream, const CacheWriteQ4Args& a) {
     return cudaErrorInvalidValue;
   const size_t blocks = ((size_t)a.T * a.Hkv * (a.D / 8) + kThreads - 1) / kThreads;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_k(a.D == 128 ? kv_write_q4_kernel<128> : kv_write_q4_kernel<64>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, true, a);
+  const bool seen = a.k_seen || a.v_seen;
+  return launch_k(a.D == 128 ? seen ? kv_write_q4_kernel<128, true> : kv_write_q4_kernel<128, false> : seen ? kv_write_q4_kernel<64, true> : kv_write_q4_kernel<64, false>,
+                  dim3((unsigned)blocks), dim3(kThreads), 0, stream, true, a);
 }
 
 }  // namespace hb
