@@ -26,7 +26,7 @@ def write(k=OK, ldk=256, v=OK, ldv=256, slots=OK, kc=OK, vc=OK, ks=None, ldks=0,
 
 @pytest.mark.parametrize("kw", [dict(k=None), dict(v=None), dict(slots=None), dict(kc=None), dict(vc=None), dict(k=OK + 2), dict(v=OK + 8), dict(kc=OK + 4), dict(vc=OK + 8),
                                 dict(ldk=248), dict(ldv=260), dict(ldk=0), dict(ks=OK, ldks=8), dict(vs=OK + 2, ldvs=256), dict(T=-1), dict(hkv=0), dict(d=96), dict(d=256),
-                                dict(page=16), dict(pages=0), dict(pages=2 ** 26), dict(T=2 ** 31 - 1, hkv=2 ** 20, ldk=2 ** 27, ldv=2 ** 27)])
+                                dict(page=16), dict(pages=0), dict(pages=2 ** 26), dict(hkv=65536, ldk=2 ** 23, ldv=2 ** 23)])
 def test_kv_write_refusals(kw):
     assert write(**kw) == 1
 
