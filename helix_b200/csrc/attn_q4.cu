@@ -11,9 +11,9 @@
 //      of nine instructions per word, but such products are summed to some 14 bits only: results whose codes are near 8 were off by 2^-15 of a group's weight.)
 //   S: the products of a group of 32 entries are summed by themselves, then times the key group's scale in fp32.
 //   O: the value group's scale depends on the position, which is summed over: it goes into P^T, one operand per group, fp16 (bf16 would add as much
-//      error as the output's own rounding; here two roundings of at most 2^-11 each).  A group's scales are brought near 1 by a power of two that
-//      follows their largest finite one so far, as the running maximum does for the scores: what falls below 2^-36 of a sequence's
-//      largest weight of that group is lost, and only there fp16's range is felt.
+//      error as the output's own rounding; here two roundings of at most 2^-11 each, and 2^-35 of the largest weight for weights far below it).  A
+//      group's scales are brought near 1 by a power of two that follows their largest finite one so far, as the running maximum does for the
+//      scores; scales below 2^-18 of that largest lose bits.
 //   q: fp16 after a power of two per column (bf16 has fewer bits; entries 2^-27 of the column's largest and below lose some).
 // Softmax statistics and sums are fp32.  A warp takes every fourth page of the block's share by itself; the four meet at the end.
 //
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
   const int all_hi = tile.pos0, all_lo = first_of(tile.pos0 + row_of(tile.cols - 1));
 
   float o[J][2][NT][4];
-  float m[NT][2], l[NT][2];  // running maximum (log2 of a weight) and sum of weights times 16
+  float m[NT][2], l[NT][2];  // running maximum (log2 of a weight) and sum of weights times 2^10
   int ex[J];                 // exponent field of a value group's largest scale so far
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
     copy_wait<2>();
     __syncwarp();
     // value scales: a lane takes those of positions 2 lane and 2 lane + 1, follows each group's largest exponent, and puts them back as
-    // fp16 pairs of the two positions with the largest in [2^10, 2^11)
+    // fp16 pairs of the two positions with the largest in [2^4, 2^5)
     {
       uint32_t w[J], pair[J];
       uint8_t* mine = vb + q4::code_bytes(D) + lane * (J * 4);
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const float near1 = __uint_as_float((uint32_t)(264 - ex[j]) << 23);  // 2^(137 - ex)
+        const float near1 = __uint_as_float((uint32_t)(258 - ex[j]) << 23);  // 2^(131 - ex)
         const uint32_t u = w[j / 2], v = w[J / 2 + j / 2];
         pair[j] = q4::pack_f16x2((j & 1 ? q4::bf16_hi(u) : q4::bf16_lo(u)) * near1, (j & 1 ? q4::bf16_hi(v) : q4::bf16_lo(v)) * near1);
       }
@@ -400,11 +400,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
       else *reinterpret_cast<uint2*>(mine) = make_uint2(pair[0], pair[1]);
       __syncwarp();
     }
-    float base[NT][2];  // weights times 16: fp16 holds them better
+    float base[NT][2];  // weights times 2^10: fp16 then holds them to 2^-35 of the largest, and their products with scales to 2^-40
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) base[n][h] = 4.f - (m[n][h] == -INFINITY ? 0.f : m[n][h]);
+      for (int h = 0; h < 2; ++h) base[n][h] = 10.f - (m[n][h] == -INFINITY ? 0.f : m[n][h]);
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
       const int p0 = blk * 8 + t;
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
       for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const float back = __uint_as_float((uint32_t)(ex[j] - 10) << 23);  // 2^(ex - 137)
+        const float back = __uint_as_float((uint32_t)(ex[j] - 4) << 23);  // 2^(ex - 131)
         *reinterpret_cast<float4*>(dst + 32 * j + 4 * g) = make_float4(o[j][0][n][i] * back, o[j][0][n][i + 2] * back, o[j][1][n][i] * back, o[j][1][n][i + 2] * back);
       }
       if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[n][i], sum);
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(sm + (w * C::COLS + c) * (D + 4) + d);
-      const float f = exp2_fast(ml[w].x - ref - 4.f);  // (sums are 16 times what they stand for)
+      const float f = exp2_fast(ml[w].x - ref - 10.f);  // (sums are 2^10 times what they stand for)
       acc = make_float4(fmaf(x.x, f, acc.x), fmaf(x.y, f, acc.y), fmaf(x.z, f, acc.z), fmaf(x.w, f, acc.w));
       sum = fmaf(ml[w].y, f, sum);
     }
@@ -665,7 +665,7 @@ size_t attn_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int
 
 cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   if (!sizes_ok(a.B, a.T, a.max_q_len, a.max_kv_len, a.Hq, a.Hkv, a.D, a.split_pages, a.window)) return cudaErrorInvalidValue;
-  if (a.page_size != PAGE || a.num_pages < 1 || a.num_pages > INT32_MAX / PAGE || a.max_pages < 0 || !(a.softcap >= 0.f) || !(a.scale == a.scale))
+  if (a.page_size != PAGE || a.num_pages < 1 || a.num_pages > INT32_MAX / PAGE || a.max_pages < 0 || !(a.softcap >= 0.f) || !(a.softcap < INFINITY) || !(fabsf(a.scale) < INFINITY))
     return cudaErrorInvalidValue;
   if (a.T == 0) return cudaSuccess;
   if (!a.q || !a.k_cache || !a.v_cache || !a.kv_lens || !a.out || (a.max_pages > 0 && !a.page_table)) return cudaErrorInvalidValue;
@@ -680,6 +680,7 @@ cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   if ((long long)p.tiles * a.Hkv > 65535) return cudaErrorInvalidValue;
   a.split_pages = p.split_pages;
   a.max_splits = p.max_splits;
+  if (a.window >= a.max_kv_len) a.window = 0;  // every position is in it
   a.group = a.Hq / a.Hkv;
   a.inv_group = ((1ull << 32) + a.group - 1) / a.group;  // x inv >> 32 = x / group for x < 2^32 / group: columns of a tile and the rest before them
   a.kv_bound = (int)std::min<long long>((long long)a.max_pages * PAGE, a.max_kv_len);

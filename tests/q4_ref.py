@@ -56,7 +56,8 @@ def make_plane(x, keys):
 
 
 def attention(q, k_plane, v_plane, table, kv_lens, rows, scale, window=0, softcap=0.0, sink=None, num_pages=None):
-    """q [T, Hq, D] -> float64 (o, sum of p |v|): rows[b] last positions of each sequence, packed."""
+    """q [T, Hq, D] -> float64 (o, sum of p |v| + 2^-24 sum of |v|): rows[b] last positions of each sequence, packed.  (The second is what the result's error
+    goes by; its small part stands for weights far below the largest, which fp16 holds to a 2^-35 of that.)"""
     t, hq, d = q.shape
     hkv = k_plane.shape[1]
     num_pages = num_pages or k_plane.shape[0]
@@ -94,7 +95,7 @@ def attention(q, k_plane, v_plane, table, kv_lens, rows, scale, window=0, softca
                 o = torch.stack([torch.einsum("hj,jd->hd", p[i][:, sees[i, some]], v[sees[i, some]]) for i in range(r)]) if not torch.isfinite(v).all() \
                     else torch.einsum("ihj,jd->ihd", p, v)
                 out[at:at + r, hs] = o
-                mass[at:at + r, hs] = torch.einsum("ihj,jd->ihd", p, torch.where(torch.isfinite(v), v.abs(), 0.0))
+                mass[at:at + r, hs] = torch.einsum("ihj,jd->ihd", torch.where(sees[:, None][..., some], p + 2.0 ** -24, p), torch.where(torch.isfinite(v), v.abs(), 0.0))
         at += r
     return out, mass
 

@@ -43,7 +43,7 @@ def attn(q=OK, ldq=1024, kc=OK, vc=OK, table=OK, max_pages=8, kv=OK, cu=OK, out=
 @pytest.mark.parametrize("kw", [dict(q=None), dict(kc=None), dict(vc=None), dict(table=None), dict(kv=None), dict(out=None), dict(work=None), dict(q=OK + 2), dict(kc=OK + 8),
                                 dict(vc=OK + 2), dict(ldq=1016), dict(ldq=1028), dict(ldo=1016), dict(out=OK + 1), dict(B=0), dict(B=65536), dict(T=-1), dict(most=0), dict(longest=-1),
                                 dict(hq=7), dict(hkv=0), dict(hkv=3), dict(d=32), dict(d=256), dict(page=128), dict(split=-1), dict(split=2 ** 25), dict(pages=0),
-                                dict(pages=2 ** 26), dict(max_pages=-1), dict(window=-1), dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("nan")), dict(cu=None, T=3),
+                                dict(pages=2 ** 26), dict(max_pages=-1), dict(window=-1), dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("nan")), dict(scale=float("inf")), dict(cap=float("inf")), dict(cu=None, T=3),
                                 dict(cu=None, most=2), dict(hq=2 ** 20, hkv=2 ** 20, ldq=2 ** 27, ldo=2 ** 27), dict(hq=4097, hkv=1, ldq=2 ** 20, ldo=2 ** 20), dict(work=OK + 4)])
 def test_attention_refusals(kw):
     assert attn(**kw) == 1

@@ -176,6 +176,20 @@ def test_kv_write(L, T, hkv, d, seen):
         assert torch.equal(k, k0) and torch.equal(v, v0)
 
 
+@pytest.mark.parametrize("T,hkv,d,start", [(1, 1, 128, 63), (2, 3, 64, 0), (130, 2, 128, 0), (131, 2, 128, 5), (64, 1, 64, 127), (77, 4, 64, 64)])
+def test_kv_write_of_positions_in_a_row(L, T, hkv, d, start):
+    """Prompts: neighbours share the words of values; first slots of either parity, a gap in the middle."""
+    pages = (start + T) // PAGE + 2
+    x = torch.randn(T, 2 * hkv * d, generator=gen(T + start), device=DEV).to(BF)
+    slots = torch.arange(start, start + T, device=DEV).int()
+    if T > 100:
+        slots[70:] += 1
+        slots[99] = -1
+    planes, ks, vs = write(L, x[:, :hkv * d], x[:, hkv * d:], slots, hkv, d, pages)
+    check_written(x[:, :hkv * d], ks, planes[0], slots, hkv, d, True)
+    check_written(x[:, hkv * d:], vs, planes[1], slots, hkv, d, False)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_kv_write_at_the_borders_of_codes(L, d):
     """Half steps, equal magnitudes of both signs, zeros, the smallest and largest numbers, infinities and NaN, every multiple of a half scale."""
@@ -271,7 +285,8 @@ def cache(seed, lens, hkv, d, spread=1.0, spare=2, width=0):
 
 def check_attn(out, want, mass, hq, d):
     """bf16 rounding of the result (2^-8 of it); every weight is rounded to fp16 by itself and again times its value scale, each by 2^-11 of it at most, so
-    (1 + 2^-11)^2 - 1 < 2^-10 + 2^-21 of the sum of p |v|; 2^-12 of that sum for all that is done in fp32."""
+    (1 + 2^-11)^2 - 1 < 2^-10 + 2^-21 of the sum of p |v|, or by half a step of fp16's smallest numbers, 2^-25 where the largest weight is 2^10: 2^-35 |v|, which
+    2^-10 of the 2^-24 |v| in `mass` covers twice; 2^-12 of that sum for all that is done in fp32."""
     got = out[:, :hq * d].view(-1, hq, d).double()
     off = (got - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -12) * mass + 1e-30)
     assert not torch.isnan(got).any() and (off <= 0).all(), (off.max().item(), (got - want).norm().item() / want.norm().item())
@@ -350,6 +365,77 @@ def test_attention_bits_depend_on_the_sequence_and_the_split_alone(L):
         assert torch.equal(full[b], attn(L, q[b:b + 1], kp, vp, table[b:b + 1].clone(), lens[b:b + 1], [1], d ** -0.5, split=8)[0])
     again = attn(L, q, kp, vp, table, lens, [1] * 5, d ** -0.5, split=8, longest_kv=50000)
     assert torch.equal(full, again)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 3e-30, 2.0])
+def test_attention_scales(L, scale):
+    """Negative, none at all (every visible position alike), next to none, large."""
+    hq, hkv, d, lens, rows = 6, 2, 64, [200, 65, 1], [3, 1, 1]
+    kp, vp, table = cache(3, lens, hkv, d)
+    q = torch.randn(5, hq, d, generator=gen(21), device=DEV).to(BF)
+    sk = torch.randn(hq, generator=gen(22), device=DEV).to(BF)
+    for window, cap in ((0, 0.0), (2 ** 31 - 1, 0.0), (70, 20.0)):
+        want, mass = ref.attention(q, kp, vp, table, lens, rows, scale, window, cap, sk)
+        for split in (0, 1):
+            check_attn(attn(L, q, kp, vp, table, lens, rows, scale, window, cap, sk, split=split), want, mass, hq, d)
+
+
+def test_attention_of_many_sequences(L):
+    hq, hkv, d, B = 40, 1, 64, 1500
+    rng = random.Random(4)
+    lens = [rng.choice([0, 1, 5, 64, 100]) for _ in range(B)]
+    kp, vp, table = cache(5, lens, hkv, d)
+    q = torch.randn(B, hq, d, generator=gen(23), device=DEV).to(BF)
+    out = attn(L, q, kp, vp, table, lens, [1] * B, d ** -0.5)
+    want, mass = ref.attention(q, kp, vp, table, lens, [1] * B, d ** -0.5)
+    check_attn(out, want, mass, hq, d)
+
+
+def test_planes_beyond_32_bit_offsets(L):
+    """Planes of 4.8 GB: a row is written to the last page and read back by attention."""
+    hkv, d, pages = 8, 128, 130000
+    size = L.hbk_kv_q4_plane_bytes(pages, hkv, d)
+    assert size > 2 ** 32
+    planes = [torch.empty(pages, hkv, size // pages // hkv, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    x = torch.randn(3, 2 * hkv * d, generator=gen(24), device=DEV).to(BF)
+    slots = ints([(pages - 1) * PAGE, (pages - 1) * PAGE + 1, (pages - 2) * PAGE + 63])
+    ck(L, L.hbk_kv_write_q4(p(x), 2 * hkv * d, p(x[:, hkv * d:]), 2 * hkv * d, p(slots), p(planes[0]), p(planes[1]), None, 0, None, 0, 3, hkv, d, PAGE, pages, here()))
+    q = torch.randn(1, 16, d, generator=gen(25), device=DEV).to(BF)
+    table, kv, out = ints([[pages - 1]]), ints([2]), torch.zeros(1, 16 * d, dtype=BF, device=DEV)
+    ck(L, L.hbk_attn_paged_q4(p(q), 16 * d, p(planes[0]), p(planes[1]), p(table), 1, p(kv), None, p(out), 16 * d, None, 1, 1, 1, 64, 16, hkv, d, PAGE, 0, d ** -0.5, pages, 0, 0.0,
+                              None, here()))
+    torch.cuda.synchronize()
+    last = [pl[-1:].clone() for pl in planes]
+    want, mass = ref.attention(q, last[0], last[1], ints([[0]]), [2], [1], d ** -0.5)
+    check_attn(out, want, mass, 16, d)
+    c, s = ref.encode(x[2, :hkv * d].view(hkv, d // 32, 32))
+    got_c, got_s = ref.plane_codes(planes[0][-2], d, True)
+    assert torch.equal(got_c[:, 63], c.flatten(1)) and torch.equal(got_s[:, 63], s)
+
+
+def test_calls_on_two_streams_at_once(L):
+    """Different workspaces, the same cache and weights: neither disturbs the other."""
+    hq, hkv, d = 32, 8, 128
+    lens = [3000, 2000, 700, 64]
+    kp, vp, table = cache(43, lens, hkv, d)
+    w, vals = ref.q4_0_blocks(torch.randn(512, hq * d, generator=gen(44), device=DEV))
+    packed = torch.zeros(L.hbk_gemm_q4_bytes(512, hq * d), dtype=torch.uint8, device=DEV)
+    ck(L, L.hbk_gemm_q4_pack(p(w), p(packed), 512, hq * d, here()))
+    qs = [torch.randn(4, hq, d, generator=gen(45 + i), device=DEV).to(BF) for i in range(2)]
+    kv = ints(lens)
+    n = L.hbk_attn_paged_q4_workspace_floats(4, 4, 1, 3000, hq, hkv, d, 0, 0)
+    state = [(q, torch.empty(n, device=DEV), torch.zeros(4, hq * d, dtype=BF, device=DEV), torch.zeros(4, 512, device=DEV), torch.cuda.Stream()) for q in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for q, work, o, y, s in state:
+            ck(L, L.hbk_attn_paged_q4(p(q), hq * d, p(kp), p(vp), p(table), table.shape[1], p(kv), None, p(o), hq * d, p(work), 4, 4, 1, 3000, hq, hkv, d, PAGE, 0, d ** -0.5,
+                                      kp.shape[0], 0, 0.0, None, s.cuda_stream))
+            ck(L, L.hbk_gemm_q4(p(o), hq * d, p(packed), p(y), 512, None, 0, None, 4, 512, hq * d, 6, s.cuda_stream))
+    torch.cuda.synchronize()
+    for q, work, o, y, s in state:
+        want, mass = ref.attention(q, kp, vp, table, lens, [1] * 4, d ** -0.5)
+        check_attn(o, want, mass, hq, d)
+        check_product(y, o, vals, 6)
 
 
 def test_attention_large_and_small_numbers(L):
