@@ -4,8 +4,13 @@
 // rows); the 16-row operand of a warp-wide 16 x 8 x 16 product is W, x the 8-column one.  c - 8 is exact in bf16; a group's products are summed by
 // themselves and multiplied by d in fp32.  16 rows x 32 columns for eight rows of x are some 32 instructions, where HBM gives an SM 50.
 //
-// A block owns 16 rows per warp; x passes through shared memory once for all its warps.  The blocks of a cluster share K and add their sums through distributed shared memory, in order: few rows of W still
-// keep every SM reading, without a workspace or a second launch.
+// A block owns 16 rows per warp; x passes through shared memory once for all its warps.  The blocks of a cluster share K and add their sums through
+// distributed shared memory, in order: few rows of W still keep every SM reading, without a workspace or a second launch.
+//
+// Measured: 1 x 28672 x 4096 19 us (66 MB, 53 % of the copy rate; the same loads without the arithmetic 13), 8 x 4096 x 14336 13.7, 13 x 4096 x 14336 17,
+// 32 x 28672 x 4096 41 (448 blocks on 148 SMs: four places carry 3.03; a third of that is the tail; half the products, no scales or no codes
+// taken apart change it by less than a tenth each).  Also tried: eight warps along K per 16 rows (x read eight times: 85), x staged whole (58), shares of
+// 5 to 8 warps (within 5 %), two tiles of rows per warp (47).
 #include <algorithm>
 #include <atomic>
 
