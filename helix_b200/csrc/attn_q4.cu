@@ -365,28 +365,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
       uint8_t* mine = vb + q4::code_bytes(D) + lane * (J * 4);
       load_words<D>(mine, w);
       const int at = pos + 2 * lane;
-      uint32_t x[J / 2], y[J / 2], most[J];
+      uint32_t x[J / 2], y[J / 2];
       bool grow = false;
 #pragma unroll
       for (int k = 0; k < J / 2; ++k) {
         x[k] = whole || (at >= tile.lo && at < tile.hi) ? w[k] & 0x7fff7fffu : 0u;
         y[k] = whole || (at + 1 >= tile.lo && at + 1 < tile.hi) ? w[J / 2 + k] & 0x7fff7fffu : 0u;
-        const uint32_t both = __vmaxu2(x[k], y[k]);
-        most[2 * k] = __reduce_max_sync(0xffffffffu, both & 0xffffu);
-        most[2 * k + 1] = __reduce_max_sync(0xffffffffu, both >> 16);
-        grow |= (int)(most[2 * k] >> 7) > ex[2 * k] || (int)(most[2 * k + 1] >> 7) > ex[2 * k + 1];
+        const uint32_t fits = (uint32_t)(ex[2 * k] << 7 | ex[2 * k + 1] << 23) | 0x007f007fu;  // the largest numbers of the present exponents
+        grow |= __vmaxu2(__vmaxu2(x[k], y[k]), fits) != fits;
       }
-      if (grow) {
+      if (__any_sync(0xffffffffu, grow)) {
         auto finite = [](uint32_t u) {  // infinities and NaN: 0 (they reach their columns through the weights)
           return ((u & 0xffffu) < 0x7f80u ? u & 0xffffu : 0u) | ((u >> 16) < 0x7f80u ? u & 0xffff0000u : 0u);
         };
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          if (most[j] >= 0x7f80u) {
-            const uint32_t z = __vmaxu2(finite(x[j / 2]), finite(y[j / 2]));
-            most[j] = __reduce_max_sync(0xffffffffu, j & 1 ? z >> 16 : z & 0xffffu);
-          }
-          const int e = max((int)(most[j] >> 7), ex[j]);
+          const uint32_t z = __vmaxu2(finite(x[j / 2]), finite(y[j / 2]));
+          const int e = max((int)(__reduce_max_sync(0xffffffffu, j & 1 ? z >> 16 : z & 0xffffu) >> 7), ex[j]);
           const float less = exp2f((float)(ex[j] - e));
           ex[j] = e;
 #pragma unroll

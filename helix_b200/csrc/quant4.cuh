@@ -30,9 +30,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t o) {
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(m), "r"(o));
   return r;
 }
-__device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
@@ -50,14 +50,15 @@ __device__ __forceinline__ uint32_t bfma2(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// The four registers (c - 8 of nibbles r and r + 4, exact) of a word.  As fp16: c in the low mantissa bits of 1024 is 1024 + c; one place of four
-// bits higher it is 1024 + 16 c, which a multiply-add by 1/16 brings back, so that only one shift is needed.
+// The four registers (c - 8 of nibbles r and r + 4, exact) of a word, two instructions each.  A byte (c + 16 c') in the low mantissa bits of 1024 is
+// v = 1024 + c + 16 c'; with its low nibble replaced by 8 it is u = 1032 + 16 c'.  v - u = c - 8 and u / 16 - 72.5 = c' - 8, each in one step.
 __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&a)[4]) {
-  const uint32_t h = w >> 8;
-  a[0] = hadd2(and_or(w, 0x000f000fu, 0x64006400u), 0xe408e408u);               // - 1032
-  a[1] = hfma2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);  // / 16 - 72
-  a[2] = hadd2(and_or(h, 0x000f000fu, 0x64006400u), 0xe408e408u);
-  a[3] = hfma2(and_or(h, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t v = __byte_perm(w, 0x64646464u, h ? 0x4341 : 0x4240), u = and_or(v, 0xfff0fff0u, 0x00080008u);
+    a[2 * h] = hsub2(v, u);
+    a[2 * h + 1] = hfma2(u, 0x2c002c00u, 0xd488d488u);
+  }
 }
 // As bf16: seven mantissa bits, c in the lowest of 128
 __device__ __forceinline__ void codes_bf16(uint32_t w, uint32_t (&a)[4]) {
