@@ -593,10 +593,12 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args
 struct Plan {
   int split_pages, max_splits, tiles, cols;
 };
-// By the rule (split_pages 0) a tile's pages are cut into so many shares that there are some 1.67 blocks per SM, and that none has more than 40 pages
-// (16 where a tile has 16 columns: a page takes twice as long there); a share is a page per warp at least.  Both sides, us: one sequence of 2k 6.4
-// in shares of 4 pages, 15.5 whole; 8 of 2k 10.4 in 8, 16.1 whole; 32 of 2k 26.1 whole, 29.0 in 16; 64 of 2k 39.3 whole, 45.8 in 16; 32 of 8k 67.5 in 32,
-// 73.0 whole; 48 of 200 to 4000 41.1 in 32, 54.8 whole (8 kv heads of 128 entries).
+// By the rule (split_pages 0) a tile's pages are cut into so many shares that there are some 1.67 blocks per SM, and that none has more than 32 pages,
+// or 40 where all blocks are resident at once, four to an SM (16 where a tile has 16 columns: a page takes twice as long there); a share is a page
+// per warp at least.  Both sides, us: one sequence of 2k 6.4 in shares of 4 pages, 15.1 whole; 8 of 2k 10.0 in 8, 15.8 whole; 32 of 1.5k to 2.2k 24.9
+// in 36, 29.9 in 24; 32 of 8k 66.2 in 32, 67.2 in 40, 73.1 in 48; three of 9k to 131k 59.4 in 32, 64.6 in 40; 48 of 200 to 4000 40.0 in 32, 43.2 in 40,
+// 53.9 whole (8 kv heads of 128 entries).  Over 28 shapes of 64 and 128 entries, even and uneven, 32 takes 2 % less than 40; 24 takes less yet where
+// the lengths are uneven and more where they are even.
 Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int split_pages, int sms) {
   Plan p;
   const long long G = Hq / Hkv, most = G * max_q_len;
@@ -607,7 +609,8 @@ Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, 
   long long seen = pages;
   if (window > 0) seen = std::min(pages, ((long long)window + rows - 1 + PAGE - 2) / PAGE + 1);
   if (split_pages <= 0) {
-    const long long items = (long long)B * Hkv * p.tiles, most_pages = p.cols == 16 ? 16 : 40;
+    const long long items = (long long)B * Hkv * p.tiles;
+    const long long most_pages = p.cols == 16 ? 16 : items * ((seen + 39) / 40) <= 4LL * sms ? 40 : 32;
     const long long shares = std::max((5LL * sms / 3 + items - 1) / items, (seen + most_pages - 1) / most_pages);
     split_pages = (int)std::max<long long>((seen + shares - 1) / std::max(shares, 1LL), kWarps);
   }
