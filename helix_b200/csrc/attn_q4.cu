@@ -2,13 +2,15 @@
 //
 //   o = sum_j p_j v_j,  p = softmax over the visible j of s_j,  s = scale q.k (capped: cap tanh(s / cap)),  a sink adds exp(sink) to the denominator
 //
-// The columns of a block are (row, query head) pairs of one kv head, eight per product: S^T[16 positions x 8 columns] = K q^T and
-// O^T[16 entries x 8 columns] += V^T P^T as warp-wide 16 x 8 x 16 products.  Both operands that come from the cache are then the 16-row one, the
-// codes go straight from their words to its registers, and no cached byte passes through shared memory twice.  The tensor-memory path would need
-// the widened entries in shared memory: four times the cache's bytes written there and read again.
+// The columns of a block are (row, query head) pairs of one kv head.  Two kernels: up to 16 columns per block, for single tokens and short portions, and 128
+// (attn_q4_wide_kernel below) where a sequence and kv head may have 256 or more.
+//
+// The first takes eight columns per product: S^T[16 positions x 8 columns] = K q^T and O^T[16 entries x 8 columns] += V^T P^T as warp-wide 16 x 8 x 16 products.
+// Both operands that come from the cache are then the 16-row one, the codes go straight from their words to its registers, and no cached byte passes through
+// shared memory twice.  (The tensor-memory path wants the widened entries in shared memory: four times the cache's bytes written there and read again.)
 // Instructions bound it (HBM gives a position of a kv head of 128 entries 25 issue slots), the products least of all.
-//   c - 8 is exact in fp16.  (Codes as they are, numbers below fp16's smallest normal one, with the 8 taken off by a further product, save four
-//      of nine instructions per word, but such products are summed to some 14 bits only: results whose codes are near 8 were off by 2^-15 of a group's weight.)
+//   c - 8 is exact in fp16.  (Codes as they are, numbers below fp16's smallest normal one, with the 8 taken off by a further product, save three
+//      of eight instructions per word, but such products are summed to some 14 bits only: results whose codes are near 8 were off by 2^-15 of a group's weight.)
 //   S: the products of a group of 32 entries are summed by themselves, then times the key group's scale in fp32.
 //   O: the value group's scale depends on the position, which is summed over: it goes into P^T, one operand per group, fp16 (bf16 would add as much
 //      error as the output's own rounding; here two roundings of at most 2^-11 each, and 2^-35 of the largest weight for weights far below it).  A
@@ -17,16 +19,16 @@
 //   q: fp16 after a power of two per column (bf16 has fewer bits; entries 2^-27 of the column's largest and below lose some).
 // Softmax statistics and sums are fp32.  A warp takes every fourth page of the block's share by itself; the four meet at the end.
 //
-// A sequence of more than `split` pages is cut into as few even shares as none is larger, so a row's bits depend on its own sequence and
-// `split`, not on who shares the launch.
+// A sequence of more than `split` pages is cut into as few even shares as none is larger, so a row's bits depend on its own sequence, `split` and whether
+// the launch allows 256 columns, not on who shares it.
 // Sequences of more than one share leave (O, m, l) per share in the workspace, which a second kernel joins in order.
 //
 // Measured (8 kv heads of 128 entries, 32 query heads): 32 sequences of 1.5k to 2.2k positions 25 us (68 MB, 41 % of the copy rate: two blocks on most SMs
-// and one on the others, some 5 us of launch, first loads and last sums), 74 of 8k 140 us (700 MB, 76 %: 18.5 instructions per position and kv head at 65 %
-// of the issue slots; at 2k each, 41.5 us, the kernel takes 7 % less without its loads, 12 % less without the 8 taken off the codes, 2 % less without V's
-// products), three of 9k to 131k 65 us (242 MB, 56 %).  Also tried: scores in shared memory and rolled loops (a fifth more instructions), e4m3 products (widened to fp16 by
-// further instructions on this chip: 41 -> 52), pages dealt evenly over all blocks by the launch's lengths (two runs of pages per block: 26 -> 37), clusters
-// that join their sums through distributed shared memory (26 -> 29 for 32 sequences in pairs).
+// and one on the others, some 5 us of launch, first loads and last sums), 74 of 2k 39 us, 32 of 8k 66 us (302 MB, 70 %: 18.5 instructions per position and kv
+// head at 65 % of the issue slots; parts left out in a copy, at 2k: 7 % less without the loads, 12 % without the 8 taken off the codes, 2 % without V's
+// products), three of 9k to 131k 60 us (242 MB, 62 %).  Also tried: scores in shared memory and rolled loops (a fifth more instructions), e4m3 products (widened to
+// fp16 by further instructions on this chip: 41 -> 52), pages dealt evenly over all blocks by the launch's lengths (two runs of pages per block: 26 -> 37), clusters
+// that join their sums through distributed shared memory (one sequence of 2k 6.4 -> 7.2, 32 of 8k 66 -> 77).
 #include <math.h>
 
 #include <algorithm>
@@ -43,6 +45,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int PAGE = q4::kPage;
+constexpr int kWideCols = 128;  // columns of a block of the kernel for portions
 constexpr int SLOTS = 3;  // halves (K or V) of pages that a warp has in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -102,15 +105,17 @@ struct Cfg {
   static constexpr int BLOCKS = NT == 2 ? (D == 128 ? 2 : 3) : (D == 128 ? 4 : 5);  // per SM, by registers and shared memory
 };
 
-// the 16 (D = 128) or 8 (D = 64) bytes that a lane takes of a row or pair
+// the 16 (D = 128), 8 (D = 64) or 4 (D = 32: half as many) bytes that a lane takes of a row or pair
 template <int D>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[D / 32]) {
   if constexpr (D == 128) {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
     w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-  } else {
+  } else if constexpr (D == 64) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
     w[0] = u.x; w[1] = u.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 // the bf16 scales of one position
@@ -131,6 +136,19 @@ __device__ __forceinline__ void store4(bf16* dst, float4 x, float sum) {
   for (int i = 0; i < 4; ++i) dst[i] = __float2bfloat16(sum == 0.f ? 0.f : y[i] / sum);
 }
 
+// the larger magnitude of two bf16 entries that is finite, as its bits
+__device__ __forceinline__ uint32_t finite_top(uint32_t u) {
+  const uint32_t lo = u & 0x7fffu, hi = (u >> 16) & 0x7fffu;
+  return max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u);
+}
+template <int D>
+__device__ __forceinline__ void zero_columns(const AttnQ4Args& a, const Tile& tile, int kvh) {
+  for (int i = threadIdx.x; i < tile.cols * D; i += kThreads) {
+    const int c = i / D, r = div_g(a, tile.rest + c);
+    a.out[(size_t)(tile.row0 + r) * a.ldo + (size_t)(kvh * a.group + tile.rest + c - r * a.group) * D + i % D] = __float2bfloat16(0.f);
+  }
+}
+
 template <int D, int NT, bool CAP>
 __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(const AttnQ4Args a) {
   using C = Cfg<D, NT>;
@@ -146,11 +164,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
   auto row_of = [&](int c) { return div_g(a, tile.rest + c); };  // row of column c
   const int shares = tile.splits;
   if (tile.pages == 0) {  // nothing to see
-    if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i < tile.cols * D; i += kThreads) {
-        const int c = i / D, r = row_of(c);
-        a.out[(size_t)(tile.row0 + r) * a.ldo + (size_t)(kvh * G + tile.rest + c - r * G) * D + i % D] = __float2bfloat16(0.f);
-      }
+    if (blockIdx.x == 0) zero_columns<D>(a, tile, kvh);
     return;
   }
   if ((int)blockIdx.x >= shares) return;
@@ -211,11 +225,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
     for (int j = 0; j < J; ++j) {
       const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
-        if (lo < 0x7f80u) mag = max(mag, lo);
-        if (hi < 0x7f80u) mag = max(mag, hi);
-      }
+      for (int i = 0; i < 4; ++i) mag = max(mag, finite_top(w[i]));
     }
     mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
     mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
@@ -516,13 +526,494 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
   }
 }
 
-// One block per (row, head): what more than one block has worked on is joined, a warp taking every fourth share
+// Portions.  A block has 128 columns, and every page of its share is widened once for all of them: codes times scales, exact in fp16 (a code has 3 bits
+// beside its sign, a bf16 scale 8), into shared memory, where the tensor cores take them from.  S[128 columns x 64 positions] = Q K^T and
+// O[128 columns x D] += P V, with S, P (over S) and O in tensor memory; P is fp16 by one rounding of at most 2^-11.
+//   warps 0-3   a column per lane: scores, running maximum, weights; O is scaled by them where a maximum has moved far or a value scale has
+//   warps 4-7   a page's words from global memory to registers to shared memory, one page ahead of the columns
+// S of a page whose keys are there is issued by warps 4 to 6 in turn, the products with V by warp 7 (an issuing lane is held up for as long as the products
+// before it take, and the columns' warps have the longest way as it is).
+//   K: [position][entry], scaled by a power of two per position that the scores take back (largest scale in [2^11, 2^12); scales below 2^-25 of a position's
+//      largest lose bits).
+//   V: [entry][position], as pairs of positions lie together in the words; its power of two is per group and follows its largest finite scale so far (scales
+//      below 2^-25 of it lose bits).
+// Both are rows of 128 bytes with 16-byte chunks at the places that the 128-byte swizzle gives them; every store of eight lanes meets all banks.
+// Measured (32 query heads over 8 kv heads of 128 entries), with the kernel above beside it: 512 rows behind 3584 positions 96 us (206), a prompt of 2048 rows
+// 127 (252), 128 rows of four sequences of 4096 99 (182), 64 rows of one 34 (37), but of 16 sequences of 1024 50 (38); 32 rows, 128 columns, of four 37 (36).
+// No unit is busy half of its time: a page takes 1100 issue slots per SM quarter, the chain scores - weights - V - scores of the page after next some
+// 2600 cycles with two blocks per SM.  Sixteen columns per warp from one widened page with the warp-wide products took 197 us for the 512 rows.
 template <int D>
+struct Wide {
+  static constexpr int COLS = kWideCols;
+  static constexpr int THREADS = 256;
+  static constexpr int BLOCK = q4::block_bytes(D);
+  static constexpr int Q_BYTES = COLS * D * 2, HALF = PAGE * D * 2;  // widened K or V
+  static constexpr int J = D / q4::kGroup;
+  struct Page {  // what a widened page is besides
+    float factor[PAGE];
+    float less[4];  // the groups' factors for O so far
+    int ex[4];
+    int id, grow, bad;
+  };
+  static constexpr int KEYS = Q_BYTES, VALUES = KEYS + 2 * HALF, PAGES = VALUES + 2 * HALF, PAIRS = PAGES + 4 * 512, BARS = PAIRS + 4 * PAGE / 2 * J * 4;
+  static constexpr int SMEM = (BARS + 128 > 80 * 1024 ? BARS + 128 : 80 * 1024) + 1024;  // (two blocks per SM: tensor memory has room for no more)
+  static_assert(sizeof(Page) <= 512);
+};
+// False where the barrier has not turned after some seconds.  (A block that gives up writes NaN.)
+__device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < 4000000000ll) {
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const AttnQ4Args a) {
+  using C = Wide<D>;
+  constexpr int J = C::J;
+  extern __shared__ uint8_t smem_raw[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.group;
+  const int b = blockIdx.z, ct = blockIdx.y / a.Hkv, kvh = blockIdx.y - ct * a.Hkv;
+  const Tile tile = tile_of(a, b, ct, C::COLS);
+  if (tile.cols <= 0) return;
+  auto row_of = [&](int c) { return div_g(a, tile.rest + c); };
+  const int shares = tile.splits;
+  if (tile.pages == 0) {
+    if (blockIdx.x == 0) zero_columns<D>(a, tile, kvh);
+    return;
+  }
+  if ((int)blockIdx.x >= shares) return;
+  const int p_begin = tile.page0 + (int)((long long)tile.pages * blockIdx.x / shares);
+  const int n_pages = tile.page0 + (int)((long long)tile.pages * (blockIdx.x + 1) / shares) - p_begin;
+
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
+  auto info_of = [&](int i) { return reinterpret_cast<typename C::Page*>(smem + C::PAGES + (i & 3) * 512); };  // (read till P is there, written when S two pages before is)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
+  // keys there (page i: i & 3), values, scores, weights there, page done with (i & 1)
+  uint64_t *k_full = bars, *v_full = bars + 4, *s_full = bars + 6, *p_full = bars + 8, *pv_done = bars + 10;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 12);
+  if (threadIdx.x == 128) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_full[i + 2], 4);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 7) {
+    tmem_alloc(tmem_ptr, 256);
+    tmem_relinquish();
+  }
+  const int all_hi = tile.pos0, all_lo = a.window > 0 ? tile.pos0 + row_of(tile.cols - 1) - a.window + 1 : 0;
+  auto whole_at = [&](int pos) { return pos >= all_lo && pos + PAGE - 1 <= all_hi; };  // every column sees all of the page at pos
+  float mul = 0.f;
+  if (warp < 4) {  // q: a column's row as fp16, its largest entry in [2^10, 2^11)
+    const int c = threadIdx.x;
+    const bool is = c < tile.cols;
+    const int r = is ? row_of(c) : 0;
+    const bf16* src = a.q + (size_t)(tile.row0 + r) * a.ldq + (size_t)(kvh * G + (is ? tile.rest + c - r * G : 0)) * D;
+    uint32_t mag = 0;
+    if (is)
+      for (int x = 0; x < D / 8; ++x) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * x);
+        mag = max(max(mag, max(finite_top(w.x), finite_top(w.y))), max(finite_top(w.z), finite_top(w.w)));
+      }
+    const int e = max((int)(mag >> 7), 20);
+    const float up = __uint_as_float((uint32_t)(264 - e) << 23), down = __uint_as_float((uint32_t)(e - 10) << 23);
+    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+    for (int x = 0; x < D / 8; ++x) {
+      uint4 w = is ? *reinterpret_cast<const uint4*>(src + 8 * x) : make_uint4(0, 0, 0, 0);
+      w.x = q4::pack_f16x2(q4::bf16_lo(w.x) * up, q4::bf16_hi(w.x) * up) ^ sign;
+      w.y = q4::pack_f16x2(q4::bf16_lo(w.y) * up, q4::bf16_hi(w.y) * up) ^ sign;
+      w.z = q4::pack_f16x2(q4::bf16_lo(w.z) * up, q4::bf16_hi(w.z) * up) ^ sign;
+      w.w = q4::pack_f16x2(q4::bf16_lo(w.w) * up, q4::bf16_hi(w.w) * up) ^ sign;
+      *reinterpret_cast<uint4*>(smem + (x >> 3) * (C::COLS * 128) + c * 128 + (((x & 7) ^ (c & 7)) << 4)) = w;
+    }
+    mul = fmaxf(down * (CAP ? fabsf(a.scale) : fabsf(a.scale) * kLog2e), 1e-37f);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0), tmem_o = tmem + 2 * PAGE;  // columns: two pages of S, then O
+  constexpr uint32_t f16 = ~((1u << 7) | (1u << 10));  // (the descriptors' types)
+  constexpr uint32_t idesc_s = umma_idesc_bf16(C::COLS, PAGE) & f16, idesc_o = umma_idesc_bf16(C::COLS, D) & f16;
+  const bool leader = elect_one_sync();
+  bool ok = true;
+  float m = -INFINITY, l = 0.f;
+  const uint32_t tmem_row = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes
+
+  if (warp < 4) {
+    const int c = threadIdx.x;
+    const int last = c < tile.cols ? tile.pos0 + row_of(c) : -1, first = a.window > 0 ? last - a.window + 1 : 0;
+    for (int i = 0; i < n_pages; ++i) {
+      const int st = i & 1, ph = (i >> 1) & 1, pos = (p_begin + i) * PAGE;
+      if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1) && wait_turn(&s_full[st], ph))) break;
+      tc_fence_after();
+      const typename C::Page& pg = *info_of(i);
+      float s[PAGE];
+      {
+        uint32_t(&lo)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
+        uint32_t(&hi)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[32]);
+        tmem_ld_32x32b_x32(tmem + tmem_row + st * PAGE, lo);
+        tmem_ld_32x32b_x32(tmem + tmem_row + st * PAGE + 32, hi);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int x = 0; x < PAGE; x += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(&pg.factor[x]);
+        f2_unpack(f2_mul(f2_pack(s[x], s[x + 1]), f2_pack(f.x, f.y)), s[x], s[x + 1]);
+        f2_unpack(f2_mul(f2_pack(s[x + 2], s[x + 3]), f2_pack(f.z, f.w)), s[x + 2], s[x + 3]);
+      }
+      if constexpr (CAP) {
+        const float in = 2.f * kLog2e / a.softcap, out = a.softcap * kLog2e;
+#pragma unroll
+        for (int x = 0; x < PAGE; ++x) s[x] = fmaf(-2.f * out, __fdividef(1.f, exp2_fast(s[x] * mul * in) + 1.f), out);
+      }
+      if (pg.id < 0 || !whole_at(pos)) {
+        const int hi = pg.id < 0 ? -1 : last - pos, lo = first - pos;
+#pragma unroll
+        for (int x = 0; x < PAGE; ++x)
+          if (x > hi || x < lo) s[x] = -INFINITY;
+      }
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int x = 4; x < PAGE; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
+      float x = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if constexpr (!CAP) x *= mul;
+      // weights up to 2^15 fit fp16, so what they are relative to moves seldom
+      const bool moved = x > m + 5.f;
+      if (__any_sync(0xffffffffu, moved) || pg.grow) {
+        x = fmaxf(m, x);
+        const float f = m == x ? 1.f : exp2_fast(m - x);  // (-inf before: 0)
+        m = x;
+        l *= f;
+        if (i > 0) {
+          if (!(ok = wait_turn(&pv_done[st ^ 1], ((i - 1) >> 1) & 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const float by = f * pg.less[j];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tmem_o + tmem_row + 32 * j + 16 * h, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * by);
+              tmem_st_32x32b_x16(tmem_o + tmem_row + 32 * j + 16 * h, o);
+            }
+          }
+        }
+      }
+      const float base = 10.f - (m == -INFINITY ? 0.f : m);
+      uint64_t sums[2] = {0, 0};
+#pragma unroll
+      for (int y = 0; y < PAGE; y += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int z = 0; z < 16; ++z) {
+          float p0 = s[y + 2 * z] + base, p1 = s[y + 2 * z + 1] + base;
+          if constexpr (!CAP) f2_unpack(f2_fma(f2_pack(s[y + 2 * z], s[y + 2 * z + 1]), f2_pack(mul, mul), f2_pack(base, base)), p0, p1);
+          p0 = exp2_fast(p0);
+          p1 = exp2_fast(p1);
+          sums[z & 1] = f2_add(sums[z & 1], f2_pack(p0, p1));
+          w[z] = q4::pack_f16x2(p0, p1);
+        }
+        tmem_st_32x32b_x16(tmem + tmem_row + st * PAGE + y / 2, w);
+      }
+      {
+        float x0, x1;
+        f2_unpack(f2_add(sums[0], sums[1]), x0, x1);
+        l += x0 + x1;
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[st]);
+      if (pg.bad) {  // infinities and NaN among value scales that not every column sees were widened as 0: for the columns that do, after the products
+        if (!(ok = wait_turn(&pv_done[st], ph))) break;
+        tc_fence_after();
+        const uint8_t* vb = a.v_cache + ((size_t)pg.id * a.Hkv + kvh) * C::BLOCK;
+        for (int j = 0; j < J; ++j)
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tmem_o + tmem_row + 32 * j + 16 * h, o);
+            tmem_ld_wait();
+            for (int p = max(first - pos, 0); p <= min(last - pos, PAGE - 1); ++p) {
+              const uint32_t d = *reinterpret_cast<const uint16_t*>(vb + q4::code_bytes(D) + (p * J + j) * 2);
+              if ((d & 0x7fffu) < 0x7f80u) continue;
+#pragma unroll
+              for (int y = 0; y < 16; ++y) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(vb + (p >> 1) * D + ((4 * h + (y >> 2)) ^ q4::place_xor(D, p >> 1)) * (D / 8) + 4 * j);
+                const int code = w >> (4 * (y & 3) + 16 * (p & 1)) & 15;
+                o[y] = __float_as_uint(__uint_as_float(o[y]) + __uint_as_float(d << 16) * (float)(code - 8));
+              }
+            }
+            __syncwarp();
+            tmem_st_32x32b_x16(tmem_o + tmem_row + 32 * j + 16 * h, o);
+          }
+        tmem_st_wait();
+        tc_fence_before();  // (the next weights say that O may be added to)
+      }
+    }
+    if (ok) ok = wait_turn(&pv_done[(n_pages - 1) & 1], ((n_pages - 1) >> 1) & 1);
+  } else {
+    const int id_x = threadIdx.x - 128;
+    const int32_t* table = a.page_table + (size_t)b * a.max_pages + p_begin;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(smem + C::PAIRS) + (warp - 4) * (PAGE / 2 * J);
+    int ids = -1;  // lane i % 32 holds the number of page i, -1 for one that is none
+    auto number_of = [&](int i) {
+      if ((i & 31) == 0) {
+        ids = -1;
+        if (i + lane < n_pages) {
+          const int id = table[i + lane];
+          if (id >= 0 && id < a.num_pages) ids = id;
+        }
+      }
+      const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+      return i < n_pages ? id : -1;
+    };
+    // keys: quarter u of rows p and p + 32; values: half a chunk of four pairs
+    const int l8 = lane >> 2, u = lane & 3, p = (warp - 4) * 8 + ((l8 & 1) << 2 | l8 >> 1);
+    const int p8 = lane & 7, chunk = id_x >> 4, half = (id_x >> 3) & 1;
+    constexpr int W = J / 2;
+    uint32_t kw[2][J], ks[2][W], vw[4][W], vs[J];  // (of a page that is none: page 0's, not used)
+    auto load_keys = [&](int id) {
+      const uint8_t* kb = a.k_cache + ((size_t)max(id, 0) * a.Hkv + kvh) * C::BLOCK;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_words<D>(kb + (p + 32 * h) * (D / 2) + u * (D / 8), kw[h]);
+        load_words<D / 2>(kb + q4::code_bytes(D) + (p + 32 * h) * J * 2, ks[h]);
+      }
+    };
+    auto load_values = [&](int id) {
+      const uint8_t* vb = a.v_cache + ((size_t)max(id, 0) * a.Hkv + kvh) * C::BLOCK;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = 4 * p8 + k;
+        load_words<D / 2>(vb + n * D + (chunk ^ q4::place_xor(D, n)) * (D / 8) + half * (D / 16), vw[k]);
+      }
+      load_words<D>(vb + q4::code_bytes(D) + lane * (J * 4), vs);
+    };
+    int ex[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) ex[j] = 12;
+    auto add_values = [&](int i) {  // O += P V of page i
+      const int st = i & 1, ph = (i >> 1) & 1;
+      if (!wait_turn(&p_full[st], ph) || !wait_turn(&v_full[st], ph)) return false;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t vd = umma_desc_kmajor_sw128(smem_u32(smem + C::VALUES + st * C::HALF));
+#pragma unroll
+        for (int k = 0; k < PAGE / 16; ++k) umma_f16_ts(tmem_o, tmem + st * PAGE + k * 8, vd + (k * 32 >> 4), idesc_o, i > 0 || k != 0);
+        umma_commit(&pv_done[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    int id = number_of(0);
+    load_keys(id);
+    load_values(id);
+    for (int i = 0; i < n_pages; ++i) {
+      const int st = i & 1, pos = (p_begin + i) * PAGE;
+      const bool whole = whole_at(pos);
+      const int id_next = number_of(i + 1);
+      if (i >= 2 && !(ok = wait_turn(&s_full[st], ((i - 2) >> 1) & 1))) break;
+      typename C::Page& pg = *info_of(i);
+      uint8_t* keys = smem + C::KEYS + st * C::HALF;
+      uint8_t* values = smem + C::VALUES + st * C::HALF;
+      if (id < 0) {  // no column sees it, and whatever the weights' zeros are multiplied with is finite
+#pragma unroll
+        for (int j = 0; j < J; ++j) vs[j] = 0;
+      }
+      bool bad = false, grow = false;
+      float less[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) less[j] = 1.f;
+      {  // a lane takes the scales of positions 2 lane and 2 lane + 1
+        const int at = pos + 2 * lane;
+        uint32_t x[W], y[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          if (!whole && !(at >= tile.lo && at < tile.hi)) vs[k] = 0;
+          if (!whole && !(at + 1 >= tile.lo && at + 1 < tile.hi)) vs[W + k] = 0;
+          x[k] = vs[k] & 0x7fff7fffu;
+          y[k] = vs[W + k] & 0x7fff7fffu;
+          const uint32_t fits = (uint32_t)(ex[2 * k] << 7 | ex[2 * k + 1] << 23) | 0x007f007fu;  // the largest numbers of the present exponents
+          grow |= __vmaxu2(__vmaxu2(x[k], y[k]), fits) != fits;
+        }
+        grow = __any_sync(0xffffffffu, grow);
+        if (grow) {
+          bool odd = false;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const uint32_t v0 = j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu, v1 = j & 1 ? y[j / 2] >> 16 : y[j / 2] & 0xffffu;
+            odd |= max(v0, v1) >= 0x7f80u;
+            if (!whole && v0 >= 0x7f80u) vs[j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
+            if (!whole && v1 >= 0x7f80u) vs[W + j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
+            const int e = max((int)(__reduce_max_sync(0xffffffffu, max(v0 < 0x7f80u ? v0 : 0u, v1 < 0x7f80u ? v1 : 0u)) >> 7), ex[j]);
+            less[j] = exp2f((float)(ex[j] - e));
+            ex[j] = e;
+          }
+          bad = __any_sync(0xffffffffu, odd && !whole);
+        }
+        uint32_t w[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const float near1 = __uint_as_float((uint32_t)(265 - ex[j]) << 23);
+          const uint32_t v0 = vs[j / 2], v1 = vs[W + j / 2];
+          w[j] = q4::pack_f16x2((j & 1 ? q4::bf16_hi(v0) : q4::bf16_lo(v0)) * near1, (j & 1 ? q4::bf16_hi(v1) : q4::bf16_lo(v1)) * near1);
+        }
+        __syncwarp();
+        if constexpr (J == 4) *reinterpret_cast<uint4*>(pairs + lane * J) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(pairs + lane * J) = make_uint2(w[0], w[1]);
+        __syncwarp();
+      }
+      if (id_x == 0) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          pg.less[j] = less[j];
+          pg.ex[j] = ex[j];
+        }
+        pg.id = id;
+        pg.grow = grow;
+        pg.bad = bad;
+      }
+      if (id >= 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = p + 32 * h;
+          float d[J];
+          uint32_t mag = 0;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            d[j] = j & 1 ? q4::bf16_hi(ks[h][j / 2]) : q4::bf16_lo(ks[h][j / 2]);
+            if (j & 1) mag = max(mag, finite_top(ks[h][j / 2]));
+          }
+          const int e = max((int)(mag >> 7), 12);
+          const float near1 = __uint_as_float((uint32_t)(265 - e) << 23);  // 2^(138 - e)
+          if (u == 0) pg.factor[r] = __uint_as_float((uint32_t)(e - 11) << 23);
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const uint32_t sc = q4::pack_f16x2(d[j] * near1, d[j] * near1);
+            uint32_t x[4];
+            q4::codes_f16(kw[h][j], x);
+            *reinterpret_cast<uint4*>(keys + (j >> 1) * (PAGE * 128) + r * 128 + (((4 * (j & 1) + u) ^ (r & 7)) << 4)) =
+                make_uint4(q4::hmul2(x[0], sc), q4::hmul2(x[1], sc), q4::hmul2(x[2], sc), q4::hmul2(x[3], sc));
+          }
+        }
+      }
+      load_keys(id_next);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[i & 3]);
+      if (i >= 2 && warp == 7 && !(ok = add_values(i - 2))) break;
+      if (i >= 2 && !(ok = wait_turn(&pv_done[st], ((i - 2) >> 1) & 1))) break;
+      if (warp == 4 + i % 3) {
+        if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1))) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t qd = umma_desc_kmajor_sw128(smem_u32(smem)), kd = umma_desc_kmajor_sw128(smem_u32(keys));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16_ss(tmem + st * PAGE, qd + (((k >> 2) * (C::COLS * 128) + (k & 3) * 32) >> 4), kd + (((k >> 2) * (PAGE * 128) + (k & 3) * 32) >> 4), idesc_s, k != 0);
+          umma_commit(&s_full[st]);
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        uint32_t x[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          q4::codes_f16(vw[k][j], x[k]);
+          const uint32_t sc = pairs[(4 * p8 + k) * J + half * W + j];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[k][y] = q4::hmul2(x[k][y], sc);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int entry = 32 * (half * W + j) + 4 * chunk + y;
+          *reinterpret_cast<uint4*>(values + entry * 128 + ((p8 ^ (entry & 7)) << 4)) = make_uint4(x[0][y], x[1][y], x[2][y], x[3][y]);
+        }
+      }
+      load_values(id_next);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
+      id = id_next;
+    }
+    for (int i = max(n_pages - 2, 0); i < n_pages && ok && warp == 7; ++i) ok = add_values(i);
+  }
+  const bool failed = __syncthreads_or(!ok);
+  tc_fence_after();
+  if (warp < 4) {
+    const int c = threadIdx.x;
+    const bool is = c < tile.cols;
+    const int r = is ? row_of(c) : 0, row = tile.row0 + r, head = kvh * G + (is ? tile.rest + c - r * G : 0);
+    const bool done = shares == 1;
+    const float sink = done && a.sink ? __bfloat162float(a.sink[head]) * kLog2e : -INFINITY;
+    const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.f : top;
+    const float f = failed ? __uint_as_float(0x7fffffffu) : exp2_fast(m - ref - 10.f);  // (sums are 2^10 times what they stand for)
+    const float sum = fmaf(l, f, exp2_fast(sink - ref));
+    bf16* dst = a.out + (size_t)row * a.ldo + (size_t)head * D;
+    float* part = a.workspace + (((size_t)row * a.Hq + head) * a.max_splits + blockIdx.x) * (D + 4);
+    const bool wide = ((uintptr_t)dst & 15) == 0;
+#pragma unroll
+    for (int j = 0; j < 2 * J; ++j) {
+      uint32_t o[16];
+      __syncwarp();
+      tmem_ld_32x32b_x16(tmem_o + tmem_row + 16 * j, o);
+      tmem_ld_wait();
+      const float back = __uint_as_float((uint32_t)(info_of(n_pages - 1)->ex[j / 2] - 11) << 23);  // 2^(ex - 138)
+      float x[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) x[y] = __uint_as_float(o[y]) * back * f;
+      if (is && !done) {
+#pragma unroll
+        for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4*>(part + 16 * j + y) = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
+      } else if (is) {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) x[y] = sum == 0.f ? 0.f : x[y] / sum;
+        if (wide) {
+#pragma unroll
+          for (int y = 0; y < 16; y += 8)
+            *reinterpret_cast<uint4*>(dst + 16 * j + y) = make_uint4(pack_bf16x2(x[y], x[y + 1]), pack_bf16x2(x[y + 2], x[y + 3]), pack_bf16x2(x[y + 4], x[y + 5]), pack_bf16x2(x[y + 6], x[y + 7]));
+        } else {
+#pragma unroll
+          for (int y = 0; y < 16; ++y) dst[16 * j + y] = __float2bfloat16(x[y]);
+        }
+      }
+    }
+    if (is && !done) *reinterpret_cast<float2*>(part + D) = make_float2(m, sum);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 7) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// What more than one block has worked on is joined: four sums of every fourth share each, then these, in order.  PER = 4 warps to a (row, head) take one each;
+// where there are many (row, head)s one warp takes all four, with the same bits (512 rows of 32 heads in two shares: 5 us with one, 23 with four; one row of 256
+// heads in eight: 3 with four, 5 with one).
+template <int D, int PER>
 __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args a, int cols_per_tile) {
-  constexpr int V = D / 32;
-  __shared__ float s_part[kWarps][D + 2];
+  constexpr int V = D / 32, SUMS = 4;
+  __shared__ float s_part[SUMS][D + 2];
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = blockIdx.x / a.Hq, head = blockIdx.x - i * a.Hq;
+  const int at = blockIdx.x * (kWarps / PER) + warp / PER, i = at / a.Hq, head = at - i * a.Hq;
   // (lengths are settled: the blocks of the kernel before let this one start only once they had waited for the kernels ahead of them)
   const int ct = (i * a.group + head % a.group) / cols_per_tile;
   const Tile tile = tile_of(a, b, ct, cols_per_tile);
@@ -533,60 +1024,88 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args
   pdl_launch_dependents();
   if (c >= tile.cols || shares <= 1) return;
   const float sink = a.sink ? __bfloat162float(a.sink[head]) * kLog2e : -INFINITY;
-  // up to eight of the warp's shares at a time
-  float m = -INFINITY, sum = 0.f, acc[V] = {};
-  for (int s0 = warp; s0 < shares; s0 += 8 * kWarps) {
-    float x[8][V];
-    float2 ml[8];
+  struct Sum {
+    float m, sum, acc[V];
+  };
+  auto sum_of = [&](int first) {  // up to eight of the shares at a time
+    Sum r = {-INFINITY, 0.f, {}};
+    for (int s0 = first; s0 < shares; s0 += 8 * SUMS) {
+      float x[8][V];
+      float2 ml[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      if (s0 + k * kWarps < shares) {
-        const float* p = src + (size_t)(s0 + k * kWarps) * (D + 4);
-        ml[k] = *reinterpret_cast<const float2*>(p + D);
+      for (int k = 0; k < 8; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (s0 + k * SUMS < shares) {
+          const float* p = src + (size_t)(s0 + k * SUMS) * (D + 4);
+          ml[k] = *reinterpret_cast<const float2*>(p + D);
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[k][v] = p[lane + 32 * v];
-      } else {
+          for (int v = 0; v < V; ++v) x[k][v] = p[lane + 32 * v];
+        } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[k][v] = 0.f;
+          for (int v = 0; v < V; ++v) x[k][v] = 0.f;
+        }
+      }
+      float top = r.m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+      const float ref = top == -INFINITY ? 0.f : top, old = exp2_fast(r.m - ref);
+      r.m = top;
+      r.sum = __fmul_rn(r.sum, old);
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.acc[v] = __fmul_rn(r.acc[v], old);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = exp2_fast(ml[k].x - ref);
+        r.sum = fmaf(ml[k].y, f, r.sum);
+#pragma unroll
+        for (int v = 0; v < V; ++v) r.acc[v] = fmaf(x[k][v], f, r.acc[v]);
       }
     }
-    float top = m;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
-    const float ref = top == -INFINITY ? 0.f : top, old = exp2_fast(m - ref);
-    m = top;
-    sum *= old;
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] *= old;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = exp2_fast(ml[k].x - ref);
-      sum = fmaf(ml[k].y, f, sum);
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = fmaf(x[k][v], f, acc[v]);
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) s_part[warp][lane + 32 * v] = acc[v];
-  if (lane == 0) {
-    s_part[warp][D] = m;
-    s_part[warp][D + 1] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x < D) {
+    return r;
+  };
+  bf16* out = a.out + (size_t)row * a.ldo + (size_t)head * D;
+  if constexpr (PER == 1) {
+    Sum part[SUMS];
     float top = sink;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_part[w][D]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float y = 0.f, all = exp2_fast(sink - ref);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2_fast(s_part[w][D] - ref);
-      y = fmaf(s_part[w][threadIdx.x], f, y);
-      all = fmaf(s_part[w][D + 1], f, all);
+    for (int w = 0; w < SUMS; ++w) {
+      part[w] = sum_of(w);
+      top = fmaxf(top, part[w].m);
     }
-    a.out[(size_t)row * a.ldo + (size_t)head * D + threadIdx.x] = __float2bfloat16(all == 0.f ? 0.f : y / all);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float y[V] = {}, all = exp2_fast(sink - ref);
+#pragma unroll
+    for (int w = 0; w < SUMS; ++w) {
+      const float f = exp2_fast(part[w].m - ref);
+      all = fmaf(part[w].sum, f, all);
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[v] = fmaf(part[w].acc[v], f, y[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[lane + 32 * v] = __float2bfloat16(all == 0.f ? 0.f : y[v] / all);
+  } else {
+    const Sum part = sum_of(warp);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_part[warp][lane + 32 * v] = part.acc[v];
+    if (lane == 0) {
+      s_part[warp][D] = part.m;
+      s_part[warp][D + 1] = part.sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float top = sink;
+#pragma unroll
+      for (int w = 0; w < SUMS; ++w) top = fmaxf(top, s_part[w][D]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float y = 0.f, all = exp2_fast(sink - ref);
+#pragma unroll
+      for (int w = 0; w < SUMS; ++w) {
+        const float f = exp2_fast(s_part[w][D] - ref);
+        y = fmaf(s_part[w][threadIdx.x], f, y);
+        all = fmaf(s_part[w][D + 1], f, all);
+      }
+      out[threadIdx.x] = __float2bfloat16(all == 0.f ? 0.f : y / all);
+    }
   }
 }
 
@@ -594,15 +1113,17 @@ struct Plan {
   int split_pages, max_splits, tiles, cols;
 };
 // By the rule (split_pages 0) a tile's pages are cut into so many shares that there are some 1.67 blocks per SM, and that none has more than 32 pages,
-// or 40 where all blocks are resident at once, four to an SM (16 where a tile has 16 columns: a page takes twice as long there); a share is a page
-// per warp at least.  Both sides, us: one sequence of 2k 6.4 in shares of 4 pages, 15.1 whole; 8 of 2k 10.0 in 8, 15.8 whole; 32 of 1.5k to 2.2k 24.9
+// or 40 where all blocks are resident at once, four to an SM (with 16 columns per tile a page takes twice as long: 16, or 32 where the tiles alone are more
+// than four to an SM); a share is a page per warp at least.  Both sides, us: one sequence of 2k 6.4 in shares of 4 pages, 15.1 whole; 8 of 2k 10.0 in 8, 15.8 whole; 32 of 1.5k to 2.2k 24.9
 // in 36, 29.9 in 24; 32 of 8k 66.2 in 32, 67.2 in 40, 73.1 in 48; three of 9k to 131k 59.4 in 32, 64.6 in 40; 48 of 200 to 4000 40.0 in 32, 43.2 in 40,
 // 53.9 whole (8 kv heads of 128 entries).  Over 28 shapes of 64 and 128 entries, even and uneven, 32 takes 2 % less than 40; 24 takes less yet where
 // the lengths are uneven and more where they are even.
+// Tiles of 128 columns: as many shares as keep all blocks resident, two to an SM, of 64 pages at most (every share of a column costs its sums a way to memory and
+// back): 512 rows of one sequence of 4096 96 in 32, 109 in 16, 217 in 4.  128 columns per tile from 256 columns on: see the kernel.
 Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int split_pages, int sms) {
   Plan p;
   const long long G = Hq / Hkv, most = G * max_q_len;
-  p.cols = most > 8 ? 16 : 8;
+  p.cols = most >= 2 * kWideCols ? kWideCols : most > 8 ? 16 : 8;
   p.tiles = (int)((most + p.cols - 1) / p.cols);
   long long pages = ((long long)max_kv_len + PAGE - 1) / PAGE;
   const long long rows = std::min<long long>((p.cols + G - 2) / G + 1, max_q_len);  // rows that a tile's columns may touch
@@ -610,8 +1131,13 @@ Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, 
   if (window > 0) seen = std::min(pages, ((long long)window + rows - 1 + PAGE - 2) / PAGE + 1);
   if (split_pages <= 0) {
     const long long items = (long long)B * Hkv * p.tiles;
-    const long long most_pages = p.cols == 16 ? 16 : items * ((seen + 39) / 40) <= 4LL * sms ? 40 : 32;
-    const long long shares = std::max((5LL * sms / 3 + items - 1) / items, (seen + most_pages - 1) / most_pages);
+    long long shares;
+    if (p.cols == kWideCols) {
+      shares = std::max(2LL * sms / items, (seen + 63) / 64);
+    } else {
+      const long long most_pages = p.cols == 16 ? (items > 4LL * sms ? 32 : 16) : items * ((seen + 39) / 40) <= 4LL * sms ? 40 : 32;
+      shares = std::max((5LL * sms / 3 + items - 1) / items, (seen + most_pages - 1) / most_pages);
+    }
     split_pages = (int)std::max<long long>((seen + shares - 1) / std::max(shares, 1LL), kWarps);
   }
   p.split_pages = split_pages;
@@ -629,28 +1155,37 @@ bool sizes_ok(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int 
 }
 
 // more than 48 KB of shared memory wants to be asked for once per device
-template <int D, int NT, bool CAP>
-cudaError_t allow_smem() {
+template <auto kernel>
+cudaError_t allow_smem(int bytes) {
   static std::atomic<uint64_t> asked{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (e != cudaSuccess || (asked.load(std::memory_order_relaxed) & bit)) return e;
-  e = cudaFuncSetAttribute(attn_q4_kernel<D, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, NT>::SMEM);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
-template <int D, int NT, bool CAP>
-cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
-  cudaError_t e = allow_smem<D, NT, CAP>();
+template <auto kernel, int D>
+cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p, int smem, int threads = kThreads) {
+  cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
-  e = launch_k(attn_q4_kernel<D, NT, CAP>, dim3(p.max_splits, p.tiles * a.Hkv, a.B), dim3(kThreads), Cfg<D, NT>::SMEM, stream, true, a);
+  e = launch_k(kernel, dim3(p.max_splits, p.tiles * a.Hkv, a.B), dim3(threads), smem, stream, true, a);
   if (e != cudaSuccess || p.max_splits == 1) return e;
-  return launch_k(attn_q4_join_kernel<D>, dim3(a.max_q_len * a.Hq, a.B), dim3(kThreads), 0, stream, true, a, p.cols);
+  const long long at_most = (long long)a.max_q_len * a.Hq;  // rows and heads of a sequence
+  if (at_most * a.B >= 4096)
+    return launch_k(attn_q4_join_kernel<D, 1>, dim3((unsigned)((at_most + kWarps - 1) / kWarps), a.B), dim3(kThreads), 0, stream, true, a, p.cols);
+  return launch_k(attn_q4_join_kernel<D, kWarps>, dim3((unsigned)at_most, a.B), dim3(kThreads), 0, stream, true, a, p.cols);
 }
-template <int D, int NT>
+template <int D, bool CAP>
 cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
-  return a.softcap > 0.f ? launch<D, NT, true>(stream, a, p) : launch<D, NT, false>(stream, a, p);
+  if (p.cols == kWideCols) return launch<attn_q4_wide_kernel<D, CAP>, D>(stream, a, p, Wide<D>::SMEM, Wide<D>::THREADS);
+  if (p.cols == 16) return launch<attn_q4_kernel<D, 2, CAP>, D>(stream, a, p, Cfg<D, 2>::SMEM);
+  return launch<attn_q4_kernel<D, 1, CAP>, D>(stream, a, p, Cfg<D, 1>::SMEM);
+}
+template <int D>
+cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
+  return a.softcap > 0.f ? launch<D, true>(stream, a, p) : launch<D, false>(stream, a, p);
 }
 
 }  // namespace
@@ -689,8 +1224,7 @@ cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   a.group = a.Hq / a.Hkv;
   a.inv_group = ((1ull << 32) + a.group - 1) / a.group;  // x inv >> 32 = x / group for x < 2^32 / group: columns of a tile and the rest before them
   a.kv_bound = (int)std::min<long long>((long long)a.max_pages * PAGE, a.max_kv_len);
-  if (a.D == 128) return p.cols == 16 ? launch<128, 2>(stream, a, p) : launch<128, 1>(stream, a, p);
-  return p.cols == 16 ? launch<64, 2>(stream, a, p) : launch<64, 1>(stream, a, p);
+  return a.D == 128 ? launch<128>(stream, a, p) : launch<64>(stream, a, p);
 }
 
 }  // namespace hb

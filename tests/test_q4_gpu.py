@@ -514,6 +514,140 @@ def test_attention_cuts_what_lies_past_the_bounds(L):
     check_attn(out, want, mass, hq, d)
 
 
+@pytest.mark.parametrize("window,softcap,sink", [(0, 0.0, False), (1, 0.0, True), (70, 30.0, False), (300, 0.0, True), (0, 5.0, True)])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (9, 1, 64)])
+def test_portions_of_many_columns(L, hq, hkv, d, window, softcap, sink):
+    """256 columns and more per kv head: whole prompts, a prefix, one token, nothing, more rows than positions; rows of no sequence stay."""
+    lens, rows = [64, 700, 130, 0, 257, 65], [64, 64, 1, 0, 40, 33]
+    kp, vp, table = cache(d + window, lens, hkv, d)
+    T = sum(rows)
+    q = (2 * torch.randn(T + 3, hq, d, generator=gen(2), device=DEV)).to(BF)
+    sk = torch.randn(hq, generator=gen(3), device=DEV).to(BF) * 3 if sink else None
+    want, mass = ref.attention(q, kp, vp, table, lens, rows, d ** -0.5, window, softcap, sk)
+    for split in (0, 1, 3):
+        out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, window, softcap, sk, split=split, ldo=hq * d + (1 if split == 1 else 8))
+        check_attn(out[:T], want[:T], mass[:T], hq, d)
+        assert (out[T:] == 9).all() and (out[:, hq * d:] == 9).all()
+    out = attn(L, q[:100], kp, vp, table, [60], [100], d ** -0.5)  # its first 40 rows see nothing
+    want, mass = ref.attention(q[40:100], kp, vp, table, [60], [60], d ** -0.5)
+    assert (out[:40] == 0).all()
+    check_attn(out[40:], want, mass, hq, d)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 3e-30, 2.0])
+def test_portions_of_many_columns_scales(L, scale):
+    hq, hkv, d, lens, rows = 8, 1, 128, [300, 65], [40, 33]
+    kp, vp, table = cache(3, lens, hkv, d)
+    q = torch.randn(sum(rows), hq, d, generator=gen(21), device=DEV).to(BF)
+    for window, cap in ((0, 0.0), (2 ** 31 - 1, 0.0), (70, 20.0)):
+        want, mass = ref.attention(q, kp, vp, table, lens, rows, scale, window, cap)
+        for split in (0, 1):
+            check_attn(attn(L, q, kp, vp, table, lens, rows, scale, window, cap, split=split), want, mass, hq, d)
+
+
+def test_portions_of_many_columns_large_and_small_numbers(L):
+    """Value scales from 2^-120 to 2^100 in different groups, growing along the sequence; keys of 2^-60 and 2^60 under queries that undo them."""
+    hq, hkv, d, n, r = 16, 2, 128, 400, 40
+    pages = 7
+    grow = torch.exp2(torch.linspace(-40, 40, pages * PAGE, device=DEV)).view(pages, 1, PAGE, 1)
+    group = torch.exp2(torch.tensor([-70.0, -20.0, 0.0, 60.0], device=DEV)).repeat_interleave(32)
+    v = torch.randn(pages, hkv, PAGE, d, generator=gen(8), device=DEV) * grow * group
+    qs = torch.exp2(torch.tensor([60.0, -60.0], device=DEV)).view(1, 2, 1, 1)
+    k = torch.randn(pages, hkv, PAGE, d, generator=gen(9), device=DEV) / qs
+    kp, vp = ref.make_plane(k.to(BF), True), ref.make_plane(v.to(BF), False)
+    q = (torch.randn(r, hkv, hq // hkv, d, generator=gen(10), device=DEV) * qs).view(r, hq, d).to(BF)
+    table = torch.arange(pages, device=DEV).int()[None]
+    want, mass = ref.attention(q, kp, vp, table, [n], [r], d ** -0.5)
+    for split in (0, 1):
+        check_attn(attn(L, q, kp, vp, table, [n], [r], d ** -0.5, split=split), want, mass, hq, d)
+
+
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("d", [64, 128])
+def test_portions_of_many_columns_keep_infinities_and_nan_where_they_are_seen(L, d, split):
+    hq, hkv, J = 16, 2, d // 32
+    lens, rows = [200, 200, 150], [40, 40, 33]
+    kp, vp, table = cache(31, lens, hkv, d)
+    q = torch.randn(sum(rows), hq, d, generator=gen(12), device=DEV).to(BF)
+
+    def scale_at(plane, b, pos, h, group, value):
+        s = plane[int(table[b, pos // PAGE]), h, PAGE * d // 2 + ((pos % PAGE) * J + group) * 2:][:2]
+        s[:] = torch.tensor([value], dtype=BF).view(torch.uint8).to(DEV)
+
+    scale_at(vp, 0, 180, 0, 1, float("nan"))   # seen by the rows from 180 on
+    scale_at(vp, 0, 199, 1, 0, float("inf"))   # by the last
+    scale_at(vp, 0, 170, 1, 1, float("-inf"))
+    scale_at(vp, 1, 20, 0, 0, float("inf"))    # by all
+    scale_at(kp, 1, 50, 1, 1, float("nan"))    # by all: the whole of these heads
+    scale_at(kp, 2, 140, 0, 0, float("nan"))   # by the rows from 140 on
+    for window in (0, 25):
+        want, mass = ref.attention(q, kp, vp, table, lens, rows, d ** -0.5, window)
+        out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, window, split=split).view(-1, hq, d)
+        fine = torch.isfinite(want)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~fine & ~torch.isnan(want)].double(), want[~fine & ~torch.isnan(want)])
+        assert fine[9].all() and fine[19, :8].all() and not fine[20:40, :8, 32:64].any() and not fine[39, 8:, :32].any()  # (of the plain result)
+        check_attn(torch.where(fine, out.double(), 0.0).flatten(1), torch.where(fine, want, 0.0), torch.where(fine, mass, 0.0), hq, d)
+
+
+def test_portions_of_many_columns_do_not_see_pages_that_are_none(L):
+    hq, hkv, d, rows = 8, 1, 128, [40, 33]
+    lens = [500, 200]
+    kp, vp, table = cache(37, lens, hkv, d)
+    table[0, 0], table[0, 2], table[0, 7], table[1, 1] = -1, kp.shape[0], 2 ** 31 - 1, -5
+    q = torch.randn(sum(rows), hq, d, generator=gen(13), device=DEV).to(BF)
+    want, mass = ref.attention(q, kp, vp, table, lens, rows, d ** -0.5)
+    for split in (0, 1, 4):
+        check_attn(attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split), want, mass, hq, d)
+    table[:] = -1
+    for split in (0, 1):
+        assert (attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split) == 0).all()
+
+
+def test_portions_of_many_columns_bits_depend_on_the_sequence_and_the_split_alone(L):
+    hq, hkv, d = 32, 4, 128
+    lens, rows = [1500, 40, 777, 3000, 0], [64, 40, 5, 33, 0]
+    kp, vp, table = cache(23, lens, hkv, d)
+    q = torch.randn(sum(rows), hq, d, generator=gen(6), device=DEV).to(BF)
+    full = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=8, longest_kv=50000)
+    for b in range(4):
+        at = slice(sum(rows[:b]), sum(rows[:b + 1]))
+        assert torch.equal(full[at], attn(L, q[at], kp, vp, table[b:b + 1].clone(), lens[b:b + 1], rows[b:b + 1], d ** -0.5, split=8, most=64))
+    assert torch.equal(full, attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=8, longest_kv=50000))
+
+
+def test_portions_of_many_columns_over_a_long_cache(L):
+    hq, hkv, d, lens, rows = 8, 1, 64, [40000, 64, 9000], [33, 64, 1]
+    kp, vp, table = cache(17, lens, hkv, d, spread=0.3, width=700)
+    q = (1.5 * torch.randn(sum(rows), hq, d, generator=gen(5), device=DEV)).to(BF)
+    want, mass = ref.attention(q, kp, vp, table, lens, rows, d ** -0.5)
+    for split in (0, 64, 1000):
+        check_attn(attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split), want, mass, hq, d)
+
+
+def test_portions_of_many_columns_captured_on_two_streams(L):
+    """Two calls at once, each captured and replayed: the same bits as by itself."""
+    hq, hkv, d, rows, lens = 16, 2, 128, [64, 40], [900, 300]
+    kp, vp, table = cache(51, lens, hkv, d)
+    calls = []
+    for i in range(2):
+        q = torch.randn(sum(rows), hq, d, generator=gen(70 + i), device=DEV).to(BF)
+        want = attn(L, q, kp, vp, table, lens, rows, d ** -0.5)
+        n = L.hbk_attn_paged_q4_workspace_floats(2, sum(rows), 64, 900, hq, hkv, d, 0, 0)
+        args = dict(q=q, out=torch.zeros_like(want), work=torch.empty(max(n, 4), device=DEV), cu=ints([0, 64, 104]), kv=ints(lens))
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ck(L, L.hbk_attn_paged_q4(p(q), hq * d, p(kp), p(vp), p(table), table.shape[1], p(args["kv"]), p(args["cu"]), p(args["out"]), hq * d, p(args["work"]),
+                                      2, sum(rows), 64, 900, hq, hkv, d, PAGE, 0, d ** -0.5, kp.shape[0], 0, 0.0, None, stream.cuda_stream))
+        calls.append((args, want, stream, graph))
+    for _ in range(20):
+        for args, _, stream, graph in calls:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for args, want, _, _ in calls:
+        assert torch.equal(args["out"], want)
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
