@@ -538,8 +538,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
 //   V: [entry][position], as pairs of positions lie together in the words; its power of two is per group and follows its largest finite scale so far (scales
 //      below 2^-25 of it lose bits).
 // Both are rows of 128 bytes with 16-byte chunks at the places that the 128-byte swizzle gives them; every store of eight lanes meets all banks.
-// Measured (32 query heads over 8 kv heads of 128 entries), with the kernel above beside it: 512 rows behind 3584 positions 96 us (206), a prompt of 2048 rows
-// 127 (252), 128 rows of four sequences of 4096 99 (182), 64 rows of one 34 (37), but of 16 sequences of 1024 50 (38); 32 rows, 128 columns, of four 37 (36).
+// Measured (32 query heads over 8 kv heads of 128 entries), with the kernel above beside it: 512 rows behind 3584 positions 97 us (206), a prompt of 2048 rows
+// 125 (252), 128 rows of four sequences of 4096 99 (182), 64 rows of one of 8192 39 (56), but of 16 sequences of 1024 47 (38); 32 rows, 128 columns, of four
+// of 4096 37 (36).
 // No unit is busy half of its time: a page takes 1100 issue slots per SM quarter, the chain scores - weights - V - scores of the page after next some
 // 2600 cycles with two blocks per SM.  Sixteen columns per warp from one widened page with the warp-wide products took 197 us for the 512 rows.
 template <int D>
@@ -555,9 +556,10 @@ struct Wide {
     int ex[4];
     int id, grow, bad;
   };
-  static constexpr int KEYS = Q_BYTES, VALUES = KEYS + 2 * HALF, PAGES = VALUES + 2 * HALF, PAIRS = PAGES + 4 * 512, BARS = PAIRS + 4 * PAGE / 2 * J * 4;
-  static constexpr int SMEM = (BARS + 128 > 80 * 1024 ? BARS + 128 : 80 * 1024) + 1024;  // (two blocks per SM: tensor memory has room for no more)
-  static_assert(sizeof(Page) <= 512);
+  static constexpr int KEYS = Q_BYTES, VALUES = KEYS + 2 * HALF, PAGES = VALUES + 2 * HALF, PAIRS = PAGES + 4 * 512, BARS = PAIRS + 4 * PAGE / 2 * J * 4,
+                       MULS = BARS + 128, END = MULS + COLS * 4;
+  static constexpr int SMEM = (END > 80 * 1024 ? END : 80 * 1024) + 1024;  // (two blocks per SM: tensor memory has room for no more)
+  static_assert(sizeof(Page) <= 512 && COLS * (D + 4) * 4 <= PAGES);  // (the sums leave through the room of Q and the widened pages)
 };
 // False where the barrier has not turned after some seconds.  (A block that gives up writes NaN.)
 __device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity) {
@@ -576,7 +578,6 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   constexpr int J = C::J;
   extern __shared__ uint8_t smem_raw[];
   pdl_wait();
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.group;
   const int b = blockIdx.z, ct = blockIdx.y / a.Hkv, kvh = blockIdx.y - ct * a.Hkv;
@@ -615,35 +616,36 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   }
   const int all_hi = tile.pos0, all_lo = a.window > 0 ? tile.pos0 + row_of(tile.cols - 1) - a.window + 1 : 0;
   auto whole_at = [&](int pos) { return pos >= all_lo && pos + PAGE - 1 <= all_hi; };  // every column sees all of the page at pos
-  float mul = 0.f;
-  if (warp < 4) {  // q: a column's row as fp16, its largest entry in [2^10, 2^11)
-    const int c = threadIdx.x;
-    const bool is = c < tile.cols;
-    const int r = is ? row_of(c) : 0;
-    const bf16* src = a.q + (size_t)(tile.row0 + r) * a.ldq + (size_t)(kvh * G + (is ? tile.rest + c - r * G : 0)) * D;
-    uint32_t mag = 0;
-    if (is)
-      for (int x = 0; x < D / 8; ++x) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * x);
-        mag = max(max(mag, max(finite_top(w.x), finite_top(w.y))), max(finite_top(w.z), finite_top(w.w)));
-      }
-    const int e = max((int)(mag >> 7), 20);
-    const float up = __uint_as_float((uint32_t)(264 - e) << 23), down = __uint_as_float((uint32_t)(e - 10) << 23);
+  float* muls = reinterpret_cast<float*>(smem + C::MULS);  // what brings a column's sums to log2 of its weights (to scores, where they are capped)
+  {  // q: a column's row as fp16, its largest entry in [2^10, 2^11)
+    constexpr int PER_ROW = D / 8, AT_ONCE = 32 / PER_ROW;
+    const int x = lane % PER_ROW;
     const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
-    for (int x = 0; x < D / 8; ++x) {
-      uint4 w = is ? *reinterpret_cast<const uint4*>(src + 8 * x) : make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int c = warp * 16 + lane / PER_ROW; c < warp * 16 + 16; c += AT_ONCE) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (c < tile.cols) {
+        const int r = row_of(c);
+        w = *reinterpret_cast<const uint4*>(a.q + (size_t)(tile.row0 + r) * a.ldq + (size_t)(kvh * G + tile.rest + c - r * G) * D + 8 * x);
+      }
+      uint32_t mag = max(max(finite_top(w.x), finite_top(w.y)), max(finite_top(w.z), finite_top(w.w)));
+#pragma unroll
+      for (int y = 1; y < PER_ROW; y <<= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, y));
+      const int e = max((int)(mag >> 7), 20);
+      const float up = __uint_as_float((uint32_t)(264 - e) << 23), down = __uint_as_float((uint32_t)(e - 10) << 23);
       w.x = q4::pack_f16x2(q4::bf16_lo(w.x) * up, q4::bf16_hi(w.x) * up) ^ sign;
       w.y = q4::pack_f16x2(q4::bf16_lo(w.y) * up, q4::bf16_hi(w.y) * up) ^ sign;
       w.z = q4::pack_f16x2(q4::bf16_lo(w.z) * up, q4::bf16_hi(w.z) * up) ^ sign;
       w.w = q4::pack_f16x2(q4::bf16_lo(w.w) * up, q4::bf16_hi(w.w) * up) ^ sign;
       *reinterpret_cast<uint4*>(smem + (x >> 3) * (C::COLS * 128) + c * 128 + (((x & 7) ^ (c & 7)) << 4)) = w;
+      if (x == 0) muls[c] = fmaxf(down * (CAP ? fabsf(a.scale) : fabsf(a.scale) * kLog2e), 1e-37f);
     }
-    mul = fmaxf(down * (CAP ? fabsf(a.scale) : fabsf(a.scale) * kLog2e), 1e-37f);
     fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();  // (its columns are held: launch.h)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0), tmem_o = tmem + 2 * PAGE;  // columns: two pages of S, then O
   constexpr uint32_t f16 = ~((1u << 7) | (1u << 10));  // (the descriptors' types)
   constexpr uint32_t idesc_s = umma_idesc_bf16(C::COLS, PAGE) & f16, idesc_o = umma_idesc_bf16(C::COLS, D) & f16;
@@ -654,6 +656,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
 
   if (warp < 4) {
     const int c = threadIdx.x;
+    const float mul = muls[c];
     const int last = c < tile.cols ? tile.pos0 + row_of(c) : -1, first = a.window > 0 ? last - a.window + 1 : 0;
     for (int i = 0; i < n_pages; ++i) {
       const int st = i & 1, ph = (i >> 1) & 1, pos = (p_begin + i) * PAGE;
@@ -957,45 +960,39 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   }
   const bool failed = __syncthreads_or(!ok);
   tc_fence_after();
+  float* sums = reinterpret_cast<float*>(smem);  // [column]: D sums, maximum, sum of weights, and 8 bytes that keep the rows aligned
+  const bool done = shares == 1;
   if (warp < 4) {
-    const int c = threadIdx.x;
-    const bool is = c < tile.cols;
-    const int r = is ? row_of(c) : 0, row = tile.row0 + r, head = kvh * G + (is ? tile.rest + c - r * G : 0);
-    const bool done = shares == 1;
-    const float sink = done && a.sink ? __bfloat162float(a.sink[head]) * kLog2e : -INFINITY;
+    const int c = threadIdx.x, r = row_of(c);
+    const float sink = done && a.sink && c < tile.cols ? __bfloat162float(a.sink[kvh * G + tile.rest + c - r * G]) * kLog2e : -INFINITY;
     const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.f : top;
     const float f = failed ? __uint_as_float(0x7fffffffu) : exp2_fast(m - ref - 10.f);  // (sums are 2^10 times what they stand for)
-    const float sum = fmaf(l, f, exp2_fast(sink - ref));
-    bf16* dst = a.out + (size_t)row * a.ldo + (size_t)head * D;
-    float* part = a.workspace + (((size_t)row * a.Hq + head) * a.max_splits + blockIdx.x) * (D + 4);
-    const bool wide = ((uintptr_t)dst & 15) == 0;
 #pragma unroll
     for (int j = 0; j < 2 * J; ++j) {
       uint32_t o[16];
-      __syncwarp();
       tmem_ld_32x32b_x16(tmem_o + tmem_row + 16 * j, o);
       tmem_ld_wait();
       const float back = __uint_as_float((uint32_t)(info_of(n_pages - 1)->ex[j / 2] - 11) << 23);  // 2^(ex - 138)
       float x[16];
 #pragma unroll
       for (int y = 0; y < 16; ++y) x[y] = __uint_as_float(o[y]) * back * f;
-      if (is && !done) {
 #pragma unroll
-        for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4*>(part + 16 * j + y) = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
-      } else if (is) {
-#pragma unroll
-        for (int y = 0; y < 16; ++y) x[y] = sum == 0.f ? 0.f : x[y] / sum;
-        if (wide) {
-#pragma unroll
-          for (int y = 0; y < 16; y += 8)
-            *reinterpret_cast<uint4*>(dst + 16 * j + y) = make_uint4(pack_bf16x2(x[y], x[y + 1]), pack_bf16x2(x[y + 2], x[y + 3]), pack_bf16x2(x[y + 4], x[y + 5]), pack_bf16x2(x[y + 6], x[y + 7]));
-        } else {
-#pragma unroll
-          for (int y = 0; y < 16; ++y) dst[16 * j + y] = __float2bfloat16(x[y]);
-        }
-      }
+      for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4*>(sums + c * (D + 4) + 16 * j + y) = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
     }
-    if (is && !done) *reinterpret_cast<float2*>(part + D) = make_float2(m, sum);
+    *reinterpret_cast<float2*>(sums + c * (D + 4) + D) = make_float2(m, fmaf(l, f, exp2_fast(sink - ref)));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < tile.cols * (D / 4); i += C::THREADS) {
+    const int c = i / (D / 4), d = i % (D / 4) * 4, r = row_of(c), row = tile.row0 + r, head = kvh * G + tile.rest + c - r * G;
+    const float4 x = *reinterpret_cast<const float4*>(sums + c * (D + 4) + d);
+    const float2 ml = *reinterpret_cast<const float2*>(sums + c * (D + 4) + D);
+    if (done) {
+      store4(a.out + (size_t)row * a.ldo + (size_t)head * D + d, x, ml.y);
+    } else {
+      float* part = a.workspace + (((size_t)row * a.Hq + head) * a.max_splits + blockIdx.x) * (D + 4);
+      *reinterpret_cast<float4*>(part + d) = x;
+      if (d == 0) *reinterpret_cast<float2*>(part + D) = ml;
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1006,8 +1003,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
 }
 
 // What more than one block has worked on is joined: four sums of every fourth share each, then these, in order.  PER = 4 warps to a (row, head) take one each;
-// where there are many (row, head)s one warp takes all four, with the same bits (512 rows of 32 heads in two shares: 5 us with one, 23 with four; one row of 256
-// heads in eight: 3 with four, 5 with one).
+// where there are many (row, head)s one warp takes all four, with the same bits (512 rows of 32 heads in two shares: the call takes 97 us with one, 116 with four;
+// eight sequences of 2k with 32 heads, eight shares: 10.2 with four, 11.9 with one).
 template <int D, int PER>
 __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args a, int cols_per_tile) {
   constexpr int V = D / 32, SUMS = 4;
@@ -1066,12 +1063,25 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args
   bf16* out = a.out + (size_t)row * a.ldo + (size_t)head * D;
   if constexpr (PER == 1) {
     Sum part[SUMS];
+    if (shares <= SUMS) {  // (one each: all loads at once)
+#pragma unroll
+      for (int w = 0; w < SUMS; ++w) {
+        part[w] = Sum{-INFINITY, 0.f, {}};
+        if (w < shares) {
+          const float* p = src + (size_t)w * (D + 4);
+          part[w].m = p[D];
+          part[w].sum = p[D + 1];
+#pragma unroll
+          for (int v = 0; v < V; ++v) part[w].acc[v] = p[lane + 32 * v];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < SUMS; ++w) part[w] = sum_of(w);
+    }
     float top = sink;
 #pragma unroll
-    for (int w = 0; w < SUMS; ++w) {
-      part[w] = sum_of(w);
-      top = fmaxf(top, part[w].m);
-    }
+    for (int w = 0; w < SUMS; ++w) top = fmaxf(top, part[w].m);
     const float ref = top == -INFINITY ? 0.f : top;
     float y[V] = {}, all = exp2_fast(sink - ref);
 #pragma unroll
@@ -1119,7 +1129,7 @@ struct Plan {
 // 53.9 whole (8 kv heads of 128 entries).  Over 28 shapes of 64 and 128 entries, even and uneven, 32 takes 2 % less than 40; 24 takes less yet where
 // the lengths are uneven and more where they are even.
 // Tiles of 128 columns: as many shares as keep all blocks resident, two to an SM, of 64 pages at most (every share of a column costs its sums a way to memory and
-// back): 512 rows of one sequence of 4096 96 in 32, 109 in 16, 217 in 4.  128 columns per tile from 256 columns on: see the kernel.
+// back): 512 rows of one sequence of 4096 97 us in 32, 107 in 16, 192 in 4.  128 columns per tile from 256 columns on: see the kernel.
 Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int split_pages, int sms) {
   Plan p;
   const long long G = Hq / Hkv, most = G * max_q_len;

@@ -126,7 +126,8 @@ int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_
  * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096.  window, softcap and sink as in
  * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
  * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  split_pages: pages that one block
- * reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq / Hkv is 256 or more, on nothing else); 0: hbk_attn_paged_q4_split's.  workspace: as many floats as
+ * reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq / Hkv is 256 or more, on nothing else); 0:
+ * hbk_attn_paged_q4_split's.  Single tokens beside portions of 256 columns (rows * Hq / Hkv) are quicker in a call of their own.  workspace: as many floats as
  * hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL; on 16 bytes); launches that may run at the same time need one each. */
 int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
                       const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
@@ -139,7 +140,7 @@ size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_k
  * [16 rows][4 groups] fp16 scales. */
 size_t hbk_gemm_q4_bytes(int N, int K); /* 0: refused sizes */
 int hbk_gemm_q4_pack(const void* blocks, void* packed, int N, int K, void* stream);
-/* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 64 rows hbk_gemm with bf16 weights is quicker); epi as in hbk_gemm: 0, 1, 3, 4
+/* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 32 rows hbk_gemm with bf16 weights is quicker), N up to 65535 * 64; epi as in hbk_gemm: 0, 1, 3, 4
  * (bf16 out) or 6 (fp32 out); R may be out itself */
 int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, const void* R, int ldr, const void* bias, int M, int N, int K, int epi,
                 void* stream);

@@ -615,6 +615,17 @@ def test_portions_of_many_columns_bits_depend_on_the_sequence_and_the_split_alon
     assert torch.equal(full, attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=8, longest_kv=50000))
 
 
+@pytest.mark.parametrize("hq,d", [(256, 64), (300, 128)])
+def test_single_tokens_of_many_heads_per_kv_head(L, hq, d):
+    lens = [1, 63, 64, 0, 65, 700]
+    kp, vp, table = cache(29, lens, 1, d)
+    q = torch.randn(len(lens), hq, d, generator=gen(15), device=DEV).to(BF)
+    want, mass = ref.attention(q, kp, vp, table, lens, [1] * 6, d ** -0.5)
+    for split in (0, 2):
+        for cu in (True, False):
+            check_attn(attn(L, q, kp, vp, table, lens, [1] * 6, d ** -0.5, split=split, cu=cu), want, mass, hq, d)
+
+
 def test_portions_of_many_columns_over_a_long_cache(L):
     hq, hkv, d, lens, rows = 8, 1, 64, [40000, 64, 9000], [33, 64, 1]
     kp, vp, table = cache(17, lens, hkv, d, spread=0.3, width=700)
