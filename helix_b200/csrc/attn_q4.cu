@@ -566,7 +566,7 @@ __device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
     const long long t0 = clock64();
-    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < 4000000000ll) {
+    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < HB_WAIT_TIMEOUT_CYCLES) {
     }
   }
   return __all_sync(0xffffffffu, ok);

@@ -589,6 +589,20 @@ def test_portions_of_many_columns_keep_infinities_and_nan_where_they_are_seen(L,
         check_attn(torch.where(fine, out.double(), 0.0).flatten(1), torch.where(fine, want, 0.0), torch.where(fine, mass, 0.0), hq, d)
 
 
+def test_portions_of_many_columns_queries_that_are_none(L):
+    """A NaN or an infinity in a query is its own column's matter."""
+    hq, hkv, d, lens, rows = 16, 2, 128, [200], [40]
+    kp, vp, table = cache(33, lens, hkv, d)
+    q = torch.randn(40, hq, d, generator=gen(16), device=DEV).to(BF)
+    want, mass = ref.attention(q, kp, vp, table, lens, rows, d ** -0.5)
+    q[3, 5, 17], q[39, 15, 0] = float("nan"), float("inf")
+    for split in (0, 1):
+        out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split).view(-1, hq, d)
+        assert torch.isnan(out[3, 5]).all() and torch.isnan(out[39, 15]).all()
+        out[3, 5], out[39, 15] = want[3, 5].to(BF), want[39, 15].to(BF)
+        check_attn(out.flatten(1), want, mass, hq, d)
+
+
 def test_portions_of_many_columns_do_not_see_pages_that_are_none(L):
     hq, hkv, d, rows = 8, 1, 128, [40, 33]
     lens = [500, 200]
