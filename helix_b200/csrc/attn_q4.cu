@@ -15,7 +15,7 @@
 //   O: the value group's scale depends on the position, which is summed over: it goes into P^T, one operand per group, fp16 (bf16 would add as much
 //      error as the output's own rounding; here two roundings of at most 2^-11 each, and 2^-35 of the largest weight for weights far below it).  A
 //      group's scales are brought near 1 by a power of two that follows their largest finite one so far, as the running maximum does for the
-//      scores; scales below 2^-18 of that largest lose bits.
+//      scores; a share in which some lie below 2^-16 of it is done again in fp32 (share_in_fp32).
 //   q: fp16 after a power of two per column (bf16 has fewer bits; entries 2^-27 of the column's largest and below lose some).
 // Softmax statistics and sums are fp32.  A warp takes every fourth page of the block's share by itself; the four meet at the end.
 //
@@ -48,6 +48,10 @@ constexpr int PAGE = q4::kPage;
 constexpr int kWideCols = 128;  // columns of a block of the kernel for portions
 constexpr int SLOTS = 3;  // halves (K or V) of pages that a warp has in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
+// Powers of two that a share's value scales of one group may differ by, beyond which share_in_fp32 takes it.  A weight times its scale is an fp16 operand of at most
+// 2^15: scales 2^-16 of the largest still have all their bits, weights down to 2^-12 of the largest all of theirs, and smaller ones are off by 2^-23 of it at
+// most.  Where models' values lie: 2^4 between neighbours, 2^8 between a first position and the others.
+constexpr int kRange = 16;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -149,8 +153,136 @@ __device__ __forceinline__ void zero_columns(const AttnQ4Args& a, const Tile& ti
   }
 }
 
+// The smallest finite scale other than 0 of each value group that a lane has met, two groups to a word, as the signed 16-bit number (bits - 1) - 2^15: 0 and what
+// is not seen become 2^15 - 1, above all of them.
+constexpr uint32_t kNoScale = 0x7fff7fffu;
+__device__ __forceinline__ uint32_t smallest_scale(uint32_t low, uint32_t x, uint32_t y) {
+  return __vmins2(__vmins2(low, (x | 0x80008000u) - 0x00010001u), (y | 0x80008000u) - 0x00010001u);
+}
+// Whether some scale of group j is less than 2^-range of the group's largest (exponent field `top`)
+__device__ __forceinline__ bool out_of_range(uint32_t low, int j, int top, int range) {
+  return (((int)(short)(j & 1 ? low >> 16 : low) + 32769) >> 7) + range < top;
+}
+
+// A share by itself in fp32, whatever its scales: for those whose value scales differ so much that the operands of the kernels below would lose bits of the small ones.
+// They are brought to fp16 under the largest of the tile's positions, and that one may be of a position that a row does not see, or of next to no weight.  A warp takes
+// four columns at a time, so that a page is widened once for them: for the scores a lane takes two neighbouring positions, for the sums the entries 32 j + lane.
+// Models do not come here, so it is short, not fast (8 kv heads of 128 entries, 4 query heads each): 32 rows of one sequence of 4096 take 385 us instead of 23,
+// 512 rows 4800 instead of 97, single tokens of 32 sequences of 2k 735 instead of 30.
+template <int D, bool CAP>
+__device__ __noinline__ void share_in_fp32(const AttnQ4Args& a, int ct, int cols_per_tile, int share) {
+  constexpr int J = D / q4::kGroup, N = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, kvh = blockIdx.y % a.Hkv;
+  const Tile tile = tile_of(a, b, ct, cols_per_tile);
+  const int p_begin = tile.page0 + (int)((long long)tile.pages * share / tile.splits);
+  const int p_end = tile.page0 + (int)((long long)tile.pages * (share + 1) / tile.splits);
+  const int32_t* table = a.page_table + (size_t)b * a.max_pages;
+  for (int c = warp * N; c < tile.cols; c += blockDim.x / 32 * N) {
+    int row[N], head[N], last[N], first[N];
+    const bf16* q[N];
+    float m[N], l[N], o[N][J];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {  // (behind the tile's last column: that one again, not stored)
+      const int at = tile.rest + min(c + n, tile.cols - 1), r = div_g(a, at);
+      row[n] = tile.row0 + r;
+      head[n] = kvh * a.group + at - r * a.group;
+      last[n] = tile.pos0 + r;
+      first[n] = a.window > 0 ? last[n] - a.window + 1 : 0;
+      q[n] = a.q + (size_t)row[n] * a.ldq + (size_t)head[n] * D;
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) o[n][j] = 0.f;
+    }
+    for (int p = p_begin; p < p_end; ++p) {
+      const int id = table[p], pos = p * PAGE + 2 * lane;
+      if (id < 0 || id >= a.num_pages) continue;
+      const uint8_t* kb = a.k_cache + ((size_t)id * a.Hkv + kvh) * q4::block_bytes(D);
+      const uint8_t* vb = a.v_cache + ((size_t)id * a.Hkv + kvh) * q4::block_bytes(D);
+      float s[2][N] = {};
+      uint32_t seen[2][N];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        for (int j = 0; j < J; ++j) {
+          float group[N] = {};
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + (2 * lane + h) * (D / 2) + t * (D / 8) + 4 * j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float code = (float)((int)(w >> (4 * (i / 2 + 4 * (i & 1))) & 15u) - 8);
+#pragma unroll
+              for (int n = 0; n < N; ++n) group[n] = fmaf(__bfloat162float(q[n][32 * j + 8 * t + i]), code, group[n]);
+            }
+          }
+          const float d = __bfloat162float(*reinterpret_cast<const bf16*>(kb + q4::code_bytes(D) + ((2 * lane + h) * J + j) * 2));
+#pragma unroll
+          for (int n = 0; n < N; ++n) s[h][n] = fmaf(d, group[n], s[h][n]);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          float x = s[h][n] * a.scale;
+          if (CAP) x = a.softcap * tanhf(x / a.softcap);
+          const bool sees = pos + h >= first[n] && pos + h <= last[n];
+          s[h][n] = sees ? x * kLog2e : -INFINITY;
+          seen[h][n] = __ballot_sync(0xffffffffu, sees);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        float top = fmaxf(s[0][n], s[1][n]);
+#pragma unroll
+        for (int w = 1; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        top = fmaxf(m[n], top);
+        const float f = m[n] == top ? 1.f : exp2_fast(m[n] - top), ref = top == -INFINITY ? 0.f : top;
+        m[n] = top;
+        s[0][n] = exp2_fast(s[0][n] - ref);
+        s[1][n] = exp2_fast(s[1][n] - ref);
+        l[n] = fmaf(l[n], f, s[0][n] + s[1][n]);  // (a lane's own positions)
+#pragma unroll
+        for (int j = 0; j < J; ++j) o[n][j] *= f;
+      }
+      for (int x = 0; x < PAGE / 2; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[J];
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(vb + x * D + ((lane >> 2) ^ q4::place_xor(D, x)) * (D / 8) + 4 * j);
+            const float d = __bfloat162float(*reinterpret_cast<const bf16*>(vb + q4::code_bytes(D) + ((2 * x + h) * J + j) * 2));
+            v[j] = d * (float)((int)(word >> (4 * (lane & 3) + 16 * h) & 15u) - 8);
+          }
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            const float w = __shfl_sync(0xffffffffu, s[h][n], x);
+            if (!(seen[h][n] >> x & 1)) continue;
+#pragma unroll
+            for (int j = 0; j < J; ++j) o[n][j] = fmaf(w, v[j], o[n][j]);
+          }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int w = 1; w < 32; w <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], w);
+      if (c + n >= tile.cols) continue;
+      if (tile.splits == 1) {
+        const float sink = a.sink ? __bfloat162float(a.sink[head[n]]) * kLog2e : -INFINITY;
+        const float top = fmaxf(m[n], sink), ref = top == -INFINITY ? 0.f : top, f = exp2_fast(m[n] - ref), sum = fmaf(l[n], f, exp2_fast(sink - ref));
+#pragma unroll
+        for (int j = 0; j < J; ++j) a.out[(size_t)row[n] * a.ldo + (size_t)head[n] * D + 32 * j + lane] = __float2bfloat16(sum == 0.f ? 0.f : o[n][j] * f / sum);
+      } else {
+        float* part = a.workspace + (((size_t)row[n] * a.Hq + head[n]) * a.max_splits + share) * (D + 4);
+#pragma unroll
+        for (int j = 0; j < J; ++j) part[32 * j + lane] = o[n][j];
+        if (lane == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[n], l[n]);
+      }
+    }
+  }
+}
+
 template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(const AttnQ4Args a) {
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(const __grid_constant__ AttnQ4Args a) {
   using C = Cfg<D, NT>;
   constexpr int J = C::J;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -258,9 +390,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
   float o[J][2][NT][4];
   float m[NT][2], l[NT][2];  // running maximum (log2 of a weight) and sum of weights times 2^10
   int ex[J];                 // exponent field of a value group's largest scale so far
+  uint32_t low[J / 2];       // and its smallest
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     ex[j] = 12;
+    low[j / 2] = kNoScale;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -383,6 +517,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
         y[k] = whole || (at + 1 >= tile.lo && at + 1 < tile.hi) ? w[J / 2 + k] & 0x7fff7fffu : 0u;
         const uint32_t fits = (uint32_t)(ex[2 * k] << 7 | ex[2 * k + 1] << 23) | 0x007f007fu;  // the largest numbers of the present exponents
         grow |= __vmaxu2(__vmaxu2(x[k], y[k]), fits) != fits;
+        low[k] = smallest_scale(low[k], x[k], y[k]);
       }
       if (__any_sync(0xffffffffu, grow)) {
         auto finite = [](uint32_t u) {  // infinities and NaN: 0 (they reach their columns through the weights)
@@ -474,7 +609,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
     slot = slot == 0 ? SLOTS - 1 : slot - 1;  // two on
   }
   copy_wait<0>();
-  __syncthreads();
+  bool wide_range = false;
+#pragma unroll
+  for (int j = 0; j < J; ++j) wide_range |= out_of_range(low[j / 2], j, ex[j], kRange);
+  if (__syncthreads_or(wide_range)) {
+    share_in_fp32<D, CAP>(a, ct, C::COLS, blockIdx.x);
+    return;
+  }
 
   // the four warps meet
   float* sm = reinterpret_cast<float*>(smem);
@@ -535,8 +676,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
 // before it take, and the columns' warps have the longest way as it is).
 //   K: [position][entry], scaled by a power of two per position that the scores take back (largest scale in [2^11, 2^12); scales below 2^-25 of a position's
 //      largest lose bits).
-//   V: [entry][position], as pairs of positions lie together in the words; its power of two is per group and follows its largest finite scale so far (scales
-//      below 2^-25 of it lose bits).
+//   V: [entry][position], as pairs of positions lie together in the words; its power of two is per group and follows its largest finite scale so far (a
+//      share with scales below 2^-25 of it: share_in_fp32).
 // Both are rows of 128 bytes with 16-byte chunks at the places that the 128-byte swizzle gives them; every store of eight lanes meets all banks.
 // Measured (32 query heads over 8 kv heads of 128 entries), with the kernel above beside it: 512 rows behind 3584 positions 97 us (206), a prompt of 2048 rows
 // 125 (252), 128 rows of four sequences of 4096 99 (182), 64 rows of one of 8192 39 (56), but of 16 sequences of 1024 47 (38); 32 rows, 128 columns, of four
@@ -550,6 +691,7 @@ struct Wide {
   static constexpr int BLOCK = q4::block_bytes(D);
   static constexpr int Q_BYTES = COLS * D * 2, HALF = PAGE * D * 2;  // widened K or V
   static constexpr int J = D / q4::kGroup;
+  static constexpr int RANGE = 25;  // as kRange: the widened values alone are fp16 here, the largest of 2^14, and a code times a scale has 11 bits
   struct Page {  // what a widened page is besides
     float factor[PAGE];
     float less[4];  // the groups' factors for O so far
@@ -573,7 +715,7 @@ __device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity) {
 }
 
 template <int D, bool CAP>
-__global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const AttnQ4Args a) {
+__global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const __grid_constant__ AttnQ4Args a) {
   using C = Wide<D>;
   constexpr int J = C::J;
   extern __shared__ uint8_t smem_raw[];
@@ -650,7 +792,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   constexpr uint32_t f16 = ~((1u << 7) | (1u << 10));  // (the descriptors' types)
   constexpr uint32_t idesc_s = umma_idesc_bf16(C::COLS, PAGE) & f16, idesc_o = umma_idesc_bf16(C::COLS, D) & f16;
   const bool leader = elect_one_sync();
-  bool ok = true;
+  bool ok = true, wide_range = false;
   float m = -INFINITY, l = 0.f;
   const uint32_t tmem_row = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes
 
@@ -809,8 +951,12 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       load_words<D>(vb + q4::code_bytes(D) + lane * (J * 4), vs);
     };
     int ex[J];
+    uint32_t low[W];
 #pragma unroll
-    for (int j = 0; j < J; ++j) ex[j] = 12;
+    for (int j = 0; j < J; ++j) {
+      ex[j] = 12;
+      low[j / 2] = kNoScale;
+    }
     auto add_values = [&](int i) {  // O += P V of page i
       const int st = i & 1, ph = (i >> 1) & 1;
       if (!wait_turn(&p_full[st], ph) || !wait_turn(&v_full[st], ph)) return false;
@@ -854,6 +1000,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
           y[k] = vs[W + k] & 0x7fff7fffu;
           const uint32_t fits = (uint32_t)(ex[2 * k] << 7 | ex[2 * k + 1] << 23) | 0x007f007fu;  // the largest numbers of the present exponents
           grow |= __vmaxu2(__vmaxu2(x[k], y[k]), fits) != fits;
+          low[k] = smallest_scale(low[k], x[k], y[k]);
         }
         grow = __any_sync(0xffffffffu, grow);
         if (grow) {
@@ -957,8 +1104,17 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       id = id_next;
     }
     for (int i = max(n_pages - 2, 0); i < n_pages && ok && warp == 7; ++i) ok = add_values(i);
+#pragma unroll
+    for (int j = 0; j < J; ++j) wide_range |= out_of_range(low[j / 2], j, ex[j], C::RANGE);
   }
+  tc_fence_before();
   const bool failed = __syncthreads_or(!ok);
+  if (__syncthreads_or(wide_range) && !failed) {
+    tc_fence_after();
+    if (warp == 7) tmem_dealloc(tmem, 256);
+    share_in_fp32<D, CAP>(a, ct, C::COLS, blockIdx.x);
+    return;
+  }
   tc_fence_after();
   float* sums = reinterpret_cast<float*>(smem);  // [column]: D sums, maximum, sum of weights, and 8 bytes that keep the rows aligned
   const bool done = shares == 1;

@@ -673,6 +673,96 @@ def test_portions_of_many_columns_captured_on_two_streams(L):
         assert torch.equal(args["out"], want)
 
 
+# (columns of a tile: up to 8, up to 16, 128)
+TILES = [(2, 1, 3), (4, 1, 4), (9, 3, 5), (8, 1, 40)]
+
+
+@pytest.mark.parametrize("up", [2, 12, 16, 17, 22, 26, 30, 100])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,rows", TILES)
+def test_attention_values_that_a_row_does_not_see_have_no_part_in_it(L, hq, hkv, rows, d, up):
+    """The last position's values are 2^up times the others' in one group: the rows before it see nothing of them."""
+    n = 200
+    k, v = (torch.randn(4, hkv, PAGE, d, generator=gen(80 + i), device=DEV) for i in range(2))
+    v[(n - 1) // PAGE, :, (n - 1) % PAGE, 32:64] *= 2.0 ** up
+    kp, vp = ref.make_plane(k.to(BF), True), ref.make_plane(v.to(BF), False)
+    q = torch.randn(rows, hq, d, generator=gen(82), device=DEV).to(BF)
+    table = torch.arange(4, device=DEV).int()[None]
+    want, mass = ref.attention(q, kp, vp, table, [n], [rows], d ** -0.5)
+    for split in (0, 1):
+        check_attn(attn(L, q, kp, vp, table, [n], [rows], d ** -0.5, split=split), want, mass, hq, d)
+
+
+@pytest.mark.parametrize("up", [10, 16, 17, 22, 30, 60])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,rows", [(1, 1, 1)] + TILES)
+def test_attention_large_values_of_no_weight_leave_the_others_as_they_are(L, hq, hkv, rows, d, up):
+    """One position's values are 2^up times the others', its weight e^-180 of theirs: every row sees it, and it counts next to nothing."""
+    n, at = 200, 70
+    base = torch.randn(hkv, 1, d, generator=gen(83), device=DEV)
+    q = (base + 0.1 * torch.randn(rows, hkv, hq // hkv, d, generator=gen(84), device=DEV)).view(rows, hq, d).to(BF)
+    k, v = (torch.randn(4, hkv, PAGE, d, generator=gen(85 + i), device=DEV) for i in range(2))
+    k[at // PAGE, :, at % PAGE] = -180 * base[:, 0] * d ** 0.5 / base[:, 0].square().sum(-1, keepdim=True)
+    kp, small = ref.make_plane(k.to(BF), True), ref.make_plane(v.to(BF), False)
+    v[at // PAGE, :, at % PAGE, :32] *= 2.0 ** up
+    vp = ref.make_plane(v.to(BF), False)
+    table = torch.arange(4, device=DEV).int()[None]
+    want, _ = ref.attention(q, kp, vp, table, [n], [rows], d ** -0.5)
+    other, mass = ref.attention(q, kp, small, table, [n], [rows], d ** -0.5)
+    assert torch.allclose(want, other, rtol=1e-12, atol=1e-12)  # (of the plain results)
+    for split in (0, 1):
+        check_attn(attn(L, q, kp, vp, table, [n], [rows], d ** -0.5, split=split), want, mass, hq, d)
+
+
+def mass_of(monkeypatch, *args):
+    """Sum of p |v|, nothing more: what a result's error goes by where values are far apart."""
+    real = ref.plane_values
+    with monkeypatch.context() as m:
+        m.setattr(ref, "plane_values", lambda plane, d, keys: real(plane, d, keys) if keys else real(plane, d, keys).abs())
+        return ref.attention(*args)[0]
+
+
+@pytest.mark.parametrize("window,softcap,sink", [(0, 0.0, False), (70, 0.0, True), (0, 20.0, True), (1, 30.0, False)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (8, 2, 128), (24, 2, 64)])
+@pytest.mark.parametrize("most", [1, 9, 140])
+def test_attention_of_values_far_apart(L, monkeypatch, hq, hkv, d, window, softcap, sink, most):
+    """Value scales from 2^-60 to 2^60 in no order: pages that are none, lengths of zero and one, more shares than one."""
+    lens = [1, 65, 130, 0, 700, 257, 64]
+    rows = [min(n, most) if i != 1 else 1 for i, n in enumerate(lens)]
+    kp, vp, table = cache(d + window, lens, hkv, d, spread=20.0)
+    table[4, 3], table[5, 0] = -1, kp.shape[0]
+    q = torch.randn(sum(rows) + 2, hq, d, generator=gen(86), device=DEV).to(BF)
+    sk = torch.randn(hq, generator=gen(87), device=DEV).to(BF) * 3 if sink else None
+    args = (q, kp, vp, table, lens, rows, d ** -0.5, window, softcap, sk)
+    want, mass = ref.attention(*args)[0], mass_of(monkeypatch, *args)
+    for split in (0, 1, 3):
+        out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, window, softcap, sk, split=split, ldo=hq * d + 8)
+        check_attn(out[:-2], want[:-2], mass[:-2], hq, d)
+        assert (out[-2:] == 9).all() and (out[:, hq * d:] == 9).all()
+
+
+@pytest.mark.parametrize("hq,hkv,rows", TILES)
+def test_attention_of_values_far_apart_keeps_infinities_and_nan_where_they_are_seen(L, monkeypatch, hq, hkv, rows):
+    d, lens = 128, [200, 200]
+    kp, vp, table = cache(88, lens, hkv, d, spread=20.0)
+    q = torch.randn(2 * rows, hq, d, generator=gen(89), device=DEV).to(BF)
+
+    def scale_at(plane, b, pos, h, group, value):
+        plane[int(table[b, pos // PAGE]), h, PAGE * d // 2 + ((pos % PAGE) * 4 + group) * 2:][:2] = torch.tensor([value], dtype=BF).view(torch.uint8).to(DEV)
+
+    scale_at(vp, 0, 199, 0, 1, float("nan"))
+    scale_at(vp, 0, 198, 0, 3, float("inf"))
+    scale_at(kp, 1, 199, hkv - 1, 2, float("nan"))
+    args = (q, kp, vp, table, lens, [rows, rows], d ** -0.5)
+    want, mass = ref.attention(*args)[0], mass_of(monkeypatch, *args)
+    fine = torch.isfinite(want)
+    assert fine[:rows - 2].all() and not fine[rows - 1, 0, 32:64].any() and fine[rows:2 * rows - 1].all()  # (of the plain result)
+    for split in (0, 1):
+        out = attn(L, q, kp, vp, table, lens, [rows, rows], d ** -0.5, split=split).view(-1, hq, d)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~fine & ~torch.isnan(want)].double(), want[~fine & ~torch.isnan(want)])
+        check_attn(torch.where(fine, out.double(), 0.0).flatten(1), torch.where(fine, want, 0.0), torch.where(fine, mass, 0.0), hq, d)
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
