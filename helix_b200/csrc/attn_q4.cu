@@ -67,6 +67,16 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// cap tanh(x / cap) as log2 of a weight.  tanh(y) = 1 - 2 / (e^2y + 1) takes two transcendentals and is off by some 2^-21 of the cap however small the score: 2^-15 of a
+// weight at kCapByExp, and more than the score itself from a cap of 10^7 on.  Above, tanh itself.
+constexpr float kCapByExp = 64.f;
+struct Cap {
+  float in, out;
+  __device__ __forceinline__ explicit Cap(float cap) : in(fminf(2.f * kLog2e / cap, 3e38f)), out(cap * kLog2e) {}  // (of a subnormal cap: no infinity, 0 stays 0)
+  __device__ __forceinline__ float by_exp(float x) const { return fmaf(-2.f * out, __fdividef(1.f, exp2_fast(x * in) + 1.f), out); }
+};
+__device__ __noinline__ float capped_far(float x, float cap) { return cap * tanhf(x / cap) * kLog2e; }
+
 // What a tile of columns of one sequence and kv head covers
 struct Tile {
   int row0;            // its first packed row; column c belongs to row0 + (rest + c) / G, head (rest + c) % G
@@ -222,9 +232,9 @@ __device__ __noinline__ void share_in_fp32(const AttnQ4Args& a, int ct, int cols
 #pragma unroll
         for (int n = 0; n < N; ++n) {
           float x = s[h][n] * a.scale;
-          if (CAP) x = a.softcap * tanhf(x / a.softcap);
+          x = CAP ? capped_far(x, a.softcap) : x * kLog2e;
           const bool sees = pos + h >= first[n] && pos + h <= last[n];
-          s[h][n] = sees ? x * kLog2e : -INFINITY;
+          s[h][n] = sees ? x : -INFINITY;
           seen[h][n] = __ballot_sync(0xffffffffu, sees);
         }
       }
@@ -444,14 +454,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
     }
     __syncwarp();  // K's slot is free: the next page's V
     fetch(a.v_cache, id_next, slot);
-    if constexpr (CAP) {  // cap tanh(x / cap) as log2 of a weight, tanh(y) = 1 - 2 / (e^2y + 1)
-      const float in = 2.f * kLog2e / a.softcap, out = a.softcap * kLog2e;
+    if constexpr (CAP) {  // as log2 of a weight
+      const Cap cap(a.softcap);
+      if (a.softcap <= kCapByExp) {
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk)
+        for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int h = 0; h < 4; ++h) s[blk][n][h] = fmaf(-2.f * out, __fdividef(1.f, exp2_fast(s[blk][n][h] * mul[n][h & 1] * in) + 1.f), out);
+            for (int h = 0; h < 4; ++h) s[blk][n][h] = cap.by_exp(s[blk][n][h] * mul[n][h & 1]);
+      } else {
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) s[blk][n][h] = capped_far(s[blk][n][h] * mul[n][h & 1], a.softcap);
+      }
     }
     if constexpr (!whole) {
 #pragma unroll
@@ -820,9 +839,14 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
         f2_unpack(f2_mul(f2_pack(s[x + 2], s[x + 3]), f2_pack(f.z, f.w)), s[x + 2], s[x + 3]);
       }
       if constexpr (CAP) {
-        const float in = 2.f * kLog2e / a.softcap, out = a.softcap * kLog2e;
+        const Cap cap(a.softcap);
+        if (a.softcap <= kCapByExp) {
 #pragma unroll
-        for (int x = 0; x < PAGE; ++x) s[x] = fmaf(-2.f * out, __fdividef(1.f, exp2_fast(s[x] * mul * in) + 1.f), out);
+          for (int x = 0; x < PAGE; ++x) s[x] = cap.by_exp(s[x] * mul);
+        } else {
+#pragma unroll
+          for (int x = 0; x < PAGE; ++x) s[x] = capped_far(s[x] * mul, a.softcap);
+        }
       }
       if (pg.id < 0 || !whole_at(pos)) {
         const int hi = pg.id < 0 ? -1 : last - pos, lo = first - pos;

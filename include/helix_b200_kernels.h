@@ -126,7 +126,7 @@ int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_
  * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096.  window, softcap and sink as in
  * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
  * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  Value scales may differ by
- * any factor; shares in which those of a group differ by more than 2^16 take some twenty times as long.  Entries of q below 2^-27 of the largest of their head's row
+ * any factor; shares in which those of a group differ by more than 2^16 take up to fifty times as long.  Entries of q below 2^-27 of the largest of their head's row
  * lose bits, and with 256 columns key scales below 2^-25 of the largest of their position.  split_pages: pages that one block
  * reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq / Hkv is 256 or more, on nothing else); 0:
  * hbk_attn_paged_q4_split's.  Single tokens beside portions of 256 columns (rows * Hq / Hkv) are quicker in a call of their own.  workspace: as many floats as

@@ -763,6 +763,19 @@ def test_attention_of_values_far_apart_keeps_infinities_and_nan_where_they_are_s
         check_attn(torch.where(fine, out.double(), 0.0).flatten(1), torch.where(fine, want, 0.0), torch.where(fine, mass, 0.0), hq, d)
 
 
+@pytest.mark.parametrize("softcap", [1e-39, 1e-30, 0.01, 60.0, 70.0, 300.0, 1e4, 1e7, 1e30, 3e38])
+@pytest.mark.parametrize("hq,hkv,rows", [(1, 1, 1)] + TILES)
+def test_attention_caps_of_any_size(L, hq, hkv, rows, softcap):
+    """Scores to some 60 on either side: a cap far above leaves them as they are, one far below makes all positions alike."""
+    d, lens = 64, [300, 65]
+    softcap = float(torch.tensor(softcap, dtype=torch.float32))
+    kp, vp, table = cache(90, lens, hkv, d)
+    q = (15 * torch.randn(2 * rows, hq, d, generator=gen(91), device=DEV)).to(BF)
+    want, mass = ref.attention(q, kp, vp, table, lens, [rows, rows], d ** -0.5, 0, softcap)
+    for split in (0, 1):
+        check_attn(attn(L, q, kp, vp, table, lens, [rows, rows], d ** -0.5, 0, softcap, split=split), want, mass, hq, d)
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
