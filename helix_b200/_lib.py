@@ -163,6 +163,8 @@ SIGNATURES = {
     "hbk_kv_q4_plane_bytes": (C.c_size_t, [I, I, I]),
     "hbk_kv_write_q4": (I, [P, I, P, I, P, P, P, P, I, P, I, I, I, I, I, I, P]),
     "hbk_attn_paged_q4": (I, [P, I, P, P, P, I, P, P, P, I, P, I, I, I, I, I, I, I, I, I, C.c_float, I, I, C.c_float, P, P]),
+    "hbk_attn_paged_q4_status": (I, []),
+    "hbk_attn_paged_q4_wait_cycles": (C.c_longlong, [C.c_longlong]),
     "hbk_attn_paged_q4_split": (I, [I, I, I, I, I, I, I]),
     "hbk_attn_paged_q4_workspace_floats": (C.c_size_t, [I, I, I, I, I, I, I, I, I]),
     "hbk_gemm_q4_bytes": (C.c_size_t, [I, I]),

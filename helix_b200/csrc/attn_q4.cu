@@ -722,12 +722,14 @@ struct Wide {
   static constexpr int SMEM = (END > 80 * 1024 ? END : 80 * 1024) + 1024;  // (two blocks per SM: tensor memory has room for no more)
   static_assert(sizeof(Page) <= 512 && COLS * (D + 4) * 4 <= PAGES);  // (the sums leave through the room of Q and the widened pages)
 };
-// False where the barrier has not turned after some seconds.  (A block that gives up writes NaN.)
-__device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity) {
-  bool ok = mbar_try_wait(bar, parity);
-  if (!ok) {
+// Set by a block that gave up a wait: attn_q4_status.  Its rows are NaN, its products in flight are waited for before their operands' room and its columns are given back.
+__device__ unsigned wait_ran_out;
+// False where the barrier has not turned after so many cycles (below 0: it is not looked at)
+__device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity, long long cycles) {
+  bool ok = cycles >= 0 && mbar_try_wait(bar, parity);
+  if (!ok && cycles > 0) {
     const long long t0 = clock64();
-    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < HB_WAIT_TIMEOUT_CYCLES) {
+    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < cycles) {
     }
   }
   return __all_sync(0xffffffffu, ok);
@@ -759,7 +761,8 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
   // keys there (page i: i & 3), values, scores, weights there, page done with (i & 1)
   uint64_t *k_full = bars, *v_full = bars + 4, *s_full = bars + 6, *p_full = bars + 8, *pv_done = bars + 10;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* all_done = bars + 12;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + 13);
   if (threadIdx.x == 128) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
@@ -769,6 +772,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
+    mbar_init(all_done, 4);
     fence_barrier_init();
   }
   if (warp == 7) {
@@ -821,7 +825,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
     const int last = c < tile.cols ? tile.pos0 + row_of(c) : -1, first = a.window > 0 ? last - a.window + 1 : 0;
     for (int i = 0; i < n_pages; ++i) {
       const int st = i & 1, ph = (i >> 1) & 1, pos = (p_begin + i) * PAGE;
-      if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1) && wait_turn(&s_full[st], ph))) break;
+      if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1, a.wait_cycles) && wait_turn(&s_full[st], ph, a.wait_cycles))) break;
       tc_fence_after();
       const typename C::Page& pg = *info_of(i);
       float s[PAGE];
@@ -867,7 +871,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
         m = x;
         l *= f;
         if (i > 0) {
-          if (!(ok = wait_turn(&pv_done[st ^ 1], ((i - 1) >> 1) & 1))) break;
+          if (!(ok = wait_turn(&pv_done[st ^ 1], ((i - 1) >> 1) & 1, a.wait_cycles))) break;
           tc_fence_after();
 #pragma unroll
           for (int j = 0; j < J; ++j) {
@@ -910,7 +914,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[st]);
       if (pg.bad) {  // infinities and NaN among value scales that not every column sees were widened as 0: for the columns that do, after the products
-        if (!(ok = wait_turn(&pv_done[st], ph))) break;
+        if (!(ok = wait_turn(&pv_done[st], ph, a.wait_cycles))) break;
         tc_fence_after();
         const uint8_t* vb = a.v_cache + ((size_t)pg.id * a.Hkv + kvh) * C::BLOCK;
         for (int j = 0; j < J; ++j)
@@ -935,7 +939,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
         tc_fence_before();  // (the next weights say that O may be added to)
       }
     }
-    if (ok) ok = wait_turn(&pv_done[(n_pages - 1) & 1], ((n_pages - 1) >> 1) & 1);
+    if (ok) ok = wait_turn(&pv_done[(n_pages - 1) & 1], ((n_pages - 1) >> 1) & 1, a.wait_cycles);
   } else {
     const int id_x = threadIdx.x - 128;
     const int32_t* table = a.page_table + (size_t)b * a.max_pages + p_begin;
@@ -983,7 +987,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
     }
     auto add_values = [&](int i) {  // O += P V of page i
       const int st = i & 1, ph = (i >> 1) & 1;
-      if (!wait_turn(&p_full[st], ph) || !wait_turn(&v_full[st], ph)) return false;
+      if (!wait_turn(&p_full[st], ph, a.wait_cycles) || !wait_turn(&v_full[st], ph, a.wait_cycles)) return false;
       tc_fence_after();
       if (leader) {
         const uint64_t vd = umma_desc_kmajor_sw128(smem_u32(smem + C::VALUES + st * C::HALF));
@@ -1001,7 +1005,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       const int st = i & 1, pos = (p_begin + i) * PAGE;
       const bool whole = whole_at(pos);
       const int id_next = number_of(i + 1);
-      if (i >= 2 && !(ok = wait_turn(&s_full[st], ((i - 2) >> 1) & 1))) break;
+      if (i >= 2 && !(ok = wait_turn(&s_full[st], ((i - 2) >> 1) & 1, a.wait_cycles))) break;
       typename C::Page& pg = *info_of(i);
       uint8_t* keys = smem + C::KEYS + st * C::HALF;
       uint8_t* values = smem + C::VALUES + st * C::HALF;
@@ -1092,9 +1096,9 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[i & 3]);
       if (i >= 2 && warp == 7 && !(ok = add_values(i - 2))) break;
-      if (i >= 2 && !(ok = wait_turn(&pv_done[st], ((i - 2) >> 1) & 1))) break;
+      if (i >= 2 && !(ok = wait_turn(&pv_done[st], ((i - 2) >> 1) & 1, a.wait_cycles))) break;
       if (warp == 4 + i % 3) {
-        if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1))) break;
+        if (!(ok = wait_turn(&k_full[i & 3], (i >> 2) & 1, a.wait_cycles))) break;
         tc_fence_after();
         if (leader) {
           const uint64_t qd = umma_desc_kmajor_sw128(smem_u32(smem)), kd = umma_desc_kmajor_sw128(smem_u32(keys));
@@ -1132,8 +1136,27 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
     for (int j = 0; j < J; ++j) wide_range |= out_of_range(low[j / 2], j, ex[j], C::RANGE);
   }
   tc_fence_before();
-  const bool failed = __syncthreads_or(!ok);
-  if (__syncthreads_or(wide_range) && !failed) {
+  if (__syncthreads_or(!ok)) {
+    if (warp >= 4 && leader) umma_commit(all_done);  // (turns when all that these four lanes have issued is done)
+    __syncwarp();
+    wait_turn(all_done, 0, HB_WAIT_TIMEOUT_CYCLES);
+    tc_fence_after();
+    const float nan = __uint_as_float(0x7fffffffu);
+    for (int i = threadIdx.x; i < tile.cols * (D + 2); i += C::THREADS) {
+      const int c = i / (D + 2), d = i % (D + 2), r = row_of(c), row = tile.row0 + r, head = kvh * G + tile.rest + c - r * G;
+      if (shares > 1) a.workspace[(((size_t)row * a.Hq + head) * a.max_splits + blockIdx.x) * (D + 4) + d] = nan;
+      else if (d < D) a.out[(size_t)row * a.ldo + (size_t)head * D + d] = __float2bfloat16(nan);
+    }
+    if (threadIdx.x == 0) wait_ran_out = 1;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 7) {
+      tc_fence_after();
+      tmem_dealloc(tmem, 256);
+    }
+    return;
+  }
+  if (__syncthreads_or(wide_range)) {
     tc_fence_after();
     if (warp == 7) tmem_dealloc(tmem, 256);
     share_in_fp32<D, CAP>(a, ct, C::COLS, blockIdx.x);
@@ -1146,7 +1169,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
     const int c = threadIdx.x, r = row_of(c);
     const float sink = done && a.sink && c < tile.cols ? __bfloat162float(a.sink[kvh * G + tile.rest + c - r * G]) * kLog2e : -INFINITY;
     const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.f : top;
-    const float f = failed ? __uint_as_float(0x7fffffffu) : exp2_fast(m - ref - 10.f);  // (sums are 2^10 times what they stand for)
+    const float f = exp2_fast(m - ref - 10.f);  // (sums are 2^10 times what they stand for)
 #pragma unroll
     for (int j = 0; j < 2 * J; ++j) {
       uint32_t o[16];
@@ -1393,6 +1416,19 @@ size_t attn_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int
   return p.max_splits > 1 ? (size_t)T * Hq * p.max_splits * (D + 4) : 0;
 }
 
+namespace {
+std::atomic<long long> wait_limit{HB_WAIT_TIMEOUT_CYCLES};
+}
+long long attn_q4_wait_cycles(long long cycles) { return wait_limit.exchange(cycles); }
+cudaError_t attn_q4_status() {
+  unsigned ran_out = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&ran_out, wait_ran_out, sizeof ran_out);
+  if (e != cudaSuccess || !ran_out) return e;
+  const unsigned none = 0;
+  e = cudaMemcpyToSymbol(wait_ran_out, &none, sizeof none);
+  return e == cudaSuccess ? cudaErrorLaunchTimeout : e;
+}
+
 cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   if (!sizes_ok(a.B, a.T, a.max_q_len, a.max_kv_len, a.Hq, a.Hkv, a.D, a.split_pages, a.window)) return cudaErrorInvalidValue;
   if (a.page_size != PAGE || a.num_pages < 1 || a.num_pages > INT32_MAX / PAGE || a.max_pages < 0 || !(a.softcap >= 0.f) || !(a.softcap < INFINITY) || !(fabsf(a.scale) < INFINITY))
@@ -1411,6 +1447,7 @@ cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   a.split_pages = p.split_pages;
   a.max_splits = p.max_splits;
   if (a.window >= a.max_kv_len) a.window = 0;  // every position is in it
+  a.wait_cycles = wait_limit.load(std::memory_order_relaxed);
   a.group = a.Hq / a.Hkv;
   a.inv_group = ((1ull << 32) + a.group - 1) / a.group;  // x inv >> 32 = x / group for x < 2^32 / group: columns of a tile and the rest before them
   a.kv_bound = (int)std::min<long long>((long long)a.max_pages * PAGE, a.max_kv_len);

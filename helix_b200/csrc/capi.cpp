@@ -409,6 +409,8 @@ int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v
   a.split_pages = split_pages; a.scale = scale; a.num_pages = num_pages; a.window = window; a.softcap = softcap; a.sink = (const hb::bf16*)sink;
   return kret(hb::attn_q4((cudaStream_t)stream, a));
 }
+int hbk_attn_paged_q4_status(void) { return kret(hb::attn_q4_status()); }
+long long hbk_attn_paged_q4_wait_cycles(long long cycles) { return hb::attn_q4_wait_cycles(cycles); }
 int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms) {
   return hb::attn_q4_split(B, max_q_len, max_kv_len, Hq, Hkv, window, sms);
 }

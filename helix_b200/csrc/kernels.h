@@ -286,8 +286,11 @@ struct AttnQ4Args {
   const bf16* sink;                    // [Hq] or NULL
   int max_splits, kv_bound, group;     // filled in by the launcher
   unsigned long long inv_group;
+  long long wait_cycles;
 };
 cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a);
+cudaError_t attn_q4_status();
+long long attn_q4_wait_cycles(long long cycles);
 int attn_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
 size_t attn_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
 

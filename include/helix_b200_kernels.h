@@ -134,6 +134,12 @@ int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_
 int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
                       const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
                       int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream);
+/* Calls with 256 columns wait inside the kernel for one another's parts.  A wait that takes some seconds is given up: the rows it was for are NaN, the kernel ends, and
+ * this says so: 0, or cudaErrorLaunchTimeout (702) where one was given up on the current device since it was last asked.  To be asked once the calls' stream is
+ * synchronised, and not while a stream is captured. */
+int hbk_attn_paged_q4_status(void);
+/* cycles after which such a wait is given up by the calls that follow (below 0: at once), of the whole process; returns the former */
+long long hbk_attn_paged_q4_wait_cycles(long long cycles);
 /* pages per block by the rule for `sms` SMs (0: the current device's); host arithmetic, -1 for refused sizes */
 int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
 size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);

@@ -96,3 +96,8 @@ def test_split_refusals():
     assert [L.hbk_attn_paged_q4_split(*a) for a in ((0, 1, 10, 8, 8, 0, 148), (1, 0, 10, 8, 8, 0, 148), (1, 1, -1, 8, 8, 0, 148), (1, 1, 10, 8, 3, 0, 148), (1, 1, 10, 8, 8, -1, 148),
                                                             (1, 1, 10, 8, 8, 0, -1))] == [-1] * 6
     assert L.hbk_attn_paged_q4_workspace_floats(1, 1, 1, 10, 8, 3, 128, 1, 0) == 0
+
+
+def test_the_limit_of_waits():
+    former = L.hbk_attn_paged_q4_wait_cycles(7)
+    assert former > 10 ** 9 and L.hbk_attn_paged_q4_wait_cycles(former) == 7

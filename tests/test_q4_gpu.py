@@ -776,6 +776,32 @@ def test_attention_caps_of_any_size(L, hq, hkv, rows, softcap):
         check_attn(attn(L, q, kp, vp, table, lens, [rows, rows], d ** -0.5, 0, softcap, split=split), want, mass, hq, d)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("split", [3, 100])
+def test_waits_that_run_out_end_the_call_and_are_said(L, d, split):
+    """A limit so short that the waits inside the kernel are given up: its rows are NaN, the status says so once, and the calls that follow are right."""
+    hq, hkv, lens, rows = 16, 2, [900, 64, 300], [64, 40, 1]
+    kp, vp, table = cache(92, lens, hkv, d)
+    T = sum(rows)
+    q = torch.randn(T + 2, hq, d, generator=gen(93), device=DEV).to(BF)
+    good = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split)
+    assert L.hbk_attn_paged_q4_status() == 0
+    former = L.hbk_attn_paged_q4_wait_cycles(-1)
+    try:
+        out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split)
+        assert torch.isnan(out[:T]).all() and (out[T:] == 9).all()
+        assert L.hbk_attn_paged_q4_status() == 702 and b"timed out" in L.hbk_last_error()
+        assert L.hbk_attn_paged_q4_status() == 0
+        for cycles in (0, 500, 2000, 8000):  # some waits go well
+            L.hbk_attn_paged_q4_wait_cycles(cycles)
+            out = attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split)
+            void = torch.isnan(out)
+            assert torch.equal(torch.where(void, 0, out), torch.where(void, 0, good)) and L.hbk_attn_paged_q4_status() == (702 if void.any() else 0)
+    finally:
+        L.hbk_attn_paged_q4_wait_cycles(former)
+    assert torch.equal(attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split), good) and L.hbk_attn_paged_q4_status() == 0
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
