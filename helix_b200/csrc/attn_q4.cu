@@ -1333,7 +1333,10 @@ struct Plan {
 // the lengths are uneven and more where they are even.
 // Tiles of 128 columns: as many shares as keep all blocks resident, two to an SM, of 64 pages at most (every share of a column costs its sums a way to memory and
 // back): 512 rows of one sequence of 4096 97 us in 32, 107 in 16, 192 in 4.  128 columns per tile from 256 columns on: see the kernel.
-Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int split_pages, int sms) {
+// No more shares than keep the workspace of T rows within 2^28 floats (one, and no workspace, where two would not; so many rows fill the machine many times over): 8192
+// rows of 131072 positions 30.9 ms in 7 shares with 1 GB, 37.1 in 32 with 4.4; 32768 rows of 32768 15.7 in one, 17.6 in 8 with 4.4 GB.
+Plan plan_of(int B, long long T, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int split_pages, int sms) {
+  constexpr long long kMostFloats = 1ll << 28;
   Plan p;
   const long long G = Hq / Hkv, most = G * max_q_len;
   p.cols = most >= 2 * kWideCols ? kWideCols : most > 8 ? 16 : 8;
@@ -1351,6 +1354,7 @@ Plan plan_of(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, 
       const long long most_pages = p.cols == 16 ? (items > 4LL * sms ? 32 : 16) : items * ((seen + 39) / 40) <= 4LL * sms ? 40 : 32;
       shares = std::max((5LL * sms / 3 + items - 1) / items, (seen + most_pages - 1) / most_pages);
     }
+    shares = std::min(shares, std::max(kMostFloats / std::max(T * Hq * (128 + 4), 1ll), 1ll));
     split_pages = (int)std::max<long long>((seen + shares - 1) / std::max(shares, 1LL), kWarps);
   }
   p.split_pages = split_pages;
@@ -1406,13 +1410,13 @@ cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
 int attn_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms) {
   if (!sizes_ok(B, 0, max_q_len, max_kv_len, Hq, Hkv, 128, 0, window) || sms < 0) return -1;
   if (sms == 0) sms = device_sms();
-  return sms > 0 ? plan_of(B, max_q_len, max_kv_len, Hq, Hkv, window, 0, sms).split_pages : -1;
+  return sms > 0 ? plan_of(B, (long long)B * max_q_len, max_q_len, max_kv_len, Hq, Hkv, window, 0, sms).split_pages : -1;
 }
 size_t attn_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window) {
   if (!sizes_ok(B, T, max_q_len, max_kv_len, Hq, Hkv, D, split_pages, window)) return 0;
   const int sms = split_pages > 0 ? 1 : device_sms();
   if (sms <= 0) return 0;
-  const Plan p = plan_of(B, max_q_len, max_kv_len, Hq, Hkv, window, split_pages, sms);
+  const Plan p = plan_of(B, T, max_q_len, max_kv_len, Hq, Hkv, window, split_pages, sms);
   return p.max_splits > 1 ? (size_t)T * Hq * p.max_splits * (D + 4) : 0;
 }
 
@@ -1441,7 +1445,7 @@ cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
     return cudaErrorInvalidValue;
   const int sms = a.split_pages > 0 ? 1 : device_sms();
   if (sms <= 0) return cudaErrorNoDevice;
-  const Plan p = plan_of(a.B, a.max_q_len, a.max_kv_len, a.Hq, a.Hkv, a.window, a.split_pages, sms);
+  const Plan p = plan_of(a.B, a.T, a.max_q_len, a.max_kv_len, a.Hq, a.Hkv, a.window, a.split_pages, sms);
   if (p.max_splits > 1 && (!a.workspace || ((uintptr_t)a.workspace & 15))) return cudaErrorInvalidValue;
   if ((long long)p.tiles * a.Hkv > 65535) return cudaErrorInvalidValue;
   a.split_pages = p.split_pages;

@@ -140,7 +140,8 @@ int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v
 int hbk_attn_paged_q4_status(void);
 /* cycles after which such a wait is given up by the calls that follow (below 0: at once), of the whole process; returns the former */
 long long hbk_attn_paged_q4_wait_cycles(long long cycles);
-/* pages per block by the rule for `sms` SMs (0: the current device's); host arithmetic, -1 for refused sizes */
+/* pages per block by the rule for `sms` SMs (0: the current device's) and T = B * max_q_len rows (where a call has fewer, its own rule may take shorter shares: the
+ * rule keeps the workspace within 2^28 floats); host arithmetic, -1 for refused sizes */
 int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
 size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
 /* 4-bit weights: N rows of K / 32 GGUF Q4_0 blocks (18 bytes: fp16 d, then byte i with entries i and i + 16; device memory) laid out as the product reads them, in

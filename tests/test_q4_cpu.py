@@ -101,3 +101,22 @@ def test_split_refusals():
 def test_the_limit_of_waits():
     former = L.hbk_attn_paged_q4_wait_cycles(7)
     assert former > 10 ** 9 and L.hbk_attn_paged_q4_wait_cycles(former) == 7
+
+
+@pytest.mark.parametrize("B,rows,longest,hq,hkv,d,window", [(1, 8192, 131072, 32, 8, 128, 0), (1, 131072, 131072, 32, 8, 128, 0), (1, 131072, 131072, 64, 8, 64, 0), (4, 32768, 131072, 32, 8, 128, 0),
+                                                            (64, 63, 131072, 32, 8, 128, 0), (1, 50000, 2 ** 20, 16, 1, 128, 0), (512, 8, 131072, 32, 8, 128, 0), (1, 65536, 131072, 32, 8, 128, 9000),
+                                                            (1024, 1, 131072, 128, 8, 128, 0)])
+def test_the_rule_bounds_the_workspace(B, rows, longest, hq, hkv, d, window):
+    """By the rule a call of many rows has shares as long as keep the workspace within a GiB, and none where two to a column would already take more."""
+    split = L.hbk_attn_paged_q4_split(B, rows, longest, hq, hkv, window, 148)
+    n = L.hbk_attn_paged_q4_workspace_floats(B, B * rows, rows, longest, hq, hkv, d, split, window)
+    assert split >= 4 and 0 <= n <= 2 ** 28
+    column = B * rows * hq * 132
+    if n == 0:
+        assert 2 * column > 2 ** 28
+
+
+@pytest.mark.parametrize("B,rows,longest,hq,hkv,window,split", [(1, 512, 4096, 32, 8, 0, 32), (3, 97, 5000, 12, 2, 0, 9), (1, 2048, 2048, 32, 8, 0, 32), (1, 2048, 65536, 32, 8, 0, 64),
+                                                               (16, 64, 131072, 32, 8, 0, 64), (3, 1, 131000, 32, 8, 0, 32), (32, 1, 2176, 32, 8, 0, 34)])
+def test_the_rule_elsewhere_is_as_it_was(B, rows, longest, hq, hkv, window, split):
+    assert L.hbk_attn_paged_q4_split(B, rows, longest, hq, hkv, window, 148) == split
