@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::BLOCKS) attn_q4_kernel(c
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = a.group;
-  const int b = blockIdx.z, ct = blockIdx.y / a.Hkv, kvh = blockIdx.y - ct * a.Hkv;
+  const int b = blockIdx.z, ct = a.tile0 + blockIdx.y / a.Hkv, kvh = blockIdx.y % a.Hkv;
   const Tile tile = tile_of(a, b, ct, C::COLS);
   if (tile.cols <= 0) return;
   auto row_of = [&](int c) { return div_g(a, tile.rest + c); };  // row of column c
@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(Wide<D>::THREADS, 2) attn_q4_wide_kernel(const
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.group;
-  const int b = blockIdx.z, ct = blockIdx.y / a.Hkv, kvh = blockIdx.y - ct * a.Hkv;
+  const int b = blockIdx.z, ct = a.tile0 + blockIdx.y / a.Hkv, kvh = blockIdx.y % a.Hkv;
   const Tile tile = tile_of(a, b, ct, C::COLS);
   if (tile.cols <= 0) return;
   auto row_of = [&](int c) { return div_g(a, tile.rest + c); };
@@ -1322,6 +1322,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const AttnQ4Args
   }
 }
 
+constexpr int kMostGridY = 65535;
 struct Plan {
   int split_pages, max_splits, tiles, cols;
 };
@@ -1367,7 +1368,7 @@ int device_sms() {
   return effective_sms(sms);
 }
 bool sizes_ok(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window) {
-  return B >= 1 && B <= 65535 && T >= 0 && max_q_len >= 1 && max_kv_len >= 0 && max_kv_len <= INT32_MAX - 2 * PAGE && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 &&
+  return B >= 1 && B <= 65535 && T >= 0 && max_q_len >= 1 && max_kv_len >= 0 && max_kv_len <= INT32_MAX - 2 * PAGE && Hkv >= 1 && Hkv <= kMostGridY && Hq >= Hkv && Hq % Hkv == 0 &&
          (long long)max_q_len * Hq <= INT32_MAX / 2 && (D == 64 || D == 128) && (long long)Hq * D <= INT32_MAX && Hq / Hkv <= 4096 && split_pages >= 0 && split_pages <= 1 << 24 && window >= 0;
 }
 
@@ -1384,10 +1385,11 @@ cudaError_t allow_smem(int bytes) {
   return e;
 }
 template <auto kernel, int D>
-cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p, int smem, int threads = kThreads) {
+cudaError_t launch(cudaStream_t stream, AttnQ4Args& a, const Plan& p, int smem, int threads = kThreads) {
   cudaError_t e = allow_smem<kernel>(smem);
-  if (e != cudaSuccess) return e;
-  e = launch_k(kernel, dim3(p.max_splits, p.tiles * a.Hkv, a.B), dim3(threads), smem, stream, true, a);
+  const int tiles = kMostGridY / a.Hkv;  // of a launch
+  for (a.tile0 = 0; e == cudaSuccess && a.tile0 < p.tiles; a.tile0 += tiles)
+    e = launch_k(kernel, dim3(p.max_splits, std::min(tiles, p.tiles - a.tile0) * a.Hkv, a.B), dim3(threads), smem, stream, true, a);
   if (e != cudaSuccess || p.max_splits == 1) return e;
   const long long at_most = (long long)a.max_q_len * a.Hq;  // rows and heads of a sequence
   if (at_most * a.B >= 4096)
@@ -1395,13 +1397,13 @@ cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p, int 
   return launch_k(attn_q4_join_kernel<D, kWarps>, dim3((unsigned)at_most, a.B), dim3(kThreads), 0, stream, true, a, p.cols);
 }
 template <int D, bool CAP>
-cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
+cudaError_t launch(cudaStream_t stream, AttnQ4Args& a, const Plan& p) {
   if (p.cols == kWideCols) return launch<attn_q4_wide_kernel<D, CAP>, D>(stream, a, p, Wide<D>::SMEM, Wide<D>::THREADS);
   if (p.cols == 16) return launch<attn_q4_kernel<D, 2, CAP>, D>(stream, a, p, Cfg<D, 2>::SMEM);
   return launch<attn_q4_kernel<D, 1, CAP>, D>(stream, a, p, Cfg<D, 1>::SMEM);
 }
 template <int D>
-cudaError_t launch(cudaStream_t stream, const AttnQ4Args& a, const Plan& p) {
+cudaError_t launch(cudaStream_t stream, AttnQ4Args& a, const Plan& p) {
   return a.softcap > 0.f ? launch<D, true>(stream, a, p) : launch<D, false>(stream, a, p);
 }
 
@@ -1447,7 +1449,6 @@ cudaError_t attn_q4(cudaStream_t stream, AttnQ4Args a) {
   if (sms <= 0) return cudaErrorNoDevice;
   const Plan p = plan_of(a.B, a.T, a.max_q_len, a.max_kv_len, a.Hq, a.Hkv, a.window, a.split_pages, sms);
   if (p.max_splits > 1 && (!a.workspace || ((uintptr_t)a.workspace & 15))) return cudaErrorInvalidValue;
-  if ((long long)p.tiles * a.Hkv > 65535) return cudaErrorInvalidValue;
   a.split_pages = p.split_pages;
   a.max_splits = p.max_splits;
   if (a.window >= a.max_kv_len) a.window = 0;  // every position is in it

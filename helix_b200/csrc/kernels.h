@@ -284,7 +284,7 @@ struct AttnQ4Args {
   int num_pages, window;
   float softcap;
   const bf16* sink;                    // [Hq] or NULL
-  int max_splits, kv_bound, group;     // filled in by the launcher
+  int max_splits, kv_bound, group, tile0;  // filled in by the launcher
   unsigned long long inv_group;
   long long wait_cycles;
 };

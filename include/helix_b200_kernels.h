@@ -123,7 +123,7 @@ size_t hbk_kv_q4_plane_bytes(int num_pages, int Hkv, int D); /* 0: refused sizes
 int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_t* slot_mapping, void* k_cache, void* v_cache, void* k_seen, int ldks,
                     void* v_seen, int ldvs, int T, int Hkv, int D, int page_size, int num_pages, void* stream);
 /* Attention over such planes: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q are the last positions of the kv_lens[b]-long sequence b (at most max_q_len of them;
- * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096.  window, softcap and sink as in
+ * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096, Hkv up to 65535, max_q_len * Hq up to 2^30.  window, softcap and sink as in
  * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
  * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  Value scales may differ by
  * any factor; shares in which those of a group differ by more than 2^16 take up to fifty times as long.  Entries of q below 2^-27 of the largest of their head's row

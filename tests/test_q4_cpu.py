@@ -120,3 +120,10 @@ def test_the_rule_bounds_the_workspace(B, rows, longest, hq, hkv, d, window):
                                                                (16, 64, 131072, 32, 8, 0, 64), (3, 1, 131000, 32, 8, 0, 32), (32, 1, 2176, 32, 8, 0, 34)])
 def test_the_rule_elsewhere_is_as_it_was(B, rows, longest, hq, hkv, window, split):
     assert L.hbk_attn_paged_q4_split(B, rows, longest, hq, hkv, window, 148) == split
+
+
+def test_sizes_that_the_call_refuses_have_no_split_and_no_workspace():
+    assert attn(hq=65536, hkv=65536, ldq=2 ** 23, ldo=2 ** 23) == 1
+    for hq, rows in ((65536, 1), (65535, 2 ** 15)):
+        assert L.hbk_attn_paged_q4_split(1, rows, 1000, hq, hq, 0, 148) == -1 and L.hbk_attn_paged_q4_workspace_floats(1, 1, rows, 1000, hq, hq, 64, 4, 0) == 0
+    assert L.hbk_attn_paged_q4_split(1, 131072, 131072, 64, 8, 0, 148) == 2048 and L.hbk_attn_paged_q4_split(1, 1, 1000, 65535, 65535, 0, 148) > 0

@@ -802,6 +802,25 @@ def test_waits_that_run_out_end_the_call_and_are_said(L, d, split):
     assert torch.equal(attn(L, q, kp, vp, table, lens, rows, d ** -0.5, split=split), good) and L.hbk_attn_paged_q4_status() == 0
 
 
+@pytest.mark.parametrize("hkv,rows,most", [(8192, 150, 200), (16400, 400, 600)])
+def test_attention_of_more_tiles_and_heads_than_a_launch_has_room_for(L, hkv, rows, most):
+    """Tiles times kv heads above 65535, with 16 and with 128 columns per tile: a few of the heads in 64 bits, and with the bits that they have by themselves."""
+    d, n = 64, rows + 30
+    pages = -(-n // PAGE)
+    kp, vp = (torch.randint(0, 256, (pages, hkv, PAGE * d // 2 + PAGE * d // 16), generator=gen(94 + i), device=DEV, dtype=torch.uint8) for i in range(2))
+    for plane in (kp, vp):
+        plane[..., PAGE * d // 2:] = (0.2 * torch.randn(pages, hkv, PAGE * d // 32, generator=gen(96), device=DEV)).to(BF).view(torch.uint8)
+    q = torch.randn(rows, hkv, d, generator=gen(97), device=DEV, dtype=BF)
+    table = torch.randperm(pages, generator=gen(98), device=DEV).int()[None]
+    for split in (3, 100):
+        out = attn(L, q, kp, vp, table, [n], [rows], d ** -0.5, split=split, most=most).view(rows, hkv, d)
+        for h in (0, hkv // 3, hkv - 1):
+            one = [x[:, h:h + 1].contiguous() for x in (q, kp, vp)]
+            got = out[:, h].contiguous()
+            check_attn(got, *ref.attention(*one, table, [n], [rows], d ** -0.5), 1, d)
+            assert torch.equal(got, attn(L, *one, table, [n], [rows], d ** -0.5, split=split, most=most))
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
