@@ -127,3 +127,32 @@ def test_sizes_that_the_call_refuses_have_no_split_and_no_workspace():
     for hq, rows in ((65536, 1), (65535, 2 ** 15)):
         assert L.hbk_attn_paged_q4_split(1, rows, 1000, hq, hq, 0, 148) == -1 and L.hbk_attn_paged_q4_workspace_floats(1, 1, rows, 1000, hq, hq, 64, 4, 0) == 0
     assert L.hbk_attn_paged_q4_split(1, 131072, 131072, 64, 8, 0, 148) == 2048 and L.hbk_attn_paged_q4_split(1, 1, 1000, 65535, 65535, 0, 148) > 0
+
+
+@pytest.mark.parametrize("B,most,longest,hq,hkv,window", [(3, 97, 5000, 12, 2, 0), (1, 300, 70000, 9, 3, 100), (1, 300, 70000, 9, 3, 20), (1, 2048, 2048, 32, 8, 0), (2, 512, 40000, 32, 8, 1),
+                                                         (1, 40, 9000, 56, 7, 4033), (1, 700, 3000, 5, 5, 64), (4, 100, 70000, 40, 1, 63), (1, 1, 3000, 300, 1, 65), (1, 256, 5000, 1, 1, 1000),
+                                                         (1, 8192, 131072, 32, 8, 0), (1, 8192, 131072, 32, 8, 30000), (2, 3, 20000, 4096, 1, 129), (5, 60, 3000, 12, 4, 127), (1, 20, 4000, 12, 1, 62)])
+def test_shares_of_wide_tiles_fit_the_workspace(B, most, longest, hq, hkv, window):
+    """Tiles of 128 columns from 256 columns on, of 16 or 8 below: no tile of any sequence has more shares than its columns have room for, by the rule and with splits of one's
+    own; windows that end on, before and behind a page's edge."""
+    group = hq // hkv
+    cols = 128 if group * most >= 256 else 16 if group * most > 8 else 8
+    rule = L.hbk_attn_paged_q4_split(B, most, longest, hq, hkv, window, 148)
+    for split in (rule, 1, 2, 3, 7):
+        n = L.hbk_attn_paged_q4_workspace_floats(B, B * most, most, longest, hq, hkv, 128, split, window)
+        column = B * most * hq * 132
+        assert n % column == 0
+        shares = max(n // column, 1)
+        worst = 0
+        for rows in {most, most // 2 + 1, 1}:
+            for length in {longest - i for i in (0, 1, 2, 31, 32, 63, 64, 65)} | {longest // 2, most, most + window, min(longest, split * 64 + 1)}:
+                if not 0 < length <= longest:
+                    continue
+                tiles = range(0, group * rows, cols)
+                for c0 in (list(tiles) if len(tiles) < 80 else list(tiles[:40]) + list(tiles[-40:])):
+                    first, last = c0 // group, (min(c0 + cols, group * rows) - 1) // group
+                    hi = min(max(length - rows + last + 1, 0), length)
+                    lo = max(length - rows + first - window + 1, 0) if window else 0
+                    if hi > lo:
+                        worst = max(worst, -(-(-(-hi // 64) - lo // 64) // split))
+        assert 0 < worst <= shares and shares <= worst + 1, (split, worst, shares)  # (nor does it have room for many that are none)

@@ -821,6 +821,25 @@ def test_attention_of_more_tiles_and_heads_than_a_launch_has_room_for(L, hkv, ro
             assert torch.equal(got, attn(L, *one, table, [n], [rows], d ** -0.5, split=split, most=most))
 
 
+@pytest.mark.parametrize("hq,hkv,rows", TILES)
+@pytest.mark.parametrize("up", [2.0 ** 100, 2.0 ** -100])
+def test_attention_one_query_entry_far_above_the_others(L, hq, hkv, rows, up):
+    """Against keys that are 0 there it adds nothing, against others it decides: results, not only that they are finite."""
+    d, lens = 128, [400, 70]
+    k, v = (torch.randn(10, hkv, PAGE, d, generator=gen(100 + i), device=DEV) for i in range(2))
+    q = torch.randn(2 * rows, hq, d, generator=gen(102), device=DEV) * up
+    q[:, 0], q[:, 0, 3] = 0, up
+    k[:, 0, :, 3] = 0
+    k /= up
+    k[5:, :, :, 3] = 0.25 / up  # of the second sequence
+    kp, vp = ref.make_plane(k.to(BF), True), ref.make_plane(v.to(BF), False)
+    q = q.to(BF)
+    table = ints([[0, 1, 2, 3, 4, 9, 8], [5, 6, -1, -1, -1, -1, -1]])
+    want, mass = ref.attention(q, kp, vp, table, lens, [rows, rows], d ** -0.5)
+    for split in (0, 1):
+        check_attn(attn(L, q, kp, vp, table, lens, [rows, rows], d ** -0.5, split=split), want, mass, hq, d)
+
+
 # ------------------------------------------------------------------ products
 def product(L, x, w, N, K, epi, out=None, r=None, bias=None, pack=True):
     M = x.shape[0]
@@ -900,6 +919,23 @@ def test_product_keeps_infinities_and_nan_in_their_rows(L):
     assert torch.isnan(out[2]).all() and not torch.isfinite(out[8]).any()
     want = torch.where(vals[:, 200] == 0, float("nan"), torch.sign(vals[:, 200]) * float("inf")).float()
     assert torch.equal(torch.nan_to_num(out[8], nan=1.0), torch.nan_to_num(want, nan=1.0))
+
+
+@pytest.mark.parametrize("M", [1, 4, 13, 32])
+def test_product_of_any_bytes_in_fp32(L, M):
+    """Random blocks, a result in fp32: its own rounding hides nothing."""
+    N, K = 200, 1280
+    c = torch.randint(0, 16, (N, K // 32, 32), generator=gen(106), device=DEV)
+    s = torch.randn(N, K // 32, generator=gen(107), device=DEV).to(torch.float16)
+    s[::3] *= 2.0 ** -14
+    s[::7] = 6e-8
+    s[::11] = 0
+    x = torch.randn(M, K, generator=gen(108), device=DEV).to(BF)
+    out = product(L, x, ref.blocks_of(c, s), N, K, 6)[:M, :N]
+    w = ((c - 8).double() * s.double()[..., None]).flatten(1)
+    check_product(out, x, w, 6)
+    for rows in (slice(0, None, 3), slice(0, None, 7)):  # the small ones by themselves
+        check_product(out[:, rows], x, w[rows], 6)
 
 
 # ------------------------------------------------------------------ together
