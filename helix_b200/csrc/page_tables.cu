@@ -161,7 +161,7 @@ cudaError_t page_tables(cudaStream_t stream, const PageTableArgs& a) {
   if (!a.ctx_lens || !a.new_lens || !a.page_table || !a.free_pages || !a.free_count || !a.free_left || !a.cu_seqlens || !a.kv_lens || !a.positions ||
       !a.slot_mapping)
     return cudaErrorInvalidValue;
-  if (a.B < 1 || a.B > kMaxReqs || a.T < 0 || a.max_pages < 1 || a.max_pages > INT32_MAX / kPage || a.num_pages < 1 || a.num_pages > INT32_MAX / kPage || a.page_size != kPage)
+  if (a.B < 1 || a.B > kMaxReqs || a.T < 0 || a.T > 1 << 30 || a.max_pages < 1 || a.max_pages > INT32_MAX / kPage || a.num_pages < 1 || a.num_pages > INT32_MAX / kPage || a.page_size != kPage)
     return cudaErrorInvalidValue;
   // few rows: one block; many: blocks of a row per thread, or a cluster where the lengths or the stack's height are overwritten
   const bool small = a.B <= 256 * kPer && a.T <= 1024, over = a.kv_lens == a.ctx_lens || a.free_left == a.free_count;

@@ -108,7 +108,7 @@ size_t hbk_attn_decode_workspace_floats(int B, int Hq, int D, int num_splits);
  * 0 for a request that has ended; positions [T] and slot_mapping [T] (page * 64 + place), 0 and -1 behind the last token.
  * A request that does not fit (more than max_pages pages, rows past T, or the first that finds too few pages and every later one that needs some) takes no page:
  * kv_lens[b] = ctx_lens[b] says so, and its rows have slot -1.  free_left may be free_count and kv_lens may be ctx_lens; nothing else may overlap.
- * free_pages has room for num_pages entries.  1 <= B <= 2048, page_size 64.  Lengths below 0 in ctx_lens count as 0. */
+ * free_pages has room for num_pages entries.  1 <= B <= 2048, T up to 2^30, page_size 64.  Lengths below 0 in ctx_lens count as 0. */
 int hbk_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int max_pages, int32_t* free_pages,
                     const int32_t* free_count, int32_t* free_left, int num_pages, int32_t* cu_seqlens, int32_t* kv_lens, int32_t* positions,
                     int32_t* slot_mapping, int T, int page_size, void* stream);

@@ -20,6 +20,10 @@ def test_page_tables_refusals(kw):
     assert tables(**kw) == 1 and b"invalid argument" in L.hbk_last_error()
 
 
+def test_page_tables_rows_that_indices_do_not_reach():
+    assert tables(T=2 ** 30 + 1) == 1 and tables(T=2 ** 31 - 1) == 1
+
+
 def write(k=OK, ldk=256, v=OK, ldv=256, slots=OK, kc=OK, vc=OK, ks=None, ldks=0, vs=None, ldvs=0, T=3, hkv=2, d=128, page=64, pages=10):
     return L.hbk_kv_write_q4(k, ldk, v, ldv, slots, kc, vc, ks, ldks, vs, ldvs, T, hkv, d, page, pages, None)
 
