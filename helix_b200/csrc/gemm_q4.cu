@@ -214,7 +214,6 @@ cudaError_t launch_q4(cudaStream_t stream, const GemmQ4Args& a, int sms) {
   }
   if (e != cudaSuccess) return e;
   const int blocks_n = (a.N + ROWS - 1) / ROWS, tiles_m = (a.M + C::COLS - 1) / C::COLS, kt_all = (a.K + TK - 1) / TK;
-  if (blocks_n > 65535) return cudaErrorInvalidValue;
   // Parts of K: twice as many while that leaves no more than some seven blocks per SM and four tiles per part.  Eight blocks join their sums slowly: only
   // where few blocks run, or where the tiles of 16 and more rows of x are slower still.  us: 1 x 4096 x 4096 12.8 in one part, 7.3 in 2, 5.9 in 4, 6.6 in 8;
   // 8 x 4096 x 14336 13.3 in 4, 15.4 in 8; 32 x 4096 x 14336 24.2 in 4, 22.2 in 8; 1 x 28672 x 4096 26.5 in one, 19.1 in 2, 19.8 in 4.
@@ -245,7 +244,7 @@ cudaError_t launch_q4(cudaStream_t stream, const GemmQ4Args& a, int sms) {
 }
 
 size_t tiles_of(int N, int K) { return (size_t)((N + TN - 1) / TN) * ((K + TK - 1) / TK); }
-bool weights_ok(int N, int K) { return N >= 1 && K >= 32 && K % 32 == 0 && N <= INT32_MAX - TN && K <= INT32_MAX - TK; }
+bool weights_ok(int N, int K) { return N >= 1 && K >= 32 && K % 32 == 0 && N <= 65535 * ROWS && K <= (1 << 30) - TK; }  // (blocks of a grid; bytes of a row of x in 32 bits)
 
 }  // namespace
 

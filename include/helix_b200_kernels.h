@@ -145,11 +145,11 @@ long long hbk_attn_paged_q4_wait_cycles(long long cycles);
 int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
 size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
 /* 4-bit weights: N rows of K / 32 GGUF Q4_0 blocks (18 bytes: fp16 d, then byte i with entries i and i + 16; device memory) laid out as the product reads them, in
- * hbk_gemm_q4_bytes(N, K) bytes (K a multiple of 32): tiles [ceil(N / 16)][ceil(K / 128)] of 16 rows of 64 bytes as K codes above with D = 128, then
+ * hbk_gemm_q4_bytes(N, K) bytes (K a multiple of 32 up to 2^30 - 128, N up to 65535 * 64): tiles [ceil(N / 16)][ceil(K / 128)] of 16 rows of 64 bytes as K codes above with D = 128, then
  * [16 rows][4 groups] fp16 scales. */
 size_t hbk_gemm_q4_bytes(int N, int K); /* 0: refused sizes */
 int hbk_gemm_q4_pack(const void* blocks, void* packed, int N, int K, void* stream);
-/* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 32 rows hbk_gemm with bf16 weights is quicker), N up to 65535 * 64; epi as in hbk_gemm: 0, 1, 3, 4
+/* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 32 rows hbk_gemm with bf16 weights is quicker); epi as in hbk_gemm: 0, 1, 3, 4
  * (bf16 out) or 6 (fp32 out); R may be out itself */
 int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, const void* R, int ldr, const void* bias, int M, int N, int K, int epi,
                 void* stream);

@@ -24,6 +24,13 @@ def test_page_tables_rows_that_indices_do_not_reach():
     assert tables(T=2 ** 30 + 1) == 1 and tables(T=2 ** 31 - 1) == 1
 
 
+@pytest.mark.parametrize("N,K", [(16, 2 ** 30), (16, 2 ** 31 - 32), (65535 * 64 + 1, 32), (2 ** 31 - 1, 128)])
+def test_weights_beyond_the_products_sizes(N, K):
+    """Refused by the size, the packing and the product alike."""
+    assert L.hbk_gemm_q4_bytes(N, K) == 0 and L.hbk_gemm_q4_pack(OK, OK, N, K, None) == 1 and gemm(N=N, K=K, ldx=2 ** 31 - 8, ldo=2 ** 31 - 1) == 1
+    assert L.hbk_gemm_q4_bytes(65535 * 64, 128) == 65535 * 64 * 72 and L.hbk_gemm_q4_bytes(16, 2 ** 30 - 128) == (2 ** 30 - 128) * 9
+
+
 def write(k=OK, ldk=256, v=OK, ldv=256, slots=OK, kc=OK, vc=OK, ks=None, ldks=0, vs=None, ldvs=0, T=3, hkv=2, d=128, page=64, pages=10):
     return L.hbk_kv_write_q4(k, ldk, v, ldv, slots, kc, vc, ks, ldks, vs, ldvs, T, hkv, d, page, pages, None)
 
