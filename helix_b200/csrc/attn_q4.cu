@@ -26,7 +26,7 @@
 // Measured (8 kv heads of 128 entries, 32 query heads): 32 sequences of 1.5k to 2.2k positions 25 us (68 MB, 41 % of the copy rate: two blocks on most SMs
 // and one on the others, some 5 us of launch, first loads and last sums), 74 of 2k 39 us, 32 of 8k 66 us (302 MB, 70 %: 18.5 instructions per position and kv
 // head at 65 % of the issue slots; parts left out in a copy, at 2k: 7 % less without the loads, 12 % without the 8 taken off the codes, 2 % without V's
-// products), three of 9k to 131k 60 us (242 MB, 62 %).  Also tried: scores in shared memory and rolled loops (a fifth more instructions), e4m3 products (widened to
+// products), three of 9k to 131k 60 us (242 MB, 61 %; 67 on another GPU).  Also tried: scores in shared memory and rolled loops (a fifth more instructions), e4m3 products (widened to
 // fp16 by further instructions on this chip: 41 -> 52), pages dealt evenly over all blocks by the launch's lengths (two runs of pages per block: 26 -> 37), clusters
 // that join their sums through distributed shared memory (one sequence of 2k 6.4 -> 7.2, 32 of 8k 66 -> 77).
 #include <math.h>
@@ -710,7 +710,7 @@ struct Wide {
   static constexpr int BLOCK = q4::block_bytes(D);
   static constexpr int Q_BYTES = COLS * D * 2, HALF = PAGE * D * 2;  // widened K or V
   static constexpr int J = D / q4::kGroup;
-  static constexpr int RANGE = 25;  // as kRange: the widened values alone are fp16 here, the largest of 2^14, and a code times a scale has 11 bits
+  static constexpr int RANGE = 25;  // as kRange: the widened values alone are fp16 here, below 2^15, and a code times a scale has 11 bits
   struct Page {  // what a widened page is besides
     float factor[PAGE];
     float less[4];  // the groups' factors for O so far

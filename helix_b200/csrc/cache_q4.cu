@@ -7,7 +7,7 @@
 // Eight entries per thread (one 16-byte load), four threads per group.  Their codes fill one word of the key layout and two half words of the
 // value layout; no byte is shared by two positions, so rows of one page may be written by any threads in any order.
 //
-// Instructions bound it: 16,001 rows of 8 heads of 128 entries with the rows written back (149 MB) 30 us, 76 % of the copy rate (one key per entry that
+// Instructions bound it: 16,001 rows of 8 heads of 128 entries with the rows written back (149 MB) 30.2 us, 76 % of the copy rate (one key per entry that
 // orders magnitude, place and sign, and half words stored singly: 38; packed maxima: 33).
 #include "kernels.h"
 #include "launch.h"

@@ -99,7 +99,7 @@ size_t hbk_attn_decode_workspace_floats(int B, int Hq, int D, int num_splits);
 /* ---- a step whose cache and weights are held in 4 bits.  32 neighbouring entries share a scale d and a code c in 0..15 stands for d (c - 8); with m the
  * entry of largest magnitude (the first of equals) d = m / -8 rounded, c = clamp(floor(x / d + 1/2) + 8, 0, 15), 8 where d = 0.  These calls take the
  * stream they run on (NULL: the legacy default stream), allocate nothing, never wait, and can be captured into a graph; a call's buffers must be on the
- * current device.  Row strides count entries and are multiples of 8, rows of bf16 read in whole begin on 16 bytes.
+ * current device, and outputs overlap no input but where it is said.  Row strides count entries and are multiples of 8, rows of bf16 read in whole begin on 16 bytes.
  *
  * Page tables, slot maps and packed-row indices from lengths, in one launch.  Request b has ctx_lens[b] cached positions in the first ceil(ctx / 64) pages of
  * its row of page_table [B][max_pages].  new_lens[b] >= 0: it has that many more tokens in this step and takes the pages that they need from the top
@@ -123,14 +123,15 @@ size_t hbk_kv_q4_plane_bytes(int num_pages, int Hkv, int D); /* 0: refused sizes
 int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_t* slot_mapping, void* k_cache, void* v_cache, void* k_seen, int ldks,
                     void* v_seen, int ldvs, int T, int Hkv, int D, int page_size, int num_pages, void* stream);
 /* Attention over such planes: rows [cu_seqlens[b], cu_seqlens[b + 1]) of q are the last positions of the kv_lens[b]-long sequence b (at most max_q_len of them;
- * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own.  Any Hq / Hkv up to 4096, Hkv up to 65535, max_q_len * Hq up to 2^30.  window, softcap and sink as in
- * hbk_attn_prefill_paged_with.  A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold.  No kv_lens entry is above max_kv_len or
- * max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen.  Value scales may differ by
- * any factor; shares in which those of a group differ by more than 2^16 take up to fifty times as long.  Entries of q below 2^-27 of the largest of their head's row
- * lose bits, and with 256 columns key scales below 2^-25 of the largest of their position.  split_pages: pages that one block
- * reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq / Hkv is 256 or more, on nothing else); 0:
- * hbk_attn_paged_q4_split's.  Single tokens beside portions of 256 columns (rows * Hq / Hkv) are quicker in a call of their own.  workspace: as many floats as
- * hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL; on 16 bytes); launches that may run at the same time need one each. */
+ * cu_seqlens NULL: one row per sequence, row b), each sees the positions up to its own. Any Hq / Hkv up to 4096, Hkv up to 65535, max_q_len * Hq up to 2^30.
+ * window, softcap and sink as in hbk_attn_prefill_paged_with. A row that sees nothing (length 0) is 0; rows of no sequence keep what they hold. No kv_lens entry
+ * is above max_kv_len or max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen. Value scales
+ * may differ by any factor (shares in which those of a group differ by more than 2^16 take up to fifty times as long); a weight counts to 2^-10 of itself or
+ * 2^-23 of its row's largest. Entries of q below 2^-27 of the largest of their head's row lose bits, and with 256 columns key scales below 2^-25 of the largest
+ * of their position. split_pages: pages that one block reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq /
+ * Hkv is 256 or more, on nothing else); 0: hbk_attn_paged_q4_split's. Single tokens beside portions of 256 columns (rows * Hq / Hkv) are quicker in a call of
+ * their own. workspace: as many floats as hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL; on 16 bytes); launches that
+ * may run at the same time need one each. */
 int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
                       const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
                       int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream);
@@ -145,8 +146,8 @@ long long hbk_attn_paged_q4_wait_cycles(long long cycles);
 int hbk_attn_paged_q4_split(int B, int max_q_len, int max_kv_len, int Hq, int Hkv, int window, int sms);
 size_t hbk_attn_paged_q4_workspace_floats(int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D, int split_pages, int window);
 /* 4-bit weights: N rows of K / 32 GGUF Q4_0 blocks (18 bytes: fp16 d, then byte i with entries i and i + 16; device memory) laid out as the product reads them, in
- * hbk_gemm_q4_bytes(N, K) bytes (K a multiple of 32 up to 2^30 - 128, N up to 65535 * 64): tiles [ceil(N / 16)][ceil(K / 128)] of 16 rows of 64 bytes as K codes above with D = 128, then
- * [16 rows][4 groups] fp16 scales. */
+ * hbk_gemm_q4_bytes(N, K) bytes (K a multiple of 32 up to 2^30 - 128, N up to 65535 * 64): tiles [ceil(N / 16)][ceil(K / 128)] of 16 rows of 64 bytes as K
+ * codes above with D = 128, then [16 rows][4 groups] fp16 scales. */
 size_t hbk_gemm_q4_bytes(int N, int K); /* 0: refused sizes */
 int hbk_gemm_q4_pack(const void* blocks, void* packed, int N, int K, void* stream);
 /* out[M, N] = X[M, K] . W4[N, K]^T, M <= 256 (made for the rows of a decode step: beyond 32 rows hbk_gemm with bf16 weights is quicker); epi as in hbk_gemm: 0, 1, 3, 4
