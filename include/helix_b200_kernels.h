@@ -128,10 +128,10 @@ int hbk_kv_write_q4(const void* k, int ldk, const void* v, int ldv, const int32_
  * is above max_kv_len or max_pages * 64 (what lies past either is cut off the sequence), positions of a page number outside the pool are not seen. Value scales
  * may differ by any factor (shares in which those of a group differ by more than 2^16 take up to fifty times as long); a weight counts to 2^-10 of itself or
  * 2^-23 of its row's largest. Entries of q below 2^-27 of the largest of their head's row lose bits, and with 256 columns key scales below 2^-25 of the largest
- * of their position. split_pages: pages that one block reads of a sequence at most (a row's bits depend on its sequence, on it and on whether max_q_len * Hq /
- * Hkv is 256 or more, on nothing else); 0: hbk_attn_paged_q4_split's. Single tokens beside portions of 256 columns (rows * Hq / Hkv) are quicker in a call of
- * their own. workspace: as many floats as hbk_attn_paged_q4_workspace_floats says for the same arguments (0: none, it may be NULL; on 16 bytes); launches that
- * may run at the same time need one each. */
+ * of their position; keys from 2^105 on overflow, however small the queries. split_pages: pages that one block reads of a sequence at most (a row's bits depend
+ * on its sequence, on it and on whether max_q_len * Hq / Hkv is 256 or more, on nothing else); 0: hbk_attn_paged_q4_split's. Single tokens beside portions of
+ * 256 columns (rows * Hq / Hkv) are quicker in a call of their own. workspace: as many floats as hbk_attn_paged_q4_workspace_floats says for the same arguments
+ * (0: none, it may be NULL; on 16 bytes); launches that may run at the same time need one each. */
 int hbk_attn_paged_q4(const void* q, int ldq, const void* k_cache, const void* v_cache, const int32_t* page_table, int max_pages, const int32_t* kv_lens,
                       const int32_t* cu_seqlens, void* out, int ldo, float* workspace, int B, int T, int max_q_len, int max_kv_len, int Hq, int Hkv, int D,
                       int page_size, int split_pages, float scale, int num_pages, int window, float softcap, const void* sink, void* stream);
