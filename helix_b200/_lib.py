@@ -170,6 +170,13 @@ SIGNATURES = {
     "hbk_gemm_q4_bytes": (C.c_size_t, [I, I]),
     "hbk_gemm_q4_pack": (I, [P, P, I, I, P]),
     "hbk_gemm_q4": (I, [P, I, P, P, I, P, I, P, I, I, I, I, P]),
+    "hbk_rows_q8": (I, [P, I, I, P, I, P, P, I, I, I, P]),
+    "hbk_gemm_q8": (I, [P, I, P, P, I, P, P, I, P, I, P, I, I, I, I, P]),
+    "hbk_head_scores": (I, [P, I, P, P, I, P, P, P, P, P, I, I, I, C.c_float, C.c_float, P]),
+    "hbk_head_scores_workspace_floats": (C.c_size_t, [I, I]),
+    "hbk_q8_status": (I, []),
+    "hbk_q8_wait_cycles": (C.c_longlong, [C.c_longlong]),
+    "hbk_token_scores": (I, [P, I, I, P, I, I, I, P, P, P, P, P, P]),
 }
 
 _lib = None

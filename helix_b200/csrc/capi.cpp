@@ -429,4 +429,25 @@ int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, cons
                                                                with_r ? (const hb::bf16*)R : nullptr, ldr, with_bias ? (const hb::bf16*)bias : nullptr, M, N, K}));
 }
 
+int hbk_rows_q8(const void* x, int x_f32, int ldx, void* codes, int ldc, float* scales, void* seen, int lds, int T, int K, void* stream) {
+  return kret(hb::rows_q8((cudaStream_t)stream, hb::RowsQ8Args{x, x_f32 != 0, ldx, (int8_t*)codes, ldc, scales, (hb::bf16*)seen, lds, T, K}));
+}
+int hbk_gemm_q8(const void* X, int ldx, const float* x_scales, const void* W, int ldw, const float* w_scales, void* out, int ldo, const void* R, int ldr,
+                const void* bias, int M, int N, int K, int epi, void* stream) {
+  if (epi < hb::EPI_NONE || epi > hb::EPI_F32) return kret(cudaErrorInvalidValue);
+  return kret(hb::gemm_q8((cudaStream_t)stream, hb::GemmQ8Args{(const int8_t*)X, ldx, x_scales, (const int8_t*)W, ldw, w_scales, out, ldo, (const hb::bf16*)R, ldr,
+                                                               (const hb::bf16*)bias, M, N, K, (hb::Epi)epi}));
+}
+int hbk_head_scores(const void* X, int ldx, const float* x_scales, const void* W, int ldw, const float* w_scales, const int32_t* targets, float* lp,
+                    float* entropy, float* workspace, int T, int V, int H, float scale, float softcap, void* stream) {
+  return kret(hb::head_scores((cudaStream_t)stream, hb::HeadScoresArgs{X, ldx, x_scales, W, ldw, w_scales, targets, lp, entropy, workspace, T, V, H, scale, softcap}));
+}
+size_t hbk_head_scores_workspace_floats(int T, int V) { return hb::head_scores_workspace_floats(T, V); }
+int hbk_q8_status(void) { return kret(hb::q8_status()); }
+long long hbk_q8_wait_cycles(long long cycles) { return hb::q8_wait_cycles(cycles); }
+int hbk_token_scores(const void* logits, int f32, int ldl, const int32_t* targets, int T, int V, int n_top, float* lp, int32_t* rank, float* entropy,
+                     int32_t* top_ids, float* top_lp, void* stream) {
+  return kret(hb::token_scores((cudaStream_t)stream, hb::TokenScoresArgs{logits, f32 != 0, ldl, targets, T, V, n_top, lp, rank, entropy, top_ids, top_lp}));
+}
+
 }  // extern "C"

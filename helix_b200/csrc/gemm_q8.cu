@@ -1,0 +1,1054 @@
+// Products of rows of 8-bit codes, out[m, n] = (X W^T)[m, n] x_scales[m] w_scales[n] and its epilogues, and scores of given tokens straight from a head's product.
+//
+// The sums are whole numbers of 32 bits on the tensor cores (tcgen05 kind::i8): exact in any order, so parts of K add up to the same bits however they are cut.  Both operands
+// lie in rows along K and come as blocks of 128 bytes of 128 or 256 rows, TMA's 128-byte swizzle: 128 codes, or 64 entries of bf16 where the head's scores take those.
+//
+// tile_kernel: persistent, one block (or a pair of blocks, cta_group::2) per SM; warp 0 loads, warp 1 multiplies, eight warps take the sums from tensor memory, which holds two
+// tiles' so that one tile's epilogue lies behind the next one's products.
+//   Scores: thread = row, so that a row's running maximum m, S = sum e^(z - m) and U = sum (z - m) e^(z - m) need no other thread; a tile leaves three numbers per row and 128 (64)
+//   columns instead of its logits, and join_scores_kernel puts them together: lp = z_t - m - log S, entropy = log S - U / S.
+// split_kernel: few tiles.  The blocks of a cluster share K and add their whole numbers through distributed shared memory; a block's X has only as many rows as there are.
+//
+// Waits are bounded (q8_wait_cycles): one that runs out ends the kernel with NaN in place of what it was for, and q8_status says so.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "kernels.h"
+#include "launch.h"
+#include "ptx.cuh"
+#include "tma_host.h"
+
+namespace hb {
+namespace {
+
+constexpr int TM = 128;                    // rows of X of a block
+constexpr int KB = 128;                    // bytes of K of a block of operands: one span of the swizzle
+constexpr int kStaging = TM * 128;         // 128 rows of 128 bytes on their way out
+constexpr int EPI_SCORES = 100;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ unsigned wait_ran_out;  // set by a block that gave up a wait: q8_status
+
+// False where the barrier has not turned after so many cycles (below 0: it is not looked at).  Warps come here whole.
+__device__ __forceinline__ bool wait_turn(uint64_t* bar, uint32_t parity, long long cycles) {
+  bool ok = cycles >= 0 && mbar_try_wait(bar, parity);
+  if (!ok && cycles > 0) {
+    const long long t0 = clock64();
+    while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < cycles) {
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+// True for all of the barrier's threads if it is for each
+__device__ __forceinline__ bool all_of(uint32_t id, uint32_t nthreads, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.u32 p, %3, 0;\n"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n"
+      "selp.u32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"((uint32_t)mine)
+      : "memory");
+  return r != 0;
+}
+// bytes that count as arrived (for copies that were announced and never asked for)
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x Phi(x) with erfc by Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most)
+__device__ __forceinline__ float gelu_erf(float x) {
+  const float z = fabsf(x) * 0.70710678118654752f;
+  const float t = rcp_fast(fmaf(0.3275911f, z, 1.f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float h = 0.5f * p * t * exp2_fast(-z * z * kLog2e);
+  return x * (x > 0.f ? 1.f - h : h);
+}
+// tanh: 1 - 2 / (e^2|x| + 1), and where that cancels (|x| < 1/4) its series, whose next term is 2^-26 of it
+__device__ __forceinline__ float tanh_fast(float x) {
+  const float u = x * x;
+  float p = fmaf(u, 62.f / 2835.f, -17.f / 315.f);
+  p = fmaf(p, u, 2.f / 15.f);
+  p = fmaf(p, u, -1.f / 3.f);
+  p = fmaf(p * u, x, x);
+  const float y = copysignf(fmaf(-2.f, rcp_fast(exp2_fast(fabsf(x) * (2.f * kLog2e)) + 1.f), 1.f), x);
+  return u < 0.0625f ? p : y;
+}
+__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
+
+__host__ __device__ constexpr bool has_bias(int epi) { return epi == EPI_BIAS || epi == EPI_BIAS_GELU || epi == EPI_BIAS_RESID; }
+__host__ __device__ constexpr bool has_resid(int epi) { return epi == EPI_RESID || epi == EPI_BIAS_RESID; }
+
+struct TileArgs {
+  const float *xs, *ws;       // scales of rows and columns (NULL: bf16 operands)
+  const bf16* bias;
+  const bf16* r;
+  void* out;
+  int ldo, ldr;
+  int M, N;
+  int kbs;                    // blocks along K
+  int grp, group_n;           // order of tiles
+  int box_rows;               // rows of a block of X that are loaded
+  const int32_t* targets;     // scores
+  float *part, *at;           // [slot][3][M], [M]
+  float scale, cap, inv_cap;
+  long long wait_cycles;
+};
+
+// Sums of bf16 products lose their last bits each time that more are added to them on the tensor cores: after so many blocks (512 terms) they are taken out and added in fp32.
+// (H = 4096: scores off by 3e-6 of themselves in one piece, 4e-7 in eight.)  Whole numbers lose nothing.
+constexpr int kPiece = 8;
+
+template <bool I8>
+__device__ __forceinline__ int k_at(int kb) {  // a block's first entry
+  return kb * (I8 ? KB : KB / 2);
+}
+
+template <int BN, int CG, int EPI>
+struct Cfg {
+  static constexpr int EG = 2;  // groups of four warps behind the products
+  static constexpr int THREADS = 64 + EG * 128;
+  static constexpr int X_BYTES = TM * KB, W_BYTES = BN / CG * KB;
+  static constexpr int STAGE = X_BYTES + W_BYTES;
+  static constexpr int STAGING = EPI == EPI_SCORES ? 0 : EG * kStaging;
+  static constexpr int FIXED = STAGING + 1024 + 512;  // alignment, barriers
+  static constexpr int RAW = (227 * 1024 - FIXED) / STAGE;
+  static constexpr int STAGES = RAW > 10 ? 10 : RAW;
+  static constexpr int SMEM = STAGES * STAGE + FIXED;
+  static constexpr int COLS = 2 * BN;  // of tensor memory
+  static_assert(COLS == 128 || COLS == 256 || COLS == 512, "columns are allocated in powers of two");
+};
+
+__device__ __forceinline__ void tile_at(const TileArgs& a, int t, int num_m, int num_n, int& mi, int& ni) {
+  const int num_a = a.group_n ? num_n : num_m, num_b = a.group_n ? num_m : num_n;  // grouped and swept dimension
+  const int per = a.grp * num_b, g = t / per, r = t % per, first = g * a.grp, ga = min(a.grp, num_a - first);
+  const int x = first + r % ga, y = r / ga;
+  mi = a.group_n ? y : x;
+  ni = a.group_n ? x : y;
+}
+
+// 32 sums of a row to values: the whole numbers times both scales, or the fp32 sums themselves
+template <bool I8>
+__device__ __forceinline__ void values_of(const uint32_t (&v)[32], const TileArgs& a, float sx, int n0, float (&f)[32]) {
+  if constexpr (I8) {
+    if (n0 + 32 <= a.N) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(a.ws + n0) + j);
+        f[4 * j] = (float)(int)v[4 * j] * w.x * sx;
+        f[4 * j + 1] = (float)(int)v[4 * j + 1] * w.y * sx;
+        f[4 * j + 2] = (float)(int)v[4 * j + 2] * w.z * sx;
+        f[4 * j + 3] = (float)(int)v[4 * j + 3] * w.w * sx;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+  }
+}
+// 32 bf16 values of a row (of N) added
+__device__ __forceinline__ void add_32(const bf16* p, int left, float (&f)[32]) {
+  if (left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float b[8];
+      unpack_bf16x8(*(reinterpret_cast<const uint4*>(p) + j), b);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[8 * j + k] += b[k];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) f[j] += __bfloat162float(p[j]);
+  }
+}
+
+template <bool I8, int BN, int CG, int EPI>
+__global__ void __launch_bounds__(Cfg<BN, CG, EPI>::THREADS, 1)
+tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
+            const __grid_constant__ TileArgs a) {
+  using C = Cfg<BN, CG, EPI>;
+  constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG;
+  constexpr bool kScores = EPI == EPI_SCORES, kGlu = EPI == EPI_SWIGLU, kF32 = EPI == EPI_F32;
+  constexpr int OUT_BN = kGlu ? BN / 2 : BN, CHUNK = kF32 ? 32 : 64, NCHUNK = OUT_BN / CHUNK;
+  static_assert(!kGlu || BN == 256, "[128 gate|128 up]");
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
+  uint8_t* smem_x = smem;
+  uint8_t* smem_w = smem + STAGES * C::X_BYTES;
+  uint8_t* staging = smem + STAGES * C::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);  // [STAGES]
+  uint64_t* empty = full + STAGES;                                     // [STAGES]
+  uint64_t* sums_full = empty + STAGES;                                // [2]
+  uint64_t* sums_empty = sums_full + 2;                                // [2]
+  uint64_t* all_done = sums_empty + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(all_done + 1);
+  int* issued_ptr = reinterpret_cast<int*>(tmem_ptr + 1);
+  int* bad_ptr = issued_ptr + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_m = (a.M + TILE_M - 1) / TILE_M, num_n = (a.N + BN - 1) / BN, tiles = num_m * num_n;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_w);
+    if (!kScores) tma_prefetch_desc(&map_c);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], CG);  // (a pair's bytes all count on the first block's)
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sums_full[i], 1);
+      mbar_init(&sums_empty[i], 4 * EG * CG);
+    }
+    mbar_init(all_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      tmem_alloc_2sm(tmem_ptr, C::COLS);
+      tmem_relinquish_2sm();
+    } else {
+      tmem_alloc(tmem_ptr, C::COLS);
+      tmem_relinquish();
+    }
+    pdl_launch_dependents();  // (launch.h)
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  pdl_wait();
+
+  bool ok = true;
+  if (warp == 0) {
+    const bool elected = elect_one_sync();
+    int s = 0, issued = 0;
+    uint32_t phase = 0;
+    for (int t = worker; t < tiles && ok; t += workers) {
+      int mi, ni;
+      tile_at(a, t, num_m, num_n, mi, ni);
+      for (int kb = 0; kb < a.kbs; ++kb) {
+        if (!(ok = wait_turn(&empty[s], phase ^ 1, a.wait_cycles))) break;
+        if (elected) {
+          if constexpr (CG == 2) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::STAGE);
+            else mbar_arrive_cluster(&full[s], 0);
+            tma_load_2d_2sm(smem_x + s * C::X_BYTES, &map_x, &full[s], k_at<I8>(kb), mi * TILE_M + (int)rank * TM);
+            tma_load_2d_2sm(smem_w + s * C::W_BYTES, &map_w, &full[s], k_at<I8>(kb), ni * BN + (int)rank * (BN / 2));
+          } else {
+            mbar_arrive_expect_tx(&full[s], a.box_rows * KB + C::W_BYTES);
+            tma_load_2d(smem_x + s * C::X_BYTES, &map_x, &full[s], k_at<I8>(kb), mi * TILE_M);
+            tma_load_2d(smem_w + s * C::W_BYTES, &map_w, &full[s], k_at<I8>(kb), ni * BN);
+          }
+        }
+        ++issued;
+        if (++s == STAGES) { s = 0; phase ^= 1; }
+      }
+    }
+    if (lane == 0) *issued_ptr = issued;
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool elected = elect_one_sync();
+      constexpr uint32_t idesc = I8 ? umma_idesc_i8(TILE_M, BN) : umma_idesc_bf16(TILE_M, BN);
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      for (int t = worker; t < tiles && ok; t += workers) {
+        uint32_t d = 0;
+        for (int kb = 0; kb < a.kbs; ++kb) {
+          const bool first = I8 ? kb == 0 : kb % kPiece == 0;
+          if (first) {
+            if (!(ok = wait_turn(&sums_empty[it & 1], ((it >> 1) & 1) ^ 1, a.wait_cycles))) break;
+            tc_fence_after();
+            d = tmem + (it & 1) * BN;
+          }
+          if (!(ok = wait_turn(&full[s], phase, a.wait_cycles))) break;
+          tc_fence_after();
+          const uint32_t xa = smem_u32(smem_x + s * C::X_BYTES), wa = smem_u32(smem_w + s * C::W_BYTES);
+          if (elected) {
+#pragma unroll
+            for (int k = 0; k < KB; k += 32) {  // a product takes 32 bytes of K
+              const uint64_t dx = umma_desc_kmajor_sw128(xa + k), dw = umma_desc_kmajor_sw128(wa + k);
+              const uint32_t more = !first || k != 0;
+              if constexpr (I8 && CG == 2) umma_i8_ss_2sm(d, dx, dw, idesc, more);
+              else if constexpr (I8) umma_i8_ss(d, dx, dw, idesc, more);
+              else if constexpr (CG == 2) umma_f16_ss_2sm(d, dx, dw, idesc, more);
+              else umma_f16_ss(d, dx, dw, idesc, more);
+            }
+            if constexpr (CG == 2) umma_commit_2sm_mc(&empty[s], 0x3); else umma_commit(&empty[s]);
+          }
+          if (++s == STAGES) { s = 0; phase ^= 1; }
+          if (kb + 1 == a.kbs || (!I8 && kb % kPiece == kPiece - 1)) {
+            if (elected) {
+              if constexpr (CG == 2) umma_commit_2sm_mc(&sums_full[it & 1], 0x3); else umma_commit(&sums_full[it & 1]);
+            }
+            ++it;
+          }
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, row = q * 32 + lane;  // row of the block's 128, lane of tensor memory
+    const int grp = (warp - 2) >> 2;
+    const bool leader = ((threadIdx.x - 64) & 127) == 0;
+    uint8_t* const buf = staging + grp * kStaging;
+    uint8_t* const my_row = buf + row * 128;
+    float m = -INFINITY, S = 0.f, U = 0.f;  // scores
+    const bool carry = num_m == 1;          // a row's sums go on through the block's tiles
+    int it = 0;
+    for (int t = worker; t < tiles && ok; t += workers) {
+      int mi, ni;
+      tile_at(a, t, num_m, num_n, mi, ni);
+      const int m0 = mi * TILE_M + (int)rank * TM, row_g = m0 + row;
+      const bool live = row_g < a.M;
+      float sx = 1.f;
+      if constexpr (I8) sx = live ? __ldg(a.xs + row_g) : 0.f;
+      int target = -1;
+      if constexpr (kScores) {
+        sx *= a.scale;
+        if (live && a.targets) target = __ldg(a.targets + row_g);
+      }
+      uint32_t t_row = 0;
+      int as = 0;
+      auto sums_there = [&] {
+        as = it & 1;
+        ok = all_of(1 + grp, 128, wait_turn(&sums_full[as], (it >> 1) & 1, a.wait_cycles));
+        tc_fence_after();
+        t_row = tmem + as * BN + (static_cast<uint32_t>(q * 32) << 16);
+        ++it;
+        return ok;
+      };
+      auto release = [&] {  // this warp has read what it needs of the tile's sums
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) { if (CG == 2) mbar_arrive_cluster(&sums_empty[as], 0); else mbar_arrive(&sums_empty[as]); }
+      };
+      if constexpr (kScores) {
+        constexpr int MINE = BN / EG;  // a thread's columns of its row
+        float sums[I8 ? 1 : MINE];
+        if constexpr (!I8) {
+#pragma unroll
+          for (int j = 0; j < MINE; ++j) sums[j] = 0.f;
+          for (int k0 = 0; k0 < a.kbs; k0 += kPiece) {
+            if (!sums_there()) break;
+#pragma unroll
+            for (int c = 0; c < MINE; c += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(t_row + grp * MINE + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sums[c + j] += __uint_as_float(v[j]);
+            }
+            release();
+          }
+        } else {
+          sums_there();
+        }
+        if (!ok) break;
+        // 32 columns from n0 on
+        auto take = [&](float(&f)[32], int n0) {
+          if (n0 >= a.N) return;
+          if constexpr (!I8) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] *= sx;
+          }
+          if (a.cap > 0.f) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = a.cap * tanh_fast(f[j] * a.inv_cap);
+          }
+          if ((unsigned)(target - n0) < 32u) {
+            float z = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z = target - n0 == j ? f[j] : z;
+            a.at[row_g] = z;  // (one tile has the target; whether it is below N is asked where it is read)
+          }
+          if (n0 + 32 > a.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = n0 + j < a.N ? f[j] : -INFINITY;
+          }
+          float top = f[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top = fmaxf(top, f[j]);
+          if (top > m) {
+            if (m > -INFINITY) {
+              const float d = m - top, w = exp2_fast(d * kLog2e);
+              U = w > 0.f ? w * fmaf(d, S, U) : 0.f;
+              S *= w;
+            }
+            m = top;
+          }
+          const float base = m > -INFINITY ? m : 0.f;
+          const uint64_t off = f2_pack(-base, -base), log2e = f2_pack(kLog2e, kLog2e);
+          uint64_t s2 = f2_pack(0.f, 0.f), u2 = s2;  // two at a time
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            uint64_t d = f2_add(f2_pack(f[j], f[j + 1]), off);
+            float x0, x1;
+            f2_unpack(f2_mul(d, log2e), x0, x1);
+            const uint64_t w = f2_pack(exp2_fast(x0), exp2_fast(x1));
+            s2 = f2_add(s2, w);
+            if (n0 + 32 > a.N) {  // (0 times what is no infinity)
+              f2_unpack(d, x0, x1);
+              d = f2_pack(fmaxf(x0, -1e4f), fmaxf(x1, -1e4f));
+            }
+            u2 = f2_fma(w, d, u2);
+          }
+          float lo, hi;
+          f2_unpack(s2, lo, hi);
+          S += lo + hi;
+          f2_unpack(u2, lo, hi);
+          U += lo + hi;
+        };
+        const int n_first = ni * BN + grp * MINE;
+        if constexpr (I8) {
+#pragma unroll 1
+          for (int c = 0; c < MINE; c += 32) {
+            uint32_t v[32];
+            float f[32];
+            tmem_ld_32x32b_x32(t_row + grp * MINE + c, v);
+            tmem_ld_wait();
+            if (c + 32 == MINE) release();
+            values_of<I8>(v, a, sx, n_first + c, f);
+            take(f, n_first + c);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < MINE; c += 32) {
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = sums[c + j];
+            take(f, n_first + c);
+          }
+        }
+        if (!carry || t + workers >= tiles) {
+          if (live) {
+            float* p = a.part + (size_t)((carry ? worker : ni) * EG + grp) * 3 * a.M + row_g;
+            p[0] = m;
+            p[a.M] = S;
+            p[2 * (size_t)a.M] = U;
+          }
+          m = -INFINITY;
+          S = U = 0.f;
+        }
+      } else {
+        if (!sums_there()) break;
+        const int n_out0 = ni * OUT_BN, n_out = kGlu ? a.N / 2 : a.N;
+#pragma unroll 1
+        for (int c = grp; c < NCHUNK; c += EG) {
+          if (leader) tma_store_wait_read<0>();  // the group's store before has read `buf`
+          bar_sync(1 + grp, 128);
+          if constexpr (kF32) {
+            uint32_t v[32];
+            float f[32];
+            tmem_ld_32x32b_x32(t_row + c * 32, v);
+            tmem_ld_wait();
+            if (c + EG >= NCHUNK) release();
+            values_of<I8>(v, a, sx, n_out0 + c * 32, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(my_row + ((j ^ (row & 7)) << 4)) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int col = c * 64 + h * 32, n0 = n_out0 + col;
+              uint32_t v[32];
+              float f[32];
+              tmem_ld_32x32b_x32(t_row + col, v);
+              if constexpr (kGlu) {
+                uint32_t u[32];
+                float g[32];
+                tmem_ld_32x32b_x32(t_row + 128 + col, u);
+                tmem_ld_wait();
+                if (h == 1 && c + EG >= NCHUNK) release();
+                values_of<I8>(v, a, sx, ni * BN + col, g);
+                values_of<I8>(u, a, sx, ni * BN + 128 + col, f);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] *= silu(g[j]);
+              } else {
+                tmem_ld_wait();
+                if (h == 1 && c + EG >= NCHUNK) release();
+                values_of<I8>(v, a, sx, n0, f);
+              }
+              if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
+              if constexpr (EPI == EPI_BIAS_GELU) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
+              }
+              if constexpr (has_resid(EPI)) {
+                if (live) add_32(a.r + (size_t)row_g * a.ldr + n0, n_out - n0, f);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4 o;
+                o.x = pack_bf16x2(f[8 * j], f[8 * j + 1]);
+                o.y = pack_bf16x2(f[8 * j + 2], f[8 * j + 3]);
+                o.z = pack_bf16x2(f[8 * j + 4], f[8 * j + 5]);
+                o.w = pack_bf16x2(f[8 * j + 6], f[8 * j + 7]);
+                *reinterpret_cast<uint4*>(my_row + (((h * 4 + j) ^ (row & 7)) << 4)) = o;
+              }
+            }
+          }
+          const int n0 = n_out0 + c * CHUNK;
+          if (n0 + CHUNK > n_out && n_out % (kF32 ? 4 : 8) != 0) {  // (a copy ends on 16 bytes: it would write zeros behind the last column)
+            if (live) {
+              for (int j = 0; n0 + j < n_out; ++j) {
+                const int at = ((j / (kF32 ? 4 : 8)) ^ (row & 7)) << 4, in = j % (kF32 ? 4 : 8);
+                if constexpr (kF32) static_cast<float*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const float*>(my_row + at)[in];
+                else static_cast<bf16*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const bf16*>(my_row + at)[in];
+              }
+            }
+            continue;
+          }
+          fence_proxy_async_smem();
+          bar_sync(1 + grp, 128);
+          if (leader) {
+            tma_store_2d(&map_c, buf, n0, m0);
+            tma_store_commit();
+          }
+        }
+      }
+    }
+    if (!kScores && leader) tma_store_wait_all<0>();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  bool bad = __syncthreads_or(!ok);
+  if constexpr (CG == 2) {
+    if (threadIdx.x == 0) *bad_ptr = bad;
+    __syncthreads();
+    cluster_sync_all();
+    bad |= *cluster_ptr<2>(bad_ptr, rank ^ 1) != 0;
+  }
+  if (bad) {
+    // what is in flight ends before its room is given back
+    if (warp == 0) {
+      const int mine = *issued_ptr, other = CG == 2 ? *cluster_ptr<2>(issued_ptr, rank ^ 1) : mine;
+      if (rank == 0) {
+        if (lane == 0) {
+          if constexpr (CG == 2) {
+            for (int i = min(mine, other); i < max(mine, other); ++i) {  // blocks that one of the pair asked for and the other did not: the other's part is made up for
+              if (other > mine) {
+                mbar_arrive_expect_tx(&full[i % STAGES], C::STAGE);
+              } else {
+                mbar_complete_tx(&full[i % STAGES], C::STAGE);
+                mbar_arrive(&full[i % STAGES]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        for (int i = max(0, max(mine, other) - STAGES); i < max(mine, other); ++i) wait_turn(&full[i % STAGES], (i / STAGES) & 1, HB_WAIT_TIMEOUT_CYCLES);
+      }
+    }
+    if (warp == 1) {
+      if (rank == 0 && elect_one_sync()) {
+        if constexpr (CG == 2) umma_commit_2sm_mc(all_done, 0x3); else umma_commit(all_done);
+      }
+      __syncwarp();
+      wait_turn(all_done, 0, HB_WAIT_TIMEOUT_CYCLES);
+    }
+    const float nan = __uint_as_float(0x7fffffffu);
+    for (int t = worker; t < tiles; t += workers) {
+      int mi, ni;
+      tile_at(a, t, num_m, num_n, mi, ni);
+      const int m0 = mi * TILE_M + (int)rank * TM;
+      if constexpr (kScores) {
+        for (int i = threadIdx.x; i < TM * EG; i += C::THREADS) {
+          const int r = m0 + i % TM;
+          if (r < a.M) a.part[(size_t)((num_m == 1 ? worker : ni) * EG + i / TM) * 3 * a.M + (size_t)a.M + r] = nan;
+        }
+      } else {
+        const int n_out = kGlu ? a.N / 2 : a.N;
+        for (int i = threadIdx.x; i < TM * OUT_BN; i += C::THREADS) {
+          const int r = m0 + i / OUT_BN, n = ni * OUT_BN + i % OUT_BN;
+          if (r < a.M && n < n_out) {
+            if constexpr (kF32) static_cast<float*>(a.out)[(size_t)r * a.ldo + n] = nan;
+            else static_cast<bf16*>(a.out)[(size_t)r * a.ldo + n] = __float2bfloat16(nan);
+          }
+        }
+      }
+    }
+    if (threadIdx.x == 0) wait_ran_out = 1;
+    __syncthreads();
+  }
+  if constexpr (CG == 2) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CG == 2) tmem_dealloc_2sm(tmem, C::COLS); else tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// ------------------------------------------------------------------ a row's sums of all tiles
+constexpr int kJoinRows = 8, kJoinThreads = 512;
+
+__global__ void __launch_bounds__(kJoinThreads) join_scores_kernel(const float* __restrict__ part, const float* __restrict__ at, const int32_t* __restrict__ targets,
+                                                                  float* __restrict__ lp, float* __restrict__ entropy, int slots, int T, int V) {
+  __shared__ float sm[3][kJoinThreads];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;  // neighbouring threads read neighbouring rows
+  const int row = blockIdx.x * kJoinRows + r;
+  float m = -INFINITY, s = 0.f, u = 0.f;
+  auto add = [&](float m2, float s2, float u2) {
+    const float top = fmaxf(m, m2);
+    auto weight = [&](float x, float& d) {
+      d = x == top ? 0.f : fmaxf(x - top, -200.f);
+      return d > -200.f ? exp2_fast(d * kLog2e) : 0.f;
+    };
+    float d1, d2;
+    const float w1 = weight(m, d1), w2 = weight(m2, d2);
+    u = (w1 > 0.f ? w1 * fmaf(d1, s, u) : 0.f) + (w2 > 0.f ? w2 * fmaf(d2, s2, u2) : 0.f);
+    s = fmaf(w1, s, w2 * s2);  // (a NaN times 0 stays one)
+    m = top;
+  };
+  if (row < T) {
+    constexpr int kAhead = 4;
+    for (int i = g; i < slots; i += kAhead * (kJoinThreads / kJoinRows)) {
+      float v[kAhead][3];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int slot = i + k * (kJoinThreads / kJoinRows);
+#pragma unroll
+        for (int c = 0; c < 3; ++c) v[k][c] = slot < slots ? part[((size_t)slot * 3 + c) * T + row] : (c == 0 ? -INFINITY : 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) add(v[k][0], v[k][1], v[k][2]);
+    }
+  }
+  sm[0][threadIdx.x] = m;
+  sm[1][threadIdx.x] = s;
+  sm[2][threadIdx.x] = u;
+  for (int o = kJoinThreads / 2; o >= kJoinRows; o >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < o) {
+      add(sm[0][threadIdx.x + o], sm[1][threadIdx.x + o], sm[2][threadIdx.x + o]);
+      sm[0][threadIdx.x] = m;
+      sm[1][threadIdx.x] = s;
+      sm[2][threadIdx.x] = u;
+    }
+  }
+  if ((int)threadIdx.x < kJoinRows && row < T) {
+    const bool none = s == 0.f;  // nothing but -inf
+    const float log_s = logf(s);
+    const int t = targets ? targets[row] : -1;
+    if (lp) lp[row] = t >= 0 && t < V && !none ? at[row] - m - log_s : -INFINITY;
+    if (entropy) entropy[row] = none ? 0.f : log_s - u / s;
+  }
+}
+
+// ------------------------------------------------------------------ few tiles: K shared by a cluster
+constexpr int SN = 128;                  // rows of W of a tile (a gated unit's: 64 of the gate, 64 beside them)
+constexpr int kDump = SN + 4;            // whole numbers of a row on their way through shared memory
+constexpr int kSplitThreads = 192;
+
+struct SplitArgs {
+  const float *xs, *ws;
+  const bf16 *bias, *r;
+  void* out;
+  int ldo, ldr, M, N, kbs, epi;
+  int box_rows, stages;
+  long long wait_cycles;
+};
+
+__global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                              const __grid_constant__ SplitArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[12], empty[12], sums_full, all_done;
+  __shared__ uint32_t tmem_at;
+  __shared__ int bad_flag;
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
+  const int x_bytes = a.box_rows * KB, stages = a.stages;
+  uint8_t* smem_w = smem + stages * x_bytes;  // (products read 128 rows of X whatever was loaded: what lies behind goes into rows that nobody reads)
+  int* dump = reinterpret_cast<int*>(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int parts = gridDim.x, part = blockIdx.x;
+  const int kb0 = (int)((long long)a.kbs * part / parts), kb1 = (int)((long long)a.kbs * (part + 1) / parts);
+  const bool glu = a.epi == EPI_SWIGLU;
+  const int m0 = blockIdx.z * TM;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_w);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&sums_full, 1);
+    mbar_init(&all_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_at, SN);
+    tmem_relinquish();
+    pdl_launch_dependents();  // (launch.h)
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0);
+  pdl_wait();
+
+  bool ok = true;
+  int issued = 0;
+  if (warp == 0) {
+    const bool elected = elect_one_sync();
+    const int w0 = glu ? blockIdx.y / 2 * 256 + blockIdx.y % 2 * 64 : blockIdx.y * SN, w1 = w0 + (glu ? 128 : 64);
+    int s = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!(ok = wait_turn(&empty[s], phase ^ 1, a.wait_cycles))) break;
+      if (elected) {
+        mbar_arrive_expect_tx(&full[s], x_bytes + SN * KB);
+        tma_load_2d(smem_w + s * SN * KB, &map_w, &full[s], kb * KB, w0, kEvictFirst);
+        tma_load_2d(smem_w + s * SN * KB + 64 * KB, &map_w, &full[s], kb * KB, w1, kEvictFirst);
+        tma_load_2d(smem + s * x_bytes, &map_x, &full[s], kb * KB, m0, kEvictLast);
+      }
+      ++issued;
+      if (++s == stages) { s = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    const bool elected = elect_one_sync();
+    constexpr uint32_t idesc = umma_idesc_i8(TM, SN);
+    int s = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!(ok = wait_turn(&full[s], phase, a.wait_cycles))) break;
+      tc_fence_after();
+      const uint32_t xa = smem_u32(smem + s * x_bytes), wa = smem_u32(smem_w + s * SN * KB);
+      if (elected) {
+#pragma unroll
+        for (int k = 0; k < KB; k += 32) umma_i8_ss(tmem, umma_desc_kmajor_sw128(xa + k), umma_desc_kmajor_sw128(wa + k), idesc, kb > kb0 || k != 0);
+        umma_commit(&empty[s]);
+      }
+      if (++s == stages) { s = 0; phase ^= 1; }
+    }
+    if (ok && elected) umma_commit(&sums_full);
+    __syncwarp();
+  } else {
+    ok = wait_turn(&sums_full, 0, a.wait_cycles);
+    const int q = warp & 3, row = q * 32 + lane;
+    if (ok && q * 32 < a.box_rows) {  // (all operands have been read: their room takes the sums)
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < SN; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
+        tmem_ld_wait();
+        if (row < a.box_rows) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(dump + row * kDump + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  bool bad = __syncthreads_or(!ok);
+  if (bad) {
+    if (warp == 0)
+      for (int i = max(0, issued - stages); i < issued; ++i) wait_turn(&full[i % stages], (i / stages) & 1, HB_WAIT_TIMEOUT_CYCLES);
+    if (warp == 1) {
+      if (elect_one_sync()) umma_commit(&all_done);
+      __syncwarp();
+      wait_turn(&all_done, 0, HB_WAIT_TIMEOUT_CYCLES);
+    }
+    if (threadIdx.x == 0) wait_ran_out = 1;
+  }
+  if (parts > 1) {
+    if (threadIdx.x == 0) bad_flag = bad;
+    __syncthreads();
+    cluster_sync_all();
+    bad = __syncthreads_or((int)threadIdx.x < parts && *cluster_ptr<2>(&bad_flag, threadIdx.x) != 0);
+  }
+  const int rows = min(a.M - m0, TM), quads = glu ? SN / 8 : SN / 4, n_out = glu ? a.N / 2 : a.N;
+  for (int i = part * kSplitThreads + threadIdx.x; i < rows * quads; i += parts * kSplitThreads) {
+    const int r = i / quads, c = i % quads * 4, m = m0 + r, n = blockIdx.y * (quads * 4) + c;
+    if (n >= n_out) continue;
+    int4 x = make_int4(0, 0, 0, 0), y = x;
+    for (int p = 0; p < parts; ++p) {
+      const int* at = parts == 1 ? dump : cluster_ptr<2>(dump, p);
+      const int4 v = *reinterpret_cast<const int4*>(at + r * kDump + c);
+      x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+      if (glu) {
+        const int4 w = *reinterpret_cast<const int4*>(at + r * kDump + 64 + c);
+        y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
+      }
+    }
+    const float sx = __ldg(a.xs + m);
+    const int acc[4] = {x.x, x.y, x.z, x.w}, up[4] = {y.x, y.y, y.z, y.w};
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = 0.f;
+      if (n + e >= n_out) continue;
+      if (glu) {
+        const int wn = blockIdx.y / 2 * 256 + blockIdx.y % 2 * 64 + c + e;
+        f[e] = (float)up[e] * __ldg(a.ws + wn + 128) * sx * silu((float)acc[e] * __ldg(a.ws + wn) * sx);
+      } else {
+        f[e] = (float)acc[e] * __ldg(a.ws + n + e) * sx;
+        if (a.bias) f[e] += __bfloat162float(a.bias[n + e]);
+        if (a.epi == EPI_BIAS_GELU) f[e] = gelu_erf(f[e]);
+        if (a.r) f[e] += __bfloat162float(a.r[(size_t)m * a.ldr + n + e]);
+      }
+      if (bad) f[e] = __uint_as_float(0x7fffffffu);
+    }
+    if (a.epi == EPI_F32) {
+      float* o = static_cast<float*>(a.out) + (size_t)m * a.ldo + n;
+      if (n + 4 <= n_out) *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
+      else
+        for (int e = 0; n + e < n_out; ++e) o[e] = f[e];
+    } else {
+      bf16* o = static_cast<bf16*>(a.out) + (size_t)m * a.ldo + n;
+      if (n + 4 <= n_out) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+      else
+        for (int e = 0; n + e < n_out; ++e) o[e] = __float2bfloat16(f[e]);
+    }
+  }
+  if (parts > 1) {
+    __syncwarp();
+    cluster_sync_all();  // others may still read this block's sums
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, SN);
+  }
+}
+
+// ------------------------------------------------------------------ host
+std::atomic<long long> wait_limit{HB_WAIT_TIMEOUT_CYCLES};
+
+int device_sms() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return effective_sms(sms);
+}
+// More than 48 KB of shared memory wants to be asked for once per device
+template <typename F>
+cudaError_t ask_smem(F kernel, int bytes, std::atomic<uint64_t>& asked) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && !(asked.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return e;
+}
+struct Launch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  Launch(dim3 grid, int threads, int smem, cudaStream_t stream, int cluster) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    int n = 0;
+    if (pdl_enabled()) {
+      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+      attr[n].id = cudaLaunchAttributeClusterDimension;
+      attr[n].val.clusterDim.x = cluster;
+      attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+  }
+};
+
+struct Operand {
+  const void* p;
+  int ld, rows;
+};
+template <bool I8>
+bool operand_map(CUtensorMap* map, const Operand& o, int K, int box_rows) {
+  return make_tmap_2d(map, o.p, I8 ? TM_U8 : TM_BF16, (uint64_t)K, (uint64_t)o.rows, (uint64_t)o.ld * (I8 ? 1 : 2), I8 ? KB : KB / 2, box_rows);
+}
+
+template <bool I8, int BN, int CG, int EPI>
+cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, const Operand& w, int K, int sms) {
+  using C = Cfg<BN, CG, EPI>;
+  static std::atomic<uint64_t> asked{0};
+  cudaError_t e = ask_smem(tile_kernel<I8, BN, CG, EPI>, C::SMEM, asked);
+  if (e != cudaSuccess) return e;
+  constexpr int TILE_M = TM * CG;
+  const int n_out = EPI == EPI_SWIGLU ? a.N / 2 : a.N;
+  a.box_rows = CG == 2 ? TM : std::min(TM, (a.M + 7) / 8 * 8);
+  CUtensorMap mx, mw, mc;
+  if (!operand_map<I8>(&mx, x, K, a.box_rows) || !operand_map<I8>(&mw, w, K, BN / CG)) return cudaErrorInvalidValue;
+  mc = mx;
+  if (EPI != EPI_SCORES &&
+      !make_tmap_2d(&mc, a.out, EPI == EPI_F32 ? TM_F32 : TM_BF16, (uint64_t)n_out, (uint64_t)a.M, (uint64_t)a.ldo * (EPI == EPI_F32 ? 4 : 2), EPI == EPI_F32 ? 32 : 64, TM))
+    return cudaErrorInvalidValue;
+  const int bytes_k = I8 ? K : 2 * K;
+  a.kbs = (bytes_k + KB - 1) / KB;
+  const int num_m = (a.M + TILE_M - 1) / TILE_M, num_n = (a.N + BN - 1) / BN;
+  if ((long long)num_m * num_n > INT32_MAX / 2) return cudaErrorInvalidValue;
+  // Order of tiles: some 32 MB of one operand stay in L2 while the other passes by
+  const double x_tile = (double)TILE_M * bytes_k, w_tile = (double)BN * bytes_k, X = x_tile * num_m, W = w_tile * num_n;
+  const int gm = (int)std::max(1.0, std::min((double)num_m, floor(32e6 / x_tile))), gn = (int)std::max(1.0, std::min((double)num_n, floor(32e6 / w_tile)));
+  a.group_n = W + X * ceil((double)num_n / gn) < X + W * ceil((double)num_m / gm);
+  a.grp = a.group_n ? gn : gm;
+  a.wait_cycles = wait_limit.load(std::memory_order_relaxed);
+  const int workers = std::max(1, std::min(num_m * num_n, sms / CG));
+  Launch l(dim3(workers * CG), C::THREADS, C::SMEM, stream, CG);
+  return cudaLaunchKernelEx(&l.cfg, tile_kernel<I8, BN, CG, EPI>, mx, mw, mc, a);
+}
+
+// K in parts: the blocks of a cluster
+struct SplitPlan {
+  int parts, stages, smem;
+};
+SplitPlan split_plan(int M, int N, int kbs, int sms) {
+  const int box = std::min(TM, (M + 7) / 8 * 8);
+  const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN);
+  int parts = 1;
+  while (parts < 8 && tiles * (parts + 1) <= 2LL * sms && kbs >= 4 * (parts + 1)) ++parts;
+  const int stage = box * KB + SN * KB, most = (kbs + parts - 1) / parts;
+  const int stages = std::min(std::min(most, 12), (box <= 64 ? 108 : 216) * 1024 / stage);
+  return {parts, stages, std::max(stages * stage, box * kDump * 4) + 1024};
+}
+
+cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
+  static std::atomic<uint64_t> asked{0};
+  cudaError_t e = ask_smem(split_kernel, 220 * 1024, asked);
+  if (e != cudaSuccess) return e;
+  const int kbs = (g.K + KB - 1) / KB, box = std::min(TM, (g.M + 7) / 8 * 8);
+  const SplitPlan p = split_plan(g.M, g.N, kbs, sms);
+  CUtensorMap mx, mw;
+  if (!operand_map<true>(&mx, {g.x, g.ldx, g.M}, g.K, box) || !operand_map<true>(&mw, {g.w, g.ldw, g.N}, g.K, 64)) return cudaErrorInvalidValue;
+  const SplitArgs a{g.x_scales, g.w_scales, has_bias(g.epi) ? g.bias : nullptr, has_resid(g.epi) ? g.r : nullptr, g.out, g.ldo, g.ldr, g.M, g.N, kbs, (int)g.epi, box, p.stages,
+                    wait_limit.load(std::memory_order_relaxed)};
+  Launch l(dim3(p.parts, (g.N + SN - 1) / SN, (g.M + TM - 1) / TM), kSplitThreads, p.smem, stream, p.parts);
+  return cudaLaunchKernelEx(&l.cfg, split_kernel, mx, mw, a);
+}
+
+template <int EPI>
+cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
+  const long long few = (long long)((g.M + TM - 1) / TM) * ((g.N + SN - 1) / SN);
+  if (g.M <= TM ? g.N <= 65535 * SN : few <= sms) return launch_split(stream, g, sms);
+  TileArgs a{};
+  a.xs = g.x_scales;
+  a.ws = g.w_scales;
+  a.bias = g.bias;
+  a.r = g.r;
+  a.out = g.out;
+  a.ldo = g.ldo;
+  a.ldr = g.ldr;
+  a.M = g.M;
+  a.N = g.N;
+  const Operand x{g.x, g.ldx, g.M}, w{g.w, g.ldw, g.N};
+  if constexpr (EPI != EPI_SWIGLU) {
+    const long long pairs = (long long)((g.M + 255) / 256) * ((g.N + 255) / 256);
+    if (pairs < sms / 2 || sms < 2) return launch_tiles<true, 128, 1, EPI>(stream, a, x, w, g.K, sms);
+  }
+  return sms < 2 ? launch_tiles<true, 256, 1, EPI>(stream, a, x, w, g.K, sms) : launch_tiles<true, 256, 2, EPI>(stream, a, x, w, g.K, sms);
+}
+
+constexpr int kMostK = 131056;  // 127^2 K stays below 2^31 (codes of -128 that a caller may have: 128^2 K too)
+
+}  // namespace
+
+long long q8_wait_cycles(long long cycles) { return wait_limit.exchange(cycles); }
+cudaError_t q8_status() {
+  unsigned ran_out = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&ran_out, wait_ran_out, sizeof ran_out);
+  if (e != cudaSuccess || !ran_out) return e;
+  const unsigned none = 0;
+  e = cudaMemcpyToSymbol(wait_ran_out, &none, sizeof none);
+  return e == cudaSuccess ? cudaErrorLaunchTimeout : e;
+}
+
+cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& g) {
+  const bool f32 = g.epi == EPI_F32, glu = g.epi == EPI_SWIGLU;
+  if (g.epi < EPI_NONE || g.epi > EPI_F32 || g.M < 0 || g.N < 1 || g.K < 1 || g.K > kMostK || (glu && g.N % 256)) return cudaErrorInvalidValue;
+  if (g.M == 0) return cudaSuccess;
+  if (!g.x || ((uintptr_t)g.x & 15) || g.ldx < g.K || g.ldx % 16 || !g.w || ((uintptr_t)g.w & 15) || g.ldw < g.K || g.ldw % 16) return cudaErrorInvalidValue;
+  if (!g.x_scales || ((uintptr_t)g.x_scales & 3) || !g.w_scales || ((uintptr_t)g.w_scales & 15)) return cudaErrorInvalidValue;
+  const int n_out = glu ? g.N / 2 : g.N;
+  if (!g.out || ((uintptr_t)g.out & 15) || g.ldo < n_out || g.ldo % (f32 ? 4 : 8)) return cudaErrorInvalidValue;
+  if ((has_bias(g.epi) && (!g.bias || ((uintptr_t)g.bias & 15))) || (has_resid(g.epi) && (!g.r || ((uintptr_t)g.r & 15) || g.ldr < n_out || g.ldr % 8))) return cudaErrorInvalidValue;
+  const int sms = device_sms();
+  if (sms <= 0) return cudaErrorNoDevice;
+  switch (g.epi) {
+    case EPI_NONE: return launch_product<EPI_NONE>(stream, g, sms);
+    case EPI_BIAS: return launch_product<EPI_BIAS>(stream, g, sms);
+    case EPI_BIAS_GELU: return launch_product<EPI_BIAS_GELU>(stream, g, sms);
+    case EPI_RESID: return launch_product<EPI_RESID>(stream, g, sms);
+    case EPI_BIAS_RESID: return launch_product<EPI_BIAS_RESID>(stream, g, sms);
+    case EPI_SWIGLU: return launch_product<EPI_SWIGLU>(stream, g, sms);
+    default: return launch_product<EPI_F32>(stream, g, sms);
+  }
+}
+
+namespace {
+bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
+int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 2 : (V + 255) / 256 * 2; }  // (of a launch with one tile of rows: its blocks', which are fewer)
+}  // namespace
+
+size_t head_scores_workspace_floats(int T, int V) { return score_sizes_ok(T, V) ? (size_t)T * (3 * (size_t)score_slots(T, V) + 1) : 0; }
+
+cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
+  const bool i8 = g.x_scales != nullptr;
+  if (!score_sizes_ok(g.T, g.V) || g.H < 1 || g.H > (i8 ? kMostK : 1 << 29) || i8 != (g.w_scales != nullptr) || !(fabsf(g.scale) < INFINITY) || !(g.softcap >= 0.f) ||
+      !(g.softcap < INFINITY))
+    return cudaErrorInvalidValue;
+  if (g.T == 0) return cudaSuccess;
+  const int step = i8 ? 16 : 8;
+  if (!g.x || ((uintptr_t)g.x & 15) || g.ldx < g.H || g.ldx % step || !g.w || ((uintptr_t)g.w & 15) || g.ldw < g.H || g.ldw % step) return cudaErrorInvalidValue;
+  if (((uintptr_t)g.x_scales & 3) || ((uintptr_t)g.w_scales & 15) || ((uintptr_t)g.targets & 3) || ((uintptr_t)g.lp & 3) || ((uintptr_t)g.entropy & 3)) return cudaErrorInvalidValue;
+  if (!g.workspace || ((uintptr_t)g.workspace & 3) || (g.lp && !g.targets) || (!g.lp && !g.entropy)) return cudaErrorInvalidValue;
+  const int sms = device_sms();
+  if (sms <= 0) return cudaErrorNoDevice;
+  TileArgs a{};
+  a.xs = g.x_scales;
+  a.ws = g.w_scales;
+  a.M = g.T;
+  a.N = g.V;
+  a.targets = g.lp ? g.targets : nullptr;
+  a.part = g.workspace;
+  a.at = g.workspace + 3 * (size_t)score_slots(g.T, g.V) * g.T;
+  a.scale = g.scale;
+  a.cap = g.softcap;
+  a.inv_cap = 1.f / g.softcap;
+  const Operand x{g.x, g.ldx, g.T}, w{g.w, g.ldw, g.V};
+  cudaError_t e;
+  int slots;
+  if (g.T <= TM) {
+    e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms);
+    slots = std::min((g.V + 127) / 128, sms) * 2;
+  } else if (sms < 2) {
+    return cudaErrorInvalidConfiguration;
+  } else {
+    e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms);
+    slots = g.T <= 2 * TM ? std::min((g.V + 255) / 256, sms / 2) * 2 : (g.V + 255) / 256 * 2;
+  }
+  if (e != cudaSuccess) return e;
+  return launch_k(join_scores_kernel, dim3((g.T + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp,
+                  g.entropy, slots, g.T, g.V);
+}
+
+}  // namespace hb

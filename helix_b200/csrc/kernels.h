@@ -306,6 +306,50 @@ cudaError_t gemm_q4(cudaStream_t stream, const GemmQ4Args& a);
 cudaError_t gemm_q4_pack(cudaStream_t stream, const void* blocks, void* out, int N, int K);
 size_t gemm_q4_bytes(int N, int K);
 
+// ---- products in 8-bit whole numbers, and scores of given tokens ----
+struct RowsQ8Args {
+  const void* x; bool x_f32; int ldx;  // [T, K]
+  int8_t* codes; int ldc;              // [T, K]
+  float* scales;                       // [T]
+  bf16* seen; int lds;                 // optional: the rows as their codes stand for them
+  int T, K;
+};
+cudaError_t rows_q8(cudaStream_t stream, const RowsQ8Args& a);
+
+struct GemmQ8Args {
+  const int8_t* x; int ldx; const float* x_scales;  // [M, K], [M]
+  const int8_t* w; int ldw; const float* w_scales;  // [N, K], [N]
+  void* out; int ldo;                  // [M, N] (EPI_SWIGLU: N / 2 columns), fp32 for EPI_F32, else bf16
+  const bf16* r; int ldr;
+  const bf16* bias;
+  int M, N, K;
+  Epi epi;                             // EPI_NONE .. EPI_F32
+};
+cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& a);
+
+struct HeadScoresArgs {
+  const void* x; int ldx; const float* x_scales;    // [T, H]: 8-bit codes with scales, or bf16 (both scales NULL)
+  const void* w; int ldw; const float* w_scales;    // [V, H]
+  const int32_t* targets;              // [T] or NULL
+  float *lp, *entropy;                 // [T], either may be NULL
+  float* workspace;                    // head_scores_workspace_floats
+  int T, V, H;
+  float scale, softcap;
+};
+cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& a);
+size_t head_scores_workspace_floats(int T, int V);
+cudaError_t q8_status();
+long long q8_wait_cycles(long long cycles);
+
+struct TokenScoresArgs {
+  const void* logits; bool f32; int ldl;  // [T, V]
+  const int32_t* targets;              // [T] or NULL
+  int T, V, n_top;
+  float* lp; int32_t* rank; float* entropy;  // [T], any may be NULL
+  int32_t* top_ids; float* top_lp;     // [T, max(n_top, 1)]
+};
+cudaError_t token_scores(cudaStream_t stream, const TokenScoresArgs& a);
+
 // ---- decode-step GEMM (M <= 256): swap-AB + deterministic stream-K, fp32 partial slabs ----
 struct SkinnyPlan {
   int grid;                  // CTAs (== SMs unless the problem is tiny)

@@ -7,7 +7,7 @@
 
 namespace hb {
 
-enum TmDtype { TM_BF16 = 0, TM_F32 = 1 };
+enum TmDtype { TM_BF16 = 0, TM_F32 = 1, TM_U8 = 2 };
 
 // 2-D row-major tensor [outer][inner]; box = [box_outer][box_inner]; 128B swizzle when the box row is
 // exactly 128 bytes, no swizzle otherwise. Out-of-bounds elements read as zero / are not written.
