@@ -2,10 +2,11 @@
 //
 // One pass over a row, read once: every thread keeps the running maximum m of its entries, S = sum e^(x - m) and U = sum (x - m) e^(x - m), so that at the end
 //   log softmax(x_t) = x_t - m - log S,   entropy = log S - U / S.
-// The first tokens pass through a list in shared memory: an entry goes there only if it is not behind a bound, the n-th best of what was seen up to some step before.  The bound
-// is drawn anew after 1, 2, 4, 8.. steps, so that some n entries are listed between two of these whatever the row's length, and the threads run freely in between.  Rows in which
-// more are listed than there is room for (rising ones, say) have those steps looked through again step by step.  Places in the order are compared as one whole number of 64
-// bits (value bits made ordered, then the id complemented): no two are alike, ties go to the lower id, and the result does not depend on who came first.
+// A thread also remembers the step in which it met its maximum, and the largest of its other steps' maxima.  The n-th best of the threads' maxima bounds what may be among
+// the row's first n: n threads have such entries, and list those of that step; the few whose other steps reach the bound too are looked through once more (from L2).  Places in the
+// order are compared as one whole number of 64 bits (value bits made ordered, then the id complemented): no two are alike, ties go to the lower id, and the result does not
+// depend on who came first.  Rows in which more entries are listed than there is room for (rising ones, say) are looked through step by step, the list thinned out to the first n
+// between two steps.
 //
 // Bytes bound it: 4 or 2 per logit.  A row belongs to a cluster of 1 to 8 blocks, so that few rows still keep all SMs reading.
 #include <algorithm>
@@ -18,11 +19,9 @@ namespace hb {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int E = 8;                    // neighbouring entries of a thread
-constexpr int kStep = kThreads * E;     // entries that a block takes at a time
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMost = 64;               // n_top at most
-constexpr int kList = 1024;             // places of the list: what is kept (kMost) and what one step may add (kMost * E) fit
+constexpr int kList = 1280;             // places of the list: what is kept (kMost) and what one step may add (kMost threads' entries) fit
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ uint32_t ordered(float x) {  // 0 for a NaN, which comes last; zeros tie
@@ -39,6 +38,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float at_least(float a, float b) {  // 1 or 0
+  float r;
+  asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 struct Sums {
@@ -62,9 +73,22 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   return r;
 }
 
+__device__ __forceinline__ Sums join_lanes(Sums my, int lanes) {  // of the first `lanes` lanes (a power of two), known to all of these afterwards
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) {
+      const Sums other{__shfl_xor_sync(0xffffffffu, my.m, o), __shfl_xor_sync(0xffffffffu, my.s, o), __shfl_xor_sync(0xffffffffu, my.u, o)};
+      my = threadIdx.x & o ? join(other, my) : join(my, other);
+    }
+  return my;
+}
+
 struct Shared {
   u64 list[kList];
-  u64 best[kMost];   // a block's first tokens
+  u64 best[kThreads];  // the threads' earliest places; a block's first tokens
+  u64 bound;
+  int step[kThreads];  // with a thread's maximum
+  int candidate[kMost], candidates;
   Sums warp_sums[kWarps];
   int warp_before[kWarps];
   Sums sums;
@@ -98,12 +122,14 @@ template <bool F32>
 __device__ __forceinline__ float logit_at(const void* row, int i) {
   return F32 ? __ldg(static_cast<const float*>(row) + i) : __bfloat162float(static_cast<const bf16*>(row)[i]);
 }
-// A thread's entries travel to its own places in shared memory some steps ahead of it: nobody else reads them, so there is nothing to wait for but its own copies
+// A thread takes two pieces of 16 bytes of each step, a warp's pieces side by side.  They travel to its own places in shared memory some steps ahead of it: nobody else reads
+// them, so there is nothing to wait for but its own copies.
+constexpr int kWide = 2;                // pieces of a thread's entries
+constexpr int kAhead = 3;               // steps
 template <bool F32>
+constexpr int kEntries = F32 ? 8 : 16;
 struct Ring {
-  static constexpr int WIDE = F32 ? 2 : 1;   // 16 bytes of a thread's entries
-  static constexpr int AHEAD = F32 ? 2 : 4;  // steps
-  uint4 v[AHEAD][WIDE][kThreads];
+  uint4 v[kAhead][kWide][kThreads];
 };
 __device__ __forceinline__ void copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -113,126 +139,91 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 template <bool F32, int NC, bool TOP>
-__global__ void __launch_bounds__(kThreads, 3) token_scores_kernel(const TokenScoresArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenScoresArgs a) {
+  constexpr int E = kEntries<F32>, P = E / kWide, kStep = kThreads * E;  // entries of a thread, of a piece, of a step
   __shared__ Shared sh;
-  __shared__ Ring<F32> ring;
-  constexpr int AHEAD = Ring<F32>::AHEAD, WIDE = Ring<F32>::WIDE;
+  __shared__ Ring ring;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = NC == 1 ? 0 : (int)(blockIdx.x % NC), t = blockIdx.x / NC;
   const void* row = static_cast<const uint8_t*>(a.logits) + (size_t)t * a.ldl * (F32 ? 4 : 2);
-  // this block's entries: a share of whole eights
-  const int eights = (a.V + E - 1) / E;
-  const int begin = (int)((long long)eights * part / NC) * E, end = min(a.V, (int)((long long)eights * (part + 1) / NC) * E);
+  // this block's entries: a share of whole groups of E
+  const int groups = (a.V + E - 1) / E;
+  const int begin = (int)((long long)groups * part / NC) * E, end = min(a.V, (int)((long long)groups * (part + 1) / NC) * E);
+  auto first_of = [&](int thread) { return begin + thread / 32 * (32 * E) + thread % 32 * P; };  // its first entry of the first step
+  auto id_of = [](int i, int e) { return i + e / P * (32 * P) + e % P; };                         // of entry e of a thread whose first of the step is i
+  auto whole = [&](int i) { return i + 32 * P + P <= end; };
+  auto piece_at = [&](int i, int k) { return static_cast<const uint8_t*>(row) + (size_t)(i + k * (32 * P)) * (F32 ? 4 : 2); };
+  auto fetch = [&](int i, int place) {
+    if (whole(i)) {
+#pragma unroll
+      for (int k = 0; k < kWide; ++k) copy16(&ring.v[place][k][tid], piece_at(i, k));
+    }
+    copy_commit();
+  };
+  const int mine = first_of(tid);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) fetch(mine + k * kStep, k);
   const int target = a.targets ? a.targets[t] : -1;
   const bool has = target >= 0 && target < a.V;
-  const float xt = has ? logit_at<F32>(row, target) : 0.f;
+  const float xt = has ? logit_at<F32>(row, target) : __uint_as_float(0x7fffffffu);
+  // the next value above the target's: what is no less comes before it wherever it stands (none does where that is a NaN)
+  const uint32_t bits = __float_as_uint(xt + 0.f);
+  const float above = xt == 0.f ? __uint_as_float(1u) : __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
   if (tid == 0) sh.count = 0;
   __syncthreads();
 
   Sums my{-INFINITY, 0.f, 0.f};
-  int before = 0;
-  u64 bound = 0;  // an entry that is listed is not behind it
-  auto entries_at = [&](int i, float (&f)[E]) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = i + e < end ? logit_at<F32>(row, i + e) : -INFINITY;
-  };
-  auto list = [&](const float(&f)[E], int i) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const u64 place = i + e < end ? place_of(f[e], i + e) : 0ull;
-      if (place > bound) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kList) sh.list[at] = place;
-      }
-    }
-  };
-  // One step, its entries seen as they are: the n-th best of the threads' first places bounds what may be among the row's first n, so that no more than n threads list theirs
-  auto careful = [&](int i0) {
-    const int i = i0 + tid * E;
-    float f[E];
-    entries_at(i, f);
-    u64 first = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const u64 place = i + e < end ? place_of(f[e], i + e) : 0ull;
-      first = place > first ? place : first;
-    }
-    if (first <= bound) first = 0;
-    const int hits = __syncthreads_count(first != 0);
-    if (hits == 0) return;
-    if (hits > a.n_top) {
-      u64 at = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const u64 trial = at | 1ull << bit;
-        const int c = __syncthreads_count(first >= trial);
-        if (c >= a.n_top) {
-          at = trial;
-          if (c == a.n_top) break;
-        }
-      }
-      bound = at - 1 > bound ? at - 1 : bound;
-    }
-    if (first > bound) list(f, i);
-    const u64 nth = thin_out(sh, a.n_top);
-    if (nth > bound) bound = nth;
-  };
-  int seen = begin, draw = begin;  // where the steps begin that the list has not been thinned out behind, and behind the last of them
-  auto settle = [&](int behind) {  // the list is thinned out behind the steps before `behind`
-    __syncthreads();
-    if (sh.count > kList) {
-      if (tid == 0) sh.count = min(seen > begin ? a.n_top : 0, kList);  // what was kept lies in front
-      __syncthreads();
-      for (int s = seen; s < behind; s += kStep) careful(s);
+  int first_at = mine;  // the step with the thread's maximum
+  float second = -INFINITY;  // the largest of its other steps
+  uint64_t before2 = f2_pack(0.f, 0.f);  // (whole numbers below 2^24)
+  int equals = 0;
+  auto values_of = [&](const uint4& u, const uint4& v, float(&f)[E]) {
+    if constexpr (F32) {
+      f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+      f[4] = __uint_as_float(v.x); f[5] = __uint_as_float(v.y); f[6] = __uint_as_float(v.z); f[7] = __uint_as_float(v.w);
     } else {
-      const u64 nth = thin_out(sh, a.n_top);
-      if (nth > bound) bound = nth;
+      unpack_bf16x8(u, *reinterpret_cast<float(*)[8]>(f));
+      unpack_bf16x8(v, *reinterpret_cast<float(*)[8]>(f + 8));
     }
-    seen = behind;
   };
-  auto whole = [&](int i) { return i + E <= end; };
-  auto fetch = [&](int i, int place) {
+  auto entries_at = [&](int i, float(&f)[E]) {  // -inf behind the last
     if (whole(i)) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(piece_at(i, 0))), v = __ldg(reinterpret_cast<const uint4*>(piece_at(i, 1)));
+      values_of(u, v, f);
+    } else {
 #pragma unroll
-      for (int k = 0; k < WIDE; ++k) copy16(&ring.v[place][k][tid], static_cast<const uint8_t*>(row) + (size_t)i * (F32 ? 4 : 2) + 16 * k);
+      for (int e = 0; e < E; ++e) f[e] = id_of(i, e) < end ? logit_at<F32>(row, id_of(i, e)) : -INFINITY;
     }
-    copy_commit();
   };
-#pragma unroll
-  for (int k = 0; k < AHEAD; ++k) fetch(begin + k * kStep + tid * E, k);
   int place = 0;
-  if constexpr (TOP) {
-    if (begin < end) careful(begin);
-    seen = begin + kStep;
-    draw = begin + 2 * kStep;
-  }
   for (int i0 = begin; i0 < end; i0 += kStep) {
-    const int i = i0 + tid * E;
+    const int i = mine + (i0 - begin);
     float f[E];
-    copy_wait<AHEAD - 1>();
+    copy_wait<kAhead - 1>();
     if (whole(i)) {
-      const uint4 u = ring.v[place][0][tid];
-      if constexpr (F32) {
-        const uint4 v = ring.v[place][WIDE - 1][tid];
-        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-        f[4] = __uint_as_float(v.x); f[5] = __uint_as_float(v.y); f[6] = __uint_as_float(v.z); f[7] = __uint_as_float(v.w);
-      } else {
-        unpack_bf16x8(u, f);
-      }
+      values_of(ring.v[place][0][tid], ring.v[place][1][tid], f);
     } else {
       entries_at(i, f);
     }
-    fetch(i + AHEAD * kStep, place);
-    place = place + 1 == AHEAD ? 0 : place + 1;
-    const float top = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+    fetch(i + kAhead * kStep, place);
+    place = place + 1 == kAhead ? 0 : place + 1;
+    float top = f[0];
+#pragma unroll
+    for (int e = 1; e + 1 < E; e += 2) top = max3(top, f[e], f[e + 1]);
+    top = fmaxf(top, f[E - 1]);
     if (top > my.m) {
       if (my.m > -INFINITY) {
         const float d = my.m - top, w = exp2_fast(d * kLog2e);
         my.u = w > 0.f ? w * fmaf(d, my.s, my.u) : 0.f;
         my.s *= w;
       }
+      second = my.m;
       my.m = top;
+      first_at = i;
+    } else {
+      second = fmaxf(second, top);
     }
     const float m = my.m > -INFINITY ? my.m : 0.f;
     const uint64_t off = f2_pack(-m, -m), log2e = f2_pack(kLog2e, kLog2e);
@@ -252,74 +243,165 @@ __global__ void __launch_bounds__(kThreads, 3) token_scores_kernel(const TokenSc
     my.s += lo + hi;
     f2_unpack(u2, lo, hi);
     my.u += lo + hi;
-    if (i >= end) {  // (nothing: the -inf in its place is no token)
-    } else if (i + E <= target) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) before += f[e] >= xt;
-    } else if (i > target) {
+    for (int k = 0; k < kWide; ++k) {
+      const int j = id_of(i, k * P);
+      const float line = j >= end ? __uint_as_float(0x7fffffffu) : j + P <= target ? xt : above;
 #pragma unroll
-      for (int e = 0; e < E; ++e) before += f[e] > xt && i + e < end;
-    } else {
+      for (int e = k * P; e < (k + 1) * P; e += 2) before2 = f2_add(before2, f2_pack(at_least(f[e], line), at_least(f[e + 1], line)));
+      if (j < end && j <= target && target < j + P) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) before += i + e < end && (f[e] > xt || (f[e] == xt && i + e < target));
-    }
-    if constexpr (TOP) {
-      if (i0 > begin) {  // (the first step has been seen)
-        if (ordered(top) >= (uint32_t)(bound >> 32)) list(f, i);
-        if (i0 + kStep >= draw && i0 + kStep < end) {
-          settle(i0 + kStep);
-          draw = i0 + kStep + (i0 + kStep - begin);
-        }
+        for (int e = 0; e < P; ++e) equals += j + e < target && f[k * P + e] == xt;
       }
     }
   }
+  float b0, b1;
+  f2_unpack(before2, b0, b1);
+  int before = (int)b0 + (int)b1 + equals;
   if constexpr (TOP) {
-    if (seen < end) settle(end);
+    const int n = a.n_top;
+    u64 first = 0;  // the thread's earliest place
+    float f[E];
+    int i = first_at;
+    for (; i < end; i += kStep) {  // (where its maximum is -inf, the first that is no NaN may lie further on)
+      entries_at(i, f);
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (id_of(i, e) < end && f[e] == my.m) first = place_of(f[e], id_of(i, e));
+      if (first) break;
+    }
+    sh.best[tid] = first;
+    if (tid == 0) sh.candidates = 0;
+    __syncthreads();
+    if (warp == 0) {  // the n-th of them, bit by bit: of the values, and where these tie of the ids
+      u64 theirs[kThreads / 32];
+      uint32_t high = 0, low = ~0u;
+      int live = 0;
+#pragma unroll
+      for (int k = 0; k < kThreads / 32; ++k) {
+        theirs[k] = sh.best[k * 32 + lane];
+        high = max(high, (uint32_t)(theirs[k] >> 32));
+        low = min(low, (uint32_t)(theirs[k] >> 32));
+        live += theirs[k] != 0;
+      }
+      u64 at = 0;
+      if (__reduce_add_sync(0xffffffffu, live) > n) {
+        high = __reduce_max_sync(0xffffffffu, high);
+        low = __reduce_min_sync(0xffffffffu, low);
+        int bit = high == low ? -1 : 31 - __clz(high ^ low);
+        uint32_t key = bit < 0 ? high : bit == 31 ? 0 : high & ~((2u << bit) - 1);
+        int c = 0;
+        for (; bit >= 0; --bit) {
+          const uint32_t trial = key | 1u << bit;
+          int above = 0;
+#pragma unroll
+          for (int k = 0; k < kThreads / 32; ++k) above += (uint32_t)(theirs[k] >> 32) >= trial;
+          above = __reduce_add_sync(0xffffffffu, above);
+          if (above >= n) {
+            key = trial;
+            c = above;
+            if (c == n) break;
+          }
+        }
+        at = (u64)key << 32;
+        if (c != n)
+          for (bit = 31; bit >= 0; --bit) {
+            const u64 trial = at | 1ull << bit;
+            int above = 0;
+#pragma unroll
+            for (int k = 0; k < kThreads / 32; ++k) above += theirs[k] >= trial;
+            above = __reduce_add_sync(0xffffffffu, above);
+            if (above >= n) {
+              at = trial;
+              if (above == n) break;
+            }
+          }
+      }
+      if (lane == 0) sh.bound = at ? at - 1 : 0;
+    }
+    __syncthreads();
+    u64 bound = sh.bound;  // what is listed lies above it
+    auto list = [&](const float(&f)[E], int i) {  // those of a thread's entries of a step
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const u64 place = id_of(i, e) < end ? place_of(f[e], id_of(i, e)) : 0ull;
+        if (place > bound) {
+          const int to = atomicAdd(&sh.count, 1);
+          if (to < kList) sh.list[to] = place;
+        }
+      }
+    };
+    if (first > bound) {  // (n threads at most)
+      list(f, i);
+      if (ordered(second) >= (uint32_t)(bound >> 32)) sh.candidate[atomicAdd(&sh.candidates, 1)] = tid;
+    }
+    sh.step[tid] = i;
+    __syncthreads();
+    const int candidates = sh.candidates;
+    for (int k = warp; k < candidates; k += kWarps) {  // a warp looks through the other entries of one of them, a step per lane
+      const int c = sh.candidate[k], done = sh.step[c];
+      for (int j = first_of(c) + lane * kStep; j < end; j += 32 * kStep) {
+        if (j == done) continue;
+        float g[E];
+        entries_at(j, g);
+        float top = g[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) top = fmaxf(top, g[e]);
+        if (ordered(top) >= (uint32_t)(bound >> 32)) list(g, j);
+      }
+    }
+    __syncthreads();
+    if (sh.count > kList) {
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      for (int i0 = begin; i0 < end; i0 += kStep) {
+        if (first > bound) {
+          entries_at(mine + (i0 - begin), f);
+          list(f, mine + (i0 - begin));
+        }
+        __syncthreads();
+        const int count = sh.count;
+        __syncthreads();
+        if (count > kMost) {
+          const u64 nth = thin_out(sh, n);
+          bound = nth > bound + 1 ? nth - 1 : bound;
+        }
+      }
+    }
+    thin_out(sh, n);
   }
 
   // the block's sums
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other{__shfl_xor_sync(0xffffffffu, my.m, o), __shfl_xor_sync(0xffffffffu, my.s, o), __shfl_xor_sync(0xffffffffu, my.u, o)};
-    my = lane & o ? join(other, my) : join(my, other);
-  }
+  my = join_lanes(my, 32);
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) {
     sh.warp_sums[warp] = my;
     sh.warp_before[warp] = before;
   }
   __syncthreads();
-  if (tid == 0) {
-    Sums all = sh.warp_sums[0];
-    int n = sh.warp_before[0];
-    for (int w = 1; w < kWarps; ++w) {
-      all = join(all, sh.warp_sums[w]);
-      n += sh.warp_before[w];
-    }
+  Sums all = join_lanes(sh.warp_sums[lane % kWarps], kWarps);
+  int n_before = __reduce_add_sync(0xffffffffu, lane < kWarps ? sh.warp_before[lane] : 0);
+  if (NC > 1 && tid == 0) {
     sh.sums = all;
-    sh.before = n;
+    sh.before = n_before;
   }
   if constexpr (TOP) {
     if (NC > 1 && tid < kMost) sh.best[tid] = tid < sh.count ? sh.list[tid] : 0ull;  // (the list is in order)
   }
-  __syncthreads();
-  Sums all = sh.sums;
-  int n_before = sh.before;
   if constexpr (NC > 1) {
-    __syncwarp();
+    __syncthreads();
     cluster_sync_all();
     if (part == 0) {
-      for (int c = 1; c < NC; ++c) {
-        all = join(all, *cluster_ptr<NC>(&sh.sums, c));
-        n_before += *cluster_ptr<NC>(&sh.before, c);
-      }
+      all = join_lanes(*cluster_ptr<NC>(&sh.sums, lane % NC), NC);
+      n_before = __reduce_add_sync(0xffffffffu, lane < NC ? *cluster_ptr<NC>(&sh.before, lane % NC) : 0);
       if constexpr (TOP) {
-        // (no more than 8 x 64 places: one per thread)
-        const int c = tid / kMost, j = tid % kMost;
-        const u64 p = c < NC && j < a.n_top ? *cluster_ptr<NC>(&sh.best[j], c) : 0ull;
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        if (p) sh.list[atomicAdd(&sh.count, 1)] = p;
+        for (int k = tid; k < NC * kMost; k += kThreads) {  // (places enough for all)
+          const u64 p = k % kMost < a.n_top ? *cluster_ptr<NC>(&sh.best[k % kMost], k / kMost) : 0ull;
+          if (p) sh.list[atomicAdd(&sh.count, 1)] = p;
+        }
         __syncthreads();
       }
     }
@@ -368,9 +450,9 @@ cudaError_t launch_nc(cudaStream_t stream, const TokenScoresArgs& a) {
 }
 template <bool F32, bool TOP>
 cudaError_t launch_top(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
-  // blocks per row: twice as many while not all SMs have one of their three and a block keeps some steps
+  // blocks per row: twice as many while not all SMs have their four and a block keeps some steps
   int nc = 1;
-  while (nc < 8 && (long long)a.T * nc * 2 <= 3LL * sms && a.V >= nc * 2 * kStep) nc *= 2;
+  while (nc < 8 && (long long)a.T * nc * 2 <= 4LL * sms && a.V >= nc * 2 * kThreads * kEntries<F32>) nc *= 2;
   switch (nc) {
     case 1: return launch_nc<F32, 1, TOP>(stream, a);
     case 2: return launch_nc<F32, 2, TOP>(stream, a);
