@@ -11,131 +11,163 @@
 namespace hb {
 namespace {
 
-constexpr int E = 8;  // neighbouring entries of a thread: 16 bytes of bf16, 8 of codes
-
 template <bool F32>
-__device__ __forceinline__ void load_entries(const void* row, int i, int K, float (&f)[E]) {
-  if (i + E <= K) {
-    if constexpr (F32) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(row) + i)), b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(row) + i) + 1);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const bf16*>(row) + i), f);
-    }
-  } else {
+constexpr int kPiece = F32 ? 4 : 8;  // neighbouring entries of a thread: 16 bytes
+
+// A piece as it lies in memory, zeros behind the last entry
+template <bool F32>
+__device__ __forceinline__ uint4 load_piece(const void* row, int i, int K) {
+  constexpr int E = kPiece<F32>;
+  if (i + E <= K) return *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + (size_t)i * (F32 ? 4 : 2));
+  uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      f[e] = i + e < K ? (F32 ? static_cast<const float*>(row)[i + e] : __bfloat162float(static_cast<const bf16*>(row)[i + e])) : 0.f;
+  for (int e = 0; e < E; ++e)
+    if (i + e < K) {
+      if constexpr (F32) u[e] = static_cast<const uint32_t*>(row)[i + e];
+      else u[e / 2] |= (uint32_t) static_cast<const uint16_t*>(row)[i + e] << (16 * (e & 1));
+    }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <bool F32, int E = kPiece<F32>>
+__device__ __forceinline__ void entries_of(const uint4& u, float (&f)[E]) {
+  if constexpr (F32) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  } else {
+    unpack_bf16x8(u, f);
   }
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
-// c for one entry.  x times the rounded 1 / s is off by at most 127 * 2^-23 < 2^-16: only quotients that lie within that of the middle of two codes need more, and there the
-// products in 64 bits are exact (8 + 24 bits).  Nearly no entry goes there.
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-  const float q = x * inv, r = rintf(q);
-  int c = (int)r;
-  if (fabsf(q - r) > 0.5f - 0x1p-15f) {
-    const float lower = floorf(fabsf(q));  // (the middle is lower + 1/2: no quotient this near to it has another whole part)
-    const double d = (double)fabsf(x) - ((double)lower + 0.5) * (double)s;
-    const int n = (int)lower;
-    const int m = d > 0.0 ? n + 1 : d < 0.0 ? n : n + (n & 1);
-    c = x < 0.f ? -m : m;
-  }
-  return max(-127, min(127, c));
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The whole number nearest to x / s where x times the rounded 1 / s lies within 2^-15 of the middle of two (that product is off by 127 * 2^-24 at most: elsewhere it decides
+// alone).  The products in 64 bits are exact (8 + 24 bits).  Nearly no entry comes here.
+__device__ __noinline__ float near_middle(float x, float s, float inv) {
+  const float lower = floorf(fabsf(x * inv));  // (no quotient this near to the middle has another whole part)
+  const double d = (double)fabsf(x) - ((double)lower + 0.5) * (double)s;
+  const int n = (int)lower;
+  const int m = d > 0.0 ? n + 1 : d < 0.0 ? n : n + (n & 1);
+  return x < 0.f ? -(float)m : (float)m;
 }
 // where 1 / s has no normal fp32 value: the quotient in 64 bits (24 + 24 bits: what is not the middle is 2^-48 from it at least)
-__device__ __noinline__ int code_of_small(float x, float s) { return max(-127, min(127, (int)rint((double)x / (double)s))); }
+__device__ __noinline__ float of_small(float x, float s) { return (float)fmax(-127.0, fmin(127.0, rint((double)x / (double)s))); }
 
 template <bool F32, int WARPS, int CH>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) rows_q8_kernel(const RowsQ8Args a) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int STEP = WARPS * 32 * E;  // entries of a row that its threads take at a time
+  constexpr int E = kPiece<F32>, STEP = WARPS * 32 * E;  // entries of a row that its threads take at a time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = WARPS == 1 ? blockIdx.x * 4 + warp : blockIdx.x;
   const int at = (WARPS == 1 ? lane : (int)threadIdx.x) * E;
   if (t >= a.T) return;  // (whole warps where a row has one, else nobody)
   const void* row = static_cast<const uint8_t*>(a.x) + (size_t)t * a.ldx * (F32 ? 4 : 2);
-  float f[CH][E];
-  uint32_t top = 0;  // of the magnitudes' bits, which are ordered as the magnitudes are, infinities and NaN above all
-  auto look = [&](const float(&v)[E]) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  uint4 x[CH];
+  float top = 0.f;
+  uint32_t top2 = 0;
+  auto look = [&](const uint4& u) {
+    if constexpr (F32) {
+      top = max3_nan(top, fabsf(__uint_as_float(u.x)), fabsf(__uint_as_float(u.y)));
+      top = max3_nan(top, fabsf(__uint_as_float(u.z)), fabsf(__uint_as_float(u.w)));
+    } else {
+      constexpr uint32_t kAbs = 0x7fff7fffu;
+      top2 = max_nan_bf16x2(max_nan_bf16x2(max_nan_bf16x2(top2, u.x & kAbs), max_nan_bf16x2(u.y & kAbs, u.z & kAbs)), u.w & kAbs);
+    }
   };
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    load_entries<F32>(row, min(c * STEP + at, a.K), a.K, f[c]);
-  }
+  for (int c = 0; c < CH; ++c) x[c] = load_piece<F32>(row, min(c * STEP + at, a.K), a.K);
 #pragma unroll
-  for (int c = 0; c < CH; ++c) look(f[c]);
-  for (int i = CH * STEP + at; i < a.K; i += STEP) {
-    float v[E];
-    load_entries<F32>(row, i, a.K, v);
-    look(v);
+  for (int c = 0; c < CH; ++c) look(x[c]);
+  for (int i = CH * STEP + at; i < a.K; i += STEP) look(load_piece<F32>(row, i, a.K));
+  if constexpr (!F32) {
+    const float2 two = unpack_bf16x2(top2);
+    top = max3_nan(top, two.x, two.y);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  // (magnitudes are ordered as their bits are, NaN above all)
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if constexpr (WARPS > 1) {
     __shared__ uint32_t tops[WARPS];
-    if (lane == 0) tops[warp] = top;
+    if (lane == 0) tops[warp] = bits;
     __syncthreads();
-    top = __reduce_max_sync(0xffffffffu, lane < WARPS ? tops[lane] : 0u);
+    bits = __reduce_max_sync(0xffffffffu, lane < WARPS ? tops[lane] : 0u);
   }
-  const float s = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7fffffffu);
+  const float s = bits < 0x7f800000u ? __fdiv_rn(__uint_as_float(bits), 127.f) : __uint_as_float(0x7fffffffu);
   const bool live = s > 0.f, small = s < 0x1p-100f;
-  const float inv = live ? __frcp_rn(s) : 0.f;
+  const float inv = live && !small ? __frcp_rn(s) : 0.f;
   if (at == 0) a.scales[t] = s;
   int8_t* codes = a.codes + (size_t)t * a.ldc;
   bf16* seen = a.seen ? a.seen + (size_t)t * a.lds : nullptr;
-  auto write = [&](int i, const float(&v)[E]) {
+  auto write = [&](int i, const uint4& u) {
     if (i >= a.K) return;
-    int c[E];
-    if (!live) {
+    float v[E];
+    entries_of<F32>(u, v);
+    // adding 3 * 2^22 rounds to a whole number, whose low byte is the code
+    constexpr float kWhole = 12582912.f;
+    const uint64_t inv2 = f2_pack(inv, inv), up = f2_pack(kWhole, kWhole), down = f2_pack(-kWhole, -kWhole), minus = f2_pack(-1.f, -1.f);
+    float w[E], far = 0.f;  // the code with its 3 * 2^22
 #pragma unroll
-      for (int e = 0; e < E; ++e) c[e] = 0;
-    } else if (small) {
+    for (int e = 0; e < E; e += 2) {
+      const uint64_t x = f2_pack(v[e], v[e + 1]), y = f2_fma(x, inv2, up), r = f2_add(y, down), off = f2_fma(x, inv2, f2_mul(r, minus));
+      float o0, o1;
+      f2_unpack(off, o0, o1);
+      f2_unpack(y, w[e], w[e + 1]);
+      far = max3_nan(far, fabsf(o0), fabsf(o1));
+    }
+    if (!live || small || !(far <= 0.5f - 0x1p-15f)) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) c[e] = code_of_small(v[e], s);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) c[e] = code_of(v[e], s, inv);
+      for (int e = 0; e < E; ++e) {
+        if (!live) w[e] = kWhole;
+        else if (small) w[e] = kWhole + of_small(v[e], s);
+        else if (fabsf(fmaf(v[e], inv, kWhole - w[e])) > 0.5f - 0x1p-15f) w[e] = kWhole + near_middle(v[e], s, inv);
+      }
     }
     if (i + E <= a.K) {
-      uint2 o;
-      o.x = (c[0] & 255) | (c[1] & 255) << 8 | (c[2] & 255) << 16 | (uint32_t)c[3] << 24;
-      o.y = (c[4] & 255) | (c[5] & 255) << 8 | (c[6] & 255) << 16 | (uint32_t)c[7] << 24;
-      *reinterpret_cast<uint2*>(codes + i) = o;
+      uint32_t o[E / 4];
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        o[e / 4] = __byte_perm(__byte_perm(__float_as_uint(w[e]), __float_as_uint(w[e + 1]), 0x0040), __byte_perm(__float_as_uint(w[e + 2]), __float_as_uint(w[e + 3]), 0x0040), 0x5410);
+      if constexpr (E == 8) *reinterpret_cast<uint2*>(codes + i) = make_uint2(o[0], o[1]);
+      else *reinterpret_cast<uint32_t*>(codes + i) = o[0];
       if (seen) {
-        uint4 w;
-        w.x = pack_bf16x2(s * (float)c[0], s * (float)c[1]);
-        w.y = pack_bf16x2(s * (float)c[2], s * (float)c[3]);
-        w.z = pack_bf16x2(s * (float)c[4], s * (float)c[5]);
-        w.w = pack_bf16x2(s * (float)c[6], s * (float)c[7]);
-        *reinterpret_cast<uint4*>(seen + i) = w;
+        uint32_t u[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          float x0, x1;
+          f2_unpack(f2_mul(f2_add(f2_pack(w[e], w[e + 1]), down), f2_pack(s, s)), x0, x1);
+          u[e / 2] = pack_bf16x2(x0, x1);
+        }
+        if constexpr (E == 8) *reinterpret_cast<uint4*>(seen + i) = make_uint4(u[0], u[1], u[2], u[3]);
+        else *reinterpret_cast<uint2*>(seen + i) = make_uint2(u[0], u[1]);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (i + e < a.K) {
-          codes[i + e] = (int8_t)c[e];
-          if (seen) seen[i + e] = __float2bfloat16(s * (float)c[e]);
+          codes[i + e] = (int8_t)__float_as_uint(w[e]);
+          if (seen) seen[i + e] = __float2bfloat16(s * (w[e] - kWhole));
         }
     }
   };
 #pragma unroll
-  for (int c = 0; c < CH; ++c) write(c * STEP + at, f[c]);
-  for (int i = CH * STEP + at; i < a.K; i += STEP) {
-    float v[E];
-    load_entries<F32>(row, i, a.K, v);
-    write(i, v);
-  }
+  for (int c = 0; c < CH; ++c) write(c * STEP + at, x[c]);
+  for (int i = CH * STEP + at; i < a.K; i += STEP) write(i, load_piece<F32>(row, i, a.K));
 }
 
-template <bool F32>
+// A row's threads: as few warps as hold it in registers, 1024 entries each
+template <bool F32, int WARPS>
 cudaError_t launch_rows(cudaStream_t stream, const RowsQ8Args& a) {
-  if (a.K <= 1024) return launch_k(rows_q8_kernel<F32, 1, 4>, dim3((a.T + 3) / 4), dim3(128), 0, stream, true, a);
-  if (a.K <= 4096) return launch_k(rows_q8_kernel<F32, 4, 4>, dim3(a.T), dim3(128), 0, stream, true, a);
-  if (a.K <= 8192) return launch_k(rows_q8_kernel<F32, 8, 4>, dim3(a.T), dim3(256), 0, stream, true, a);
-  return launch_k(rows_q8_kernel<F32, 16, 4>, dim3(a.T), dim3(512), 0, stream, true, a);
+  if constexpr (WARPS < 16) {
+    if (a.K > WARPS * 1024) return launch_rows<F32, (WARPS < 4 ? WARPS + 1 : WARPS + 2)>(stream, a);
+  }
+  return launch_k(rows_q8_kernel<F32, WARPS, 1024 / (32 * kPiece<F32>)>, dim3(WARPS == 1 ? (a.T + 3) / 4 : a.T), dim3(WARPS == 1 ? 128 : WARPS * 32), 0, stream, true, a);
 }
 
 }  // namespace
@@ -146,7 +178,7 @@ cudaError_t rows_q8(cudaStream_t stream, const RowsQ8Args& a) {
   if (!a.x || ((uintptr_t)a.x & 15) || a.ldx < a.K || a.ldx % 8 || !a.codes || ((uintptr_t)a.codes & 15) || a.ldc < a.K || a.ldc % 16 || !a.scales || ((uintptr_t)a.scales & 3) ||
       (a.seen && (((uintptr_t)a.seen & 15) || a.lds < a.K || a.lds % 8)))
     return cudaErrorInvalidValue;
-  return a.x_f32 ? launch_rows<true>(stream, a) : launch_rows<false>(stream, a);
+  return a.x_f32 ? launch_rows<true, 1>(stream, a) : launch_rows<false, 1>(stream, a);
 }
 
 }  // namespace hb
