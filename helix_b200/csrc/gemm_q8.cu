@@ -70,16 +70,22 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// x Phi(x) with erfc by Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most)
-__device__ __forceinline__ float gelu_erf(float x) {
-  const float z = fabsf(x) * 0.70710678118654752f;
-  const float t = rcp_fast(fmaf(0.3275911f, z, 1.f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float h = 0.5f * p * t * exp2_fast(-z * z * kLog2e);
-  return x * (x > 0.f ? 1.f - h : h);
+// x Phi(x) = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 for two values, erfc by Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most; nothing is left of it at 16)
+__device__ __forceinline__ void gelu_erf2(float& x0, float& x1) {
+  auto c2 = [](float c) { return f2_pack(c, c); };
+  const uint64_t ax = f2_pack(fminf(fabsf(x0), 16.f), fminf(fabsf(x1), 16.f)), z = f2_mul(ax, c2(0.70710678118654752f));
+  float a0, a1, e0, e1;
+  f2_unpack(f2_fma(z, c2(0.3275911f), c2(1.f)), a0, a1);
+  const uint64_t t = f2_pack(rcp_fast(a0), rcp_fast(a1));
+  uint64_t p = f2_fma(t, c2(-0.5f * 1.061405429f), c2(0.5f * 1.453152027f));
+  p = f2_fma(p, t, c2(-0.5f * 1.421413741f));
+  p = f2_fma(p, t, c2(0.5f * 0.284496736f));
+  p = f2_mul(f2_fma(p, t, c2(-0.5f * 0.254829592f)), t);
+  f2_unpack(f2_mul(f2_mul(z, z), c2(-kLog2e)), e0, e1);
+  p = f2_mul(p, f2_pack(exp2_fast(e0), exp2_fast(e1)));
+  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(x0));
+  asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(x1));
+  f2_unpack(f2_fma(ax, p, f2_pack(x0, x1)), x0, x1);
 }
 // tanh: 1 - 2 / (e^2|x| + 1), and where that cancels (|x| < 1/4) its series, whose next term is 2^-26 of it
 __device__ __forceinline__ float tanh_fast(float x) {
@@ -91,7 +97,7 @@ __device__ __forceinline__ float tanh_fast(float x) {
   const float y = copysignf(fmaf(-2.f, rcp_fast(exp2_fast(fabsf(x) * (2.f * kLog2e)) + 1.f), 1.f), x);
   return u < 0.0625f ? p : y;
 }
-__device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
+__device__ __forceinline__ float silu(float x) { return x * rcp_fast(1.f + exp2_fast(-kLog2e * x)); }
 
 __host__ __device__ constexpr bool has_bias(int epi) { return epi == EPI_BIAS || epi == EPI_BIAS_GELU || epi == EPI_BIAS_RESID; }
 __host__ __device__ constexpr bool has_resid(int epi) { return epi == EPI_RESID || epi == EPI_BIAS_RESID; }
@@ -121,19 +127,18 @@ __device__ __forceinline__ int k_at(int kb) {  // a block's first entry
   return kb * (I8 ? KB : KB / 2);
 }
 
-template <int BN, int CG, int EPI>
+template <bool I8, int BN, int CG, int EPI>
 struct Cfg {
-  static constexpr int EG = 2;  // groups of four warps behind the products
+  static constexpr int EG = I8 ? 4 : 2;  // groups of four warps behind the products (two where a thread holds sums of 128 columns)
   static constexpr int THREADS = 64 + EG * 128;
   static constexpr int X_BYTES = TM * KB, W_BYTES = BN / CG * KB;
   static constexpr int STAGE = X_BYTES + W_BYTES;
-  static constexpr int STAGING = EPI == EPI_SCORES ? 0 : EG * kStaging;
+  static constexpr int STAGING = EPI == EPI_SCORES ? 0 : 2 * kStaging;
   static constexpr int FIXED = STAGING + 1024 + 512;  // alignment, barriers
   static constexpr int RAW = (227 * 1024 - FIXED) / STAGE;
   static constexpr int STAGES = RAW > 10 ? 10 : RAW;
   static constexpr int SMEM = STAGES * STAGE + FIXED;
-  static constexpr int COLS = 2 * BN;  // of tensor memory
-  static_assert(COLS == 128 || COLS == 256 || COLS == 512, "columns are allocated in powers of two");
+  static constexpr int COLS = 2 * BN > 256 ? 512 : 2 * BN > 128 ? 256 : 128;  // of tensor memory (allocated in powers of two)
 };
 
 __device__ __forceinline__ void tile_at(const TileArgs& a, int t, int num_m, int num_n, int& mi, int& ni) {
@@ -144,29 +149,28 @@ __device__ __forceinline__ void tile_at(const TileArgs& a, int t, int num_m, int
   ni = a.group_n ? x : y;
 }
 
-// 32 sums of a row to values: the whole numbers times both scales, or the fp32 sums themselves
-template <bool I8>
-__device__ __forceinline__ void values_of(const uint32_t (&v)[32], const TileArgs& a, float sx, int n0, float (&f)[32]) {
+// NC sums of a row to values: the whole numbers times both scales, or the fp32 sums themselves
+template <bool I8, int NC>
+__device__ __forceinline__ void values_of(const uint32_t (&v)[NC], const TileArgs& a, float sx, int n0, float (&f)[NC]) {
   if constexpr (I8) {
-    if (n0 + 32 <= a.N) {
+    if (n0 + NC <= a.N) {
+      const uint64_t s2 = f2_pack(sx, sx);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 w = __ldg(reinterpret_cast<const float4*>(a.ws + n0) + j);
-        f[4 * j] = (float)(int)v[4 * j] * w.x * sx;
-        f[4 * j + 1] = (float)(int)v[4 * j + 1] * w.y * sx;
-        f[4 * j + 2] = (float)(int)v[4 * j + 2] * w.z * sx;
-        f[4 * j + 3] = (float)(int)v[4 * j + 3] * w.w * sx;
+      for (int j = 0; j < NC; j += 4) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(a.ws + n0 + j));
+        f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j], (float)(int)v[j + 1]), f2_pack(w.x, w.y)), s2), f[j], f[j + 1]);
+        f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j + 2], (float)(int)v[j + 3]), f2_pack(w.z, w.w)), s2), f[j + 2], f[j + 3]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
+      for (int j = 0; j < NC; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+    for (int j = 0; j < NC; ++j) f[j] = __uint_as_float(v[j]);
   }
 }
-// 32 bf16 values of a row (of N) added
+// 32 bf16 values of a row (of which `left` are there) added
 __device__ __forceinline__ void add_32(const bf16* p, int left, float (&f)[32]) {
   if (left >= 32) {
 #pragma unroll
@@ -174,7 +178,7 @@ __device__ __forceinline__ void add_32(const bf16* p, int left, float (&f)[32]) 
       float b[8];
       unpack_bf16x8(*(reinterpret_cast<const uint4*>(p) + j), b);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[8 * j + k] += b[k];
+      for (int k = 0; k < 8; k += 2) f2_unpack(f2_add(f2_pack(f[8 * j + k], f[8 * j + k + 1]), f2_pack(b[k], b[k + 1])), f[8 * j + k], f[8 * j + k + 1]);
     }
   } else {
 #pragma unroll
@@ -184,10 +188,10 @@ __device__ __forceinline__ void add_32(const bf16* p, int left, float (&f)[32]) 
 }
 
 template <bool I8, int BN, int CG, int EPI>
-__global__ void __launch_bounds__(Cfg<BN, CG, EPI>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<I8, BN, CG, EPI>::THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
             const __grid_constant__ TileArgs a) {
-  using C = Cfg<BN, CG, EPI>;
+  using C = Cfg<I8, BN, CG, EPI>;
   constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG;
   constexpr bool kScores = EPI == EPI_SCORES, kGlu = EPI == EPI_SWIGLU, kF32 = EPI == EPI_F32;
   constexpr int OUT_BN = kGlu ? BN / 2 : BN, CHUNK = kF32 ? 32 : 64, NCHUNK = OUT_BN / CHUNK;
@@ -313,8 +317,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
   } else {
     const int q = warp & 3, row = q * 32 + lane;  // row of the block's 128, lane of tensor memory
     const int grp = (warp - 2) >> 2;
-    const bool leader = ((threadIdx.x - 64) & 127) == 0;
-    uint8_t* const buf = staging + grp * kStaging;
+    // products: two groups share a chunk of 128 bytes per row, half each; scores: each has its columns
+    constexpr int TEAM = kScores ? 128 : 256;
+    const int team = kScores ? grp : grp >> 1, half = grp & 1;
+    const bool leader = (threadIdx.x - 64) % TEAM == 0;
+    uint8_t* const buf = staging + team * kStaging;
     uint8_t* const my_row = buf + row * 128;
     float m = -INFINITY, S = 0.f, U = 0.f;  // scores
     const bool carry = num_m == 1;          // a row's sums go on through the block's tiles
@@ -335,7 +342,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       int as = 0;
       auto sums_there = [&] {
         as = it & 1;
-        ok = all_of(1 + grp, 128, wait_turn(&sums_full[as], (it >> 1) & 1, a.wait_cycles));
+        ok = all_of(1 + team, TEAM, wait_turn(&sums_full[as], (it >> 1) & 1, a.wait_cycles));
         tc_fence_after();
         t_row = tmem + as * BN + (static_cast<uint32_t>(q * 32) << 16);
         ++it;
@@ -457,63 +464,68 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         if (!sums_there()) break;
         const int n_out0 = ni * OUT_BN, n_out = kGlu ? a.N / 2 : a.N;
 #pragma unroll 1
-        for (int c = grp; c < NCHUNK; c += EG) {
-          if (leader) tma_store_wait_read<0>();  // the group's store before has read `buf`
-          bar_sync(1 + grp, 128);
+        for (int c = team; c < NCHUNK; c += EG / 2) {
+          const bool last = c + EG / 2 >= NCHUNK;
+          if (leader) tma_store_wait_read<0>();  // the team's store before has read `buf`
           if constexpr (kF32) {
-            uint32_t v[32];
-            float f[32];
-            tmem_ld_32x32b_x32(t_row + c * 32, v);
+            const int col = c * 32 + half * 16;
+            uint32_t v[16];
+            float f[16];
+            tmem_ld_32x32b_x16(t_row + col, v);
             tmem_ld_wait();
-            if (c + EG >= NCHUNK) release();
-            values_of<I8>(v, a, sx, n_out0 + c * 32, f);
+            if (last) release();
+            values_of<I8>(v, a, sx, n_out0 + col, f);
+            bar_sync(1 + team, TEAM);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(my_row + ((j ^ (row & 7)) << 4)) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(my_row + (((half * 4 + j) ^ (row & 7)) << 4)) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
           } else {
+            const int col = c * 64 + half * 32, n0 = n_out0 + col;
+            float f[32];
+            if constexpr (kGlu) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int col = c * 64 + h * 32, n0 = n_out0 + col;
+              for (int h = 0; h < 32; h += 16) {
+                uint32_t v[16], u[16];
+                float g[16], x[16];
+                tmem_ld_32x32b_x16(t_row + col + h, v);
+                tmem_ld_32x32b_x16(t_row + 128 + col + h, u);
+                tmem_ld_wait();
+                if (h == 16 && last) release();
+                values_of<I8>(v, a, sx, ni * BN + col + h, g);
+                values_of<I8>(u, a, sx, ni * BN + 128 + col + h, x);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[h + j] = silu(g[j]) * x[j];
+              }
+            } else {
               uint32_t v[32];
-              float f[32];
               tmem_ld_32x32b_x32(t_row + col, v);
-              if constexpr (kGlu) {
-                uint32_t u[32];
-                float g[32];
-                tmem_ld_32x32b_x32(t_row + 128 + col, u);
-                tmem_ld_wait();
-                if (h == 1 && c + EG >= NCHUNK) release();
-                values_of<I8>(v, a, sx, ni * BN + col, g);
-                values_of<I8>(u, a, sx, ni * BN + 128 + col, f);
+              tmem_ld_wait();
+              if (last) release();
+              values_of<I8>(v, a, sx, n0, f);
+            }
+            if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
+            if constexpr (EPI == EPI_BIAS_GELU) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] *= silu(g[j]);
-              } else {
-                tmem_ld_wait();
-                if (h == 1 && c + EG >= NCHUNK) release();
-                values_of<I8>(v, a, sx, n0, f);
-              }
-              if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
-              if constexpr (EPI == EPI_BIAS_GELU) {
+              for (int j = 0; j < 32; j += 2) gelu_erf2(f[j], f[j + 1]);
+            }
+            if constexpr (has_resid(EPI)) {
+              if (live) add_32(a.r + (size_t)row_g * a.ldr + n0, n_out - n0, f);
+            }
+            bar_sync(1 + team, TEAM);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
-              }
-              if constexpr (has_resid(EPI)) {
-                if (live) add_32(a.r + (size_t)row_g * a.ldr + n0, n_out - n0, f);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint4 o;
-                o.x = pack_bf16x2(f[8 * j], f[8 * j + 1]);
-                o.y = pack_bf16x2(f[8 * j + 2], f[8 * j + 3]);
-                o.z = pack_bf16x2(f[8 * j + 4], f[8 * j + 5]);
-                o.w = pack_bf16x2(f[8 * j + 6], f[8 * j + 7]);
-                *reinterpret_cast<uint4*>(my_row + (((h * 4 + j) ^ (row & 7)) << 4)) = o;
-              }
+            for (int j = 0; j < 4; ++j) {
+              uint4 o;
+              o.x = pack_bf16x2(f[8 * j], f[8 * j + 1]);
+              o.y = pack_bf16x2(f[8 * j + 2], f[8 * j + 3]);
+              o.z = pack_bf16x2(f[8 * j + 4], f[8 * j + 5]);
+              o.w = pack_bf16x2(f[8 * j + 6], f[8 * j + 7]);
+              *reinterpret_cast<uint4*>(my_row + (((half * 4 + j) ^ (row & 7)) << 4)) = o;
             }
           }
           const int n0 = n_out0 + c * CHUNK;
           if (n0 + CHUNK > n_out && n_out % (kF32 ? 4 : 8) != 0) {  // (a copy ends on 16 bytes: it would write zeros behind the last column)
             if (live) {
-              for (int j = 0; n0 + j < n_out; ++j) {
+              for (int j = half * (CHUNK / 2); j < (half + 1) * (CHUNK / 2) && n0 + j < n_out; ++j) {
                 const int at = ((j / (kF32 ? 4 : 8)) ^ (row & 7)) << 4, in = j % (kF32 ? 4 : 8);
                 if constexpr (kF32) static_cast<float*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const float*>(my_row + at)[in];
                 else static_cast<bf16*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const bf16*>(my_row + at)[in];
@@ -522,7 +534,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             continue;
           }
           fence_proxy_async_smem();
-          bar_sync(1 + grp, 128);
+          bar_sync(1 + team, TEAM);
           if (leader) {
             tma_store_2d(&map_c, buf, n0, m0);
             tma_store_commit();
@@ -808,7 +820,10 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
       } else {
         f[e] = (float)acc[e] * __ldg(a.ws + n + e) * sx;
         if (a.bias) f[e] += __bfloat162float(a.bias[n + e]);
-        if (a.epi == EPI_BIAS_GELU) f[e] = gelu_erf(f[e]);
+        if (a.epi == EPI_BIAS_GELU) {
+          float other = 0.f;
+          gelu_erf2(f[e], other);
+        }
         if (a.r) f[e] += __bfloat162float(a.r[(size_t)m * a.ldr + n + e]);
       }
       if (bad) f[e] = __uint_as_float(0x7fffffffu);
@@ -890,7 +905,7 @@ bool operand_map(CUtensorMap* map, const Operand& o, int K, int box_rows) {
 
 template <bool I8, int BN, int CG, int EPI>
 cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, const Operand& w, int K, int sms) {
-  using C = Cfg<BN, CG, EPI>;
+  using C = Cfg<I8, BN, CG, EPI>;
   static std::atomic<uint64_t> asked{0};
   cudaError_t e = ask_smem(tile_kernel<I8, BN, CG, EPI>, C::SMEM, asked);
   if (e != cudaSuccess) return e;
@@ -1006,7 +1021,7 @@ cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& g) {
 
 namespace {
 bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
-int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 2 : (V + 255) / 256 * 2; }  // (of a launch with one tile of rows: its blocks', which are fewer)
+int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 4 : (V + 255) / 256 * 4; }  // at most (a launch with one tile of rows has its blocks', bf16 half of them)
 }  // namespace
 
 size_t head_scores_workspace_floats(int T, int V) { return score_sizes_ok(T, V) ? (size_t)T * (3 * (size_t)score_slots(T, V) + 1) : 0; }
@@ -1035,17 +1050,12 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   a.cap = g.softcap;
   a.inv_cap = 1.f / g.softcap;
   const Operand x{g.x, g.ldx, g.T}, w{g.w, g.ldw, g.V};
+  if (sms < 2) return cudaErrorInvalidConfiguration;
   cudaError_t e;
-  int slots;
-  if (g.T <= TM) {
-    e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms);
-    slots = std::min((g.V + 127) / 128, sms) * 2;
-  } else if (sms < 2) {
-    return cudaErrorInvalidConfiguration;
-  } else {
-    e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms);
-    slots = g.T <= 2 * TM ? std::min((g.V + 255) / 256, sms / 2) * 2 : (g.V + 255) / 256 * 2;
-  }
+  if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms);
+  else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms);
+  const int cg = g.T <= TM ? 1 : 2, tiles = (g.V + 128 * cg - 1) / (128 * cg), one = g.T <= TM * cg;  // (one tile of rows: a block's sums go on through its tiles)
+  const int slots = (one ? std::min(tiles, sms / cg) : tiles) * (i8 ? Cfg<true, 128, 1, EPI_SCORES>::EG : Cfg<false, 128, 1, EPI_SCORES>::EG);
   if (e != cudaSuccess) return e;
   return launch_k(join_scores_kernel, dim3((g.T + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp,
                   g.entropy, slots, g.T, g.V);

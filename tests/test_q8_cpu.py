@@ -62,7 +62,7 @@ def test_workspace():
     for T, V in ((1, 1), (32, 128256), (128, 129), (129, 257), (2048, 128256), (100000, 151936)):
         n = L.hbk_head_scores_workspace_floats(T, V)
         tiles = -(-V // (128 if T <= 128 else 256))
-        assert n == T * (6 * tiles + 1)
+        assert n == T * (12 * tiles + 1)
 
 
 def test_the_limit_of_waits():
