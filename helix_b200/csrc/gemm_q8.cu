@@ -87,15 +87,29 @@ __device__ __forceinline__ void gelu_erf2(float& x0, float& x1) {
   asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(x1));
   f2_unpack(f2_fma(ax, p, f2_pack(x0, x1)), x0, x1);
 }
-// tanh: 1 - 2 / (e^2|x| + 1), and where that cancels (|x| < 1/4) its series, whose next term is 2^-26 of it
-__device__ __forceinline__ float tanh_fast(float x) {
-  const float u = x * x;
-  float p = fmaf(u, 62.f / 2835.f, -17.f / 315.f);
-  p = fmaf(p, u, 2.f / 15.f);
-  p = fmaf(p, u, -1.f / 3.f);
-  p = fmaf(p * u, x, x);
-  const float y = copysignf(fmaf(-2.f, rcp_fast(exp2_fast(fabsf(x) * (2.f * kLog2e)) + 1.f), 1.f), x);
-  return u < 0.0625f ? p : y;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+struct Cap {
+  float cap, inv;  // 0: none
+};
+// cap tanh(x / cap) for two values: 1 - 2 / (e^2y + 1), and where that cancels (|y| < 1/4) the series, whose next term is 2^-26 of it
+__device__ __forceinline__ void cap2(const Cap& c, float& x0, float& x1) {
+  auto c2 = [](float c) { return f2_pack(c, c); };
+  const uint64_t x = f2_pack(x0, x1), y = f2_mul(x, c2(c.inv)), u = f2_mul(y, y);
+  float a0, a1, u0, u1, s0, s1;
+  f2_unpack(f2_mul(y, c2(2.f * kLog2e)), a0, a1);
+  f2_unpack(f2_add(f2_pack(exp2_fast(a0), exp2_fast(a1)), c2(1.f)), a0, a1);
+  f2_unpack(f2_fma(f2_pack(rcp_fast(a0), rcp_fast(a1)), c2(-2.f * c.cap), c2(c.cap)), a0, a1);
+  uint64_t p = f2_fma(u, c2(62.f / 2835.f), c2(-17.f / 315.f));
+  p = f2_fma(p, u, c2(2.f / 15.f));
+  p = f2_mul(f2_fma(p, u, c2(-1.f / 3.f)), u);
+  f2_unpack(f2_fma(p, x, x), s0, s1);
+  f2_unpack(u, u0, u1);
+  x0 = u0 < 0.0625f ? s0 : a0;
+  x1 = u1 < 0.0625f ? s1 : a1;
 }
 __device__ __forceinline__ float silu(float x) { return x * rcp_fast(1.f + exp2_fast(-kLog2e * x)); }
 
@@ -114,7 +128,9 @@ struct TileArgs {
   int box_rows;               // rows of a block of X that are loaded
   const int32_t* targets;     // scores
   float *part, *at;           // [slot][3][M], [M]
-  float scale, cap, inv_cap;
+  float scale;
+  Cap cap;
+  int carry;                  // scores: a block's tiles are of the same rows
   long long wait_cycles;
 };
 
@@ -324,7 +340,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     uint8_t* const buf = staging + team * kStaging;
     uint8_t* const my_row = buf + row * 128;
     float m = -INFINITY, S = 0.f, U = 0.f;  // scores
-    const bool carry = num_m == 1;          // a row's sums go on through the block's tiles
+    const bool carry = a.carry != 0;        // a row's sums go on through the block's tiles
     int it = 0;
     for (int t = worker; t < tiles && ok; t += workers) {
       int mi, ni;
@@ -382,9 +398,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] *= sx;
           }
-          if (a.cap > 0.f) {
+          if (a.cap.cap > 0.f) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = a.cap * tanh_fast(f[j] * a.inv_cap);
+            for (int j = 0; j < 32; j += 2) cap2(a.cap, f[j], f[j + 1]);
           }
           if ((unsigned)(target - n0) < 32u) {
             float z = 0.f;
@@ -392,13 +408,15 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             for (int j = 0; j < 32; ++j) z = target - n0 == j ? f[j] : z;
             a.at[row_g] = z;  // (one tile has the target; whether it is below N is asked where it is read)
           }
-          if (n0 + 32 > a.N) {
+          const int left = a.N - n0;
+          if (left < 32) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = n0 + j < a.N ? f[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) f[j] = j < left ? f[j] : -INFINITY;
           }
           float top = f[0];
 #pragma unroll
-          for (int j = 1; j < 32; ++j) top = fmaxf(top, f[j]);
+          for (int j = 1; j < 31; j += 2) top = max3(top, f[j], f[j + 1]);
+          top = fmaxf(top, f[31]);
           if (top > m) {
             if (m > -INFINITY) {
               const float d = m - top, w = exp2_fast(d * kLog2e);
@@ -408,19 +426,19 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             m = top;
           }
           const float base = m > -INFINITY ? m : 0.f;
+          if (left < 32) {  // (0 times what is no infinity)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = j < left ? f[j] : base - 1e4f;
+          }
           const uint64_t off = f2_pack(-base, -base), log2e = f2_pack(kLog2e, kLog2e);
           uint64_t s2 = f2_pack(0.f, 0.f), u2 = s2;  // two at a time
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            uint64_t d = f2_add(f2_pack(f[j], f[j + 1]), off);
+            const uint64_t d = f2_add(f2_pack(f[j], f[j + 1]), off);
             float x0, x1;
             f2_unpack(f2_mul(d, log2e), x0, x1);
             const uint64_t w = f2_pack(exp2_fast(x0), exp2_fast(x1));
             s2 = f2_add(s2, w);
-            if (n0 + 32 > a.N) {  // (0 times what is no infinity)
-              f2_unpack(d, x0, x1);
-              d = f2_pack(fmaxf(x0, -1e4f), fmaxf(x1, -1e4f));
-            }
             u2 = f2_fma(w, d, u2);
           }
           float lo, hi;
@@ -452,7 +470,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
         if (!carry || t + workers >= tiles) {
           if (live) {
-            float* p = a.part + (size_t)((carry ? worker : ni) * EG + grp) * 3 * a.M + row_g;
+            float* p = a.part + (size_t)((carry ? worker / num_m : ni) * EG + grp) * 3 * a.M + row_g;
             p[0] = m;
             p[a.M] = S;
             p[2 * (size_t)a.M] = U;
@@ -590,7 +608,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       if constexpr (kScores) {
         for (int i = threadIdx.x; i < TM * EG; i += C::THREADS) {
           const int r = m0 + i % TM;
-          if (r < a.M) a.part[(size_t)((num_m == 1 ? worker : ni) * EG + i / TM) * 3 * a.M + (size_t)a.M + r] = nan;
+          if (r < a.M) a.part[(size_t)((a.carry ? worker / num_m : ni) * EG + i / TM) * 3 * a.M + (size_t)a.M + r] = nan;
         }
       } else {
         const int n_out = kGlu ? a.N / 2 : a.N;
@@ -614,8 +632,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 }
 
 // ------------------------------------------------------------------ a row's sums of all tiles
-constexpr int kJoinRows = 8, kJoinThreads = 512;
+constexpr int kJoinRows = 8;
 
+template <int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) join_scores_kernel(const float* __restrict__ part, const float* __restrict__ at, const int32_t* __restrict__ targets,
                                                                   float* __restrict__ lp, float* __restrict__ entropy, int slots, int T, int V) {
   __shared__ float sm[3][kJoinThreads];
@@ -674,7 +693,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_scores_kernel(const float* 
 // ------------------------------------------------------------------ few tiles: K shared by a cluster
 constexpr int SN = 128;                  // rows of W of a tile (a gated unit's: 64 of the gate, 64 beside them)
 constexpr int kDump = SN + 4;            // whole numbers of a row on their way through shared memory
-constexpr int kSplitThreads = 192;
+constexpr int kSplitThreads = 320;       // warp 0 loads, warp 1 multiplies, eight take the sums out
 
 struct SplitArgs {
   const float *xs, *ws;
@@ -691,6 +710,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   __shared__ uint64_t full[12], empty[12], sums_full, all_done;
   __shared__ uint32_t tmem_at;
   __shared__ int bad_flag;
+  __shared__ float s_xs[TM], s_ws[SN], s_bias[SN];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
   const int x_bytes = a.box_rows * KB, stages = a.stages;
   uint8_t* smem_w = smem + stages * x_bytes;  // (products read 128 rows of X whatever was loaded: what lies behind goes into rows that nobody reads)
@@ -700,6 +720,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   const int kb0 = (int)((long long)a.kbs * part / parts), kb1 = (int)((long long)a.kbs * (part + 1) / parts);
   const bool glu = a.epi == EPI_SWIGLU;
   const int m0 = blockIdx.z * TM;
+  const int w0 = glu ? blockIdx.y / 2 * 256 + blockIdx.y % 2 * 64 : blockIdx.y * SN, w1 = w0 + (glu ? 128 : 64);  // rows of W: 64 from each
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_x);
     tma_prefetch_desc(&map_w);
@@ -726,7 +747,6 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   int issued = 0;
   if (warp == 0) {
     const bool elected = elect_one_sync();
-    const int w0 = glu ? blockIdx.y / 2 * 256 + blockIdx.y % 2 * 64 : blockIdx.y * SN, w1 = w0 + (glu ? 128 : 64);
     int s = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
@@ -759,12 +779,19 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
     if (ok && elected) umma_commit(&sums_full);
     __syncwarp();
   } else {
+    // scales and bias come while the products are made
+    for (int i = threadIdx.x - 64; i < 3 * 128; i += kSplitThreads - 64) {
+      const int j = i & 127, n = j < 64 ? w0 + j : w1 + j - 64;
+      if (i < 128) s_ws[j] = n < a.N ? __ldg(a.ws + n) : 0.f;
+      else if (i < 256) s_xs[j] = m0 + j < a.M ? __ldg(a.xs + m0 + j) : 0.f;
+      else s_bias[j] = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+    }
     ok = wait_turn(&sums_full, 0, a.wait_cycles);
-    const int q = warp & 3, row = q * 32 + lane;
+    const int q = warp & 3, row = q * 32 + lane, c0 = warp < 6 ? 0 : SN / 2;
     if (ok && q * 32 < a.box_rows) {  // (all operands have been read: their room takes the sums)
       tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < SN; c += 32) {
+#pragma unroll
+      for (int c = c0; c < c0 + SN / 2; c += 32) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
         tmem_ld_wait();
@@ -797,37 +824,49 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   for (int i = part * kSplitThreads + threadIdx.x; i < rows * quads; i += parts * kSplitThreads) {
     const int r = i / quads, c = i % quads * 4, m = m0 + r, n = blockIdx.y * (quads * 4) + c;
     if (n >= n_out) continue;
-    int4 x = make_int4(0, 0, 0, 0), y = x;
-    for (int p = 0; p < parts; ++p) {
-      const int* at = parts == 1 ? dump : cluster_ptr<2>(dump, p);
-      const int4 v = *reinterpret_cast<const int4*>(at + r * kDump + c);
-      x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
-      if (glu) {
-        const int4 w = *reinterpret_cast<const int4*>(at + r * kDump + 64 + c);
-        y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
-      }
-    }
-    const float sx = __ldg(a.xs + m);
-    const int acc[4] = {x.x, x.y, x.z, x.w}, up[4] = {y.x, y.y, y.z, y.w};
-    float f[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[e] = 0.f;
-      if (n + e >= n_out) continue;
-      if (glu) {
-        const int wn = blockIdx.y / 2 * 256 + blockIdx.y % 2 * 64 + c + e;
-        f[e] = (float)up[e] * __ldg(a.ws + wn + 128) * sx * silu((float)acc[e] * __ldg(a.ws + wn) * sx);
+    float resid[4] = {};
+    if (a.r) {
+      const bf16* at = a.r + (size_t)m * a.ldr + n;
+      if (n + 4 <= n_out) {
+        const uint2 u = *reinterpret_cast<const uint2*>(at);
+        const float2 lo = unpack_bf16x2(u.x), hi = unpack_bf16x2(u.y);
+        resid[0] = lo.x; resid[1] = lo.y; resid[2] = hi.x; resid[3] = hi.y;
       } else {
-        f[e] = (float)acc[e] * __ldg(a.ws + n + e) * sx;
-        if (a.bias) f[e] += __bfloat162float(a.bias[n + e]);
-        if (a.epi == EPI_BIAS_GELU) {
-          float other = 0.f;
-          gelu_erf2(f[e], other);
-        }
-        if (a.r) f[e] += __bfloat162float(a.r[(size_t)m * a.ldr + n + e]);
+        for (int e = 0; n + e < n_out; ++e) resid[e] = __bfloat162float(at[e]);
       }
-      if (bad) f[e] = __uint_as_float(0x7fffffffu);
     }
+    auto sum_at = [&](int col, int(&sum)[4]) {  // all parts' numbers at once, added in any order
+      int4 v[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        if (p < parts) v[p] = *reinterpret_cast<const int4*>((parts == 1 ? dump : cluster_ptr<2>(dump, p)) + r * kDump + col);
+      sum[0] = v[0].x; sum[1] = v[0].y; sum[2] = v[0].z; sum[3] = v[0].w;
+#pragma unroll
+      for (int p = 1; p < 8; ++p)
+        if (p < parts) {
+          sum[0] += v[p].x; sum[1] += v[p].y; sum[2] += v[p].z; sum[3] += v[p].w;
+        }
+    };
+    const float sx = s_xs[r];
+    int acc[4];
+    float f[4];
+    sum_at(c, acc);
+    if (glu) {
+      int up[4];
+      sum_at(64 + c, up);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(silu(__fmul_rn(__fmul_rn((float)acc[e], s_ws[c + e]), sx)), __fmul_rn(__fmul_rn((float)up[e], s_ws[64 + c + e]), sx));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(__fmul_rn(__fmul_rn((float)acc[e], s_ws[c + e]), sx), s_bias[c + e]);  // (roundings as in tile_kernel)
+      if (a.epi == EPI_BIAS_GELU) {
+        gelu_erf2(f[0], f[1]);
+        gelu_erf2(f[2], f[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(f[e], resid[e]);
+    }
+    if (bad) f[0] = f[1] = f[2] = f[3] = __uint_as_float(0x7fffffffu);
     if (a.epi == EPI_F32) {
       float* o = static_cast<float*>(a.out) + (size_t)m * a.ldo + n;
       if (n + 4 <= n_out) *reinterpret_cast<float4*>(o) = make_float4(f[0], f[1], f[2], f[3]);
@@ -904,7 +943,7 @@ bool operand_map(CUtensorMap* map, const Operand& o, int K, int box_rows) {
 }
 
 template <bool I8, int BN, int CG, int EPI>
-cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, const Operand& w, int K, int sms) {
+cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, const Operand& w, int K, int sms, int* slots = nullptr) {
   using C = Cfg<I8, BN, CG, EPI>;
   static std::atomic<uint64_t> asked{0};
   cudaError_t e = ask_smem(tile_kernel<I8, BN, CG, EPI>, C::SMEM, asked);
@@ -928,7 +967,18 @@ cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, cons
   a.group_n = W + X * ceil((double)num_n / gn) < X + W * ceil((double)num_m / gm);
   a.grp = a.group_n ? gn : gm;
   a.wait_cycles = wait_limit.load(std::memory_order_relaxed);
-  const int workers = std::max(1, std::min(num_m * num_n, sms / CG));
+  int workers = std::max(1, std::min(num_m * num_n, sms / CG));
+  if constexpr (EPI == EPI_SCORES) {
+    // Each block keeps to one tile of rows where that costs no round of tiles: its sums are joined on the way, and few are left to be joined behind it
+    const int per = workers / num_m;
+    a.carry = per > 0 && (num_n + per - 1) / per <= (num_m * num_n + workers - 1) / workers;
+    if (a.carry) {
+      workers = per * num_m;
+      a.group_n = 0;
+      a.grp = num_m;
+    }
+    if (slots) *slots = (a.carry ? per : num_n) * C::EG;
+  }
   Launch l(dim3(workers * CG), C::THREADS, C::SMEM, stream, CG);
   return cudaLaunchKernelEx(&l.cfg, tile_kernel<I8, BN, CG, EPI>, mx, mw, mc, a);
 }
@@ -947,6 +997,12 @@ SplitPlan split_plan(int M, int N, int kbs, int sms) {
   return {parts, stages, std::max(stages * stage, box * kDump * 4) + 1024};
 }
 
+double split_us(int M, int N, int kbs, int sms) {
+  const SplitPlan p = split_plan(M, N, kbs, sms);
+  const long long blocks = (long long)p.parts * ((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = (M <= 64 ? 2LL : 1LL) * sms;
+  return (double)((blocks + room - 1) / room) * ((kbs + p.parts - 1) / p.parts * 0.287 + 3.0 + 8.0 / p.parts) + 4.0;
+}
+
 cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   static std::atomic<uint64_t> asked{0};
   cudaError_t e = ask_smem(split_kernel, 220 * 1024, asked);
@@ -961,10 +1017,38 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   return cudaLaunchKernelEx(&l.cfg, split_kernel, mx, mw, a);
 }
 
+// Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile, the least that a round takes (what follows the products, plain | gelu and gated
+// units) and the part that does not depend on sizes, fitted to runs (us):
+//                            256 x 256 pair  192 pair  128 pair  128 x 256  128 x 192  128 x 128  parts of K
+//   8192 x 28672 x  4096            586         652       806       660        746        896
+//   1100 x  4096 x 14336 (R)         76          63        89        52         80         68
+//    512 x  2048 x  8192             24.6        21.6      20.9      28.4       26.5       22.1
+//   5000 x  2304 x   768 (bias)      18.4        19.4      17.1      17.1       18.2       16.5
+//    777 x  8960 x  1536 (gelu)      20.2        22.0      21.2      19.3       21.2       21.5
+//    200 x  4096 x  4096             15.7        14.1      13.1      17.0       15.8       13.4
+// A row's sums are whole numbers: its bits do not depend on the choice.
+struct TileShape {
+  int bn, cg;
+  double kb, floor, deep_floor;
+};
+constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.5, 7.0}, {192, 2, 0.311, 3.6, 5.4}, {128, 2, 0.258, 2.4, 3.8}, {256, 1, 0.418, 4.2, 7.0}, {192, 1, 0.356, 3.4, 5.3}, {128, 1, 0.287, 2.4, 3.8}};
+
 template <int EPI>
 cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
-  const long long few = (long long)((g.M + TM - 1) / TM) * ((g.N + SN - 1) / SN);
-  if (g.M <= TM ? g.N <= 65535 * SN : few <= sms) return launch_split(stream, g, sms);
+  constexpr bool kGlu = EPI == EPI_SWIGLU, kDeep = kGlu || EPI == EPI_BIAS_GELU;
+  const int kbs = (g.K + KB - 1) / KB;
+  const TileShape* pick = nullptr;
+  double best = 1e30;
+  for (const TileShape& t : kShapes) {
+    if ((t.cg == 2 && sms < 2) || (kGlu && t.bn != 256)) continue;
+    const long long tiles = (long long)((g.M + TM * t.cg - 1) / (TM * t.cg)) * ((g.N + t.bn - 1) / t.bn), workers = sms / t.cg;
+    const double us = (double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor) + 4.8;
+    if (us < best) {
+      best = us;
+      pick = &t;
+    }
+  }
+  if (g.N <= 65535 * SN && (g.M <= TM || split_us(g.M, g.N, kbs, sms) < best)) return launch_split(stream, g, sms);
   TileArgs a{};
   a.xs = g.x_scales;
   a.ws = g.w_scales;
@@ -976,11 +1060,23 @@ cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   a.M = g.M;
   a.N = g.N;
   const Operand x{g.x, g.ldx, g.M}, w{g.w, g.ldw, g.N};
-  if constexpr (EPI != EPI_SWIGLU) {
-    const long long pairs = (long long)((g.M + 255) / 256) * ((g.N + 255) / 256);
-    if (pairs < sms / 2 || sms < 2) return launch_tiles<true, 128, 1, EPI>(stream, a, x, w, g.K, sms);
+  switch (pick->bn * 10 + pick->cg) {
+    case 2562: return launch_tiles<true, 256, 2, EPI>(stream, a, x, w, g.K, sms);
+    case 2561: return launch_tiles<true, 256, 1, EPI>(stream, a, x, w, g.K, sms);
+    case 1922:
+      if constexpr (!kGlu) return launch_tiles<true, 192, 2, EPI>(stream, a, x, w, g.K, sms);
+      break;
+    case 1921:
+      if constexpr (!kGlu) return launch_tiles<true, 192, 1, EPI>(stream, a, x, w, g.K, sms);
+      break;
+    case 1282:
+      if constexpr (!kGlu) return launch_tiles<true, 128, 2, EPI>(stream, a, x, w, g.K, sms);
+      break;
+    case 1281:
+      if constexpr (!kGlu) return launch_tiles<true, 128, 1, EPI>(stream, a, x, w, g.K, sms);
+      break;
   }
-  return sms < 2 ? launch_tiles<true, 256, 1, EPI>(stream, a, x, w, g.K, sms) : launch_tiles<true, 256, 2, EPI>(stream, a, x, w, g.K, sms);
+  return cudaErrorInvalidValue;
 }
 
 constexpr int kMostK = 131056;  // 127^2 K stays below 2^31 (codes of -128 that a caller may have: 128^2 K too)
@@ -1021,7 +1117,7 @@ cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& g) {
 
 namespace {
 bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
-int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 4 : (V + 255) / 256 * 4; }  // at most (a launch with one tile of rows has its blocks', bf16 half of them)
+int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 4 : (V + 255) / 256 * 4; }  // at most
 }  // namespace
 
 size_t head_scores_workspace_floats(int T, int V) { return score_sizes_ok(T, V) ? (size_t)T * (3 * (size_t)score_slots(T, V) + 1) : 0; }
@@ -1047,18 +1143,18 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   a.part = g.workspace;
   a.at = g.workspace + 3 * (size_t)score_slots(g.T, g.V) * g.T;
   a.scale = g.scale;
-  a.cap = g.softcap;
-  a.inv_cap = 1.f / g.softcap;
+  a.cap = {g.softcap, 1.f / g.softcap};
   const Operand x{g.x, g.ldx, g.T}, w{g.w, g.ldw, g.V};
   if (sms < 2) return cudaErrorInvalidConfiguration;
   cudaError_t e;
-  if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms);
-  else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms);
-  const int cg = g.T <= TM ? 1 : 2, tiles = (g.V + 128 * cg - 1) / (128 * cg), one = g.T <= TM * cg;  // (one tile of rows: a block's sums go on through its tiles)
-  const int slots = (one ? std::min(tiles, sms / cg) : tiles) * (i8 ? Cfg<true, 128, 1, EPI_SCORES>::EG : Cfg<false, 128, 1, EPI_SCORES>::EG);
+  int slots = 0;
+  if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
+  else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   if (e != cudaSuccess) return e;
-  return launch_k(join_scores_kernel, dim3((g.T + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp,
-                  g.entropy, slots, g.T, g.V);
+  // (few threads find room beside the kernel before, and wait there for its end)
+  const dim3 grid((g.T + kJoinRows - 1) / kJoinRows);
+  if (slots <= 600) return launch_k(join_scores_kernel<128>, grid, dim3(128), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
+  return launch_k(join_scores_kernel<512>, grid, dim3(512), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
 }
 
 }  // namespace hb

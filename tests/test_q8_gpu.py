@@ -243,13 +243,17 @@ def test_product_residual_in_place_and_again(L, M, N):
     assert torch.equal(a, b)
 
 
-def test_product_bits_do_not_depend_on_the_other_rows(L):
-    """A row's sums are whole numbers: alone, among few and among many it has the same bits."""
+@pytest.mark.parametrize("epi", [1, 2, 4, 5, 6])
+def test_product_bits_do_not_depend_on_the_other_rows(L, epi):
+    """A row's sums are whole numbers: alone, among few and among many it has the same bits, whichever kernel it goes through."""
     N, K = 2304, 1000
     (x, xs), (w, ws) = any_codes(3, 2600, K), any_codes(4, N, K)
-    whole = product(L, x, xs, w, ws, K, 6)[:2600]
+    bias = randn(1, N).to(BF) if epi in (1, 2, 4) else None
+    r = randn(2, 2600, N).to(BF) if epi == 4 else None
+    whole = product(L, x, xs, w, ws, K, epi, r=r, bias=bias)[:2600]
     for rows in (slice(0, 1), slice(70, 100), slice(1000, 1300), slice(2000, 2500)):
-        assert torch.equal(product(L, x[rows], xs[rows].contiguous(), w, ws, K, 6)[:-1], whole[rows])
+        part = product(L, x[rows], xs[rows].contiguous(), w, ws, K, epi, r=r[rows] if r is not None else None, bias=bias)
+        assert torch.equal(part[:-1], whole[rows])
 
 
 @pytest.mark.parametrize("M", [3, 130, 2600])
