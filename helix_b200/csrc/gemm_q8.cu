@@ -983,24 +983,23 @@ cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, cons
   return cudaLaunchKernelEx(&l.cfg, tile_kernel<I8, BN, CG, EPI>, mx, mw, mc, a);
 }
 
-// K in parts: the blocks of a cluster
+// K in parts: the blocks of a cluster.  More parts while all clusters are resident at once: with two blocks per SM (up to 64 rows of X, 108 KB) some 260 blocks, with one some 130,
+// as a cluster lies within one group of SMs (us in 4 | 5 | 6 parts, 1 x 6144 x 4096: 8.7 | 8.9 | 13.9, 300 x 1024 x 8192: 12.1 | 11.1 | 17.1), and four blocks of K are left for each.
 struct SplitPlan {
-  int parts, stages, smem;
+  int parts, stages, smem, rounds;
 };
 SplitPlan split_plan(int M, int N, int kbs, int sms) {
   const int box = std::min(TM, (M + 7) / 8 * 8);
-  const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN);
+  const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = (long long)((box <= 64 ? 2 : 1) * 0.88 * sms);
   int parts = 1;
-  while (parts < 8 && tiles * (parts + 1) <= 2LL * sms && kbs >= 4 * (parts + 1)) ++parts;
+  while (parts < 8 && tiles * (parts + 1) <= room && kbs >= 4 * (parts + 1)) ++parts;
   const int stage = box * KB + SN * KB, most = (kbs + parts - 1) / parts;
   const int stages = std::min(std::min(most, 12), (box <= 64 ? 108 : 216) * 1024 / stage);
-  return {parts, stages, std::max(stages * stage, box * kDump * 4) + 1024};
+  return {parts, stages, std::max(stages * stage, box * kDump * 4) + 1024, (int)std::min<long long>((tiles * parts + room - 1) / room, INT32_MAX)};
 }
-
-double split_us(int M, int N, int kbs, int sms) {
+double split_us(int M, int N, int kbs, int sms, double load_us) {  // (fitted as below)
   const SplitPlan p = split_plan(M, N, kbs, sms);
-  const long long blocks = (long long)p.parts * ((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = (M <= 64 ? 2LL : 1LL) * sms;
-  return (double)((blocks + room - 1) / room) * ((kbs + p.parts - 1) / p.parts * 0.287 + 3.0 + 8.0 / p.parts) + 4.0;
+  return std::max(p.rounds * ((kbs + p.parts - 1) / p.parts * 0.287 + std::min(M, TM) / 16.0 / p.parts), load_us) + 4.4 + std::min(M, TM) / 100.0;
 }
 
 cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
@@ -1025,7 +1024,10 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
 //    512 x  2048 x  8192             24.6        21.6      20.9      28.4       26.5       22.1
 //   5000 x  2304 x   768 (bias)      18.4        19.4      17.1      17.1       18.2       16.5
 //    777 x  8960 x  1536 (gelu)      20.2        22.0      21.2      19.3       21.2       21.5
-//    200 x  4096 x  4096             15.7        14.1      13.1      17.0       15.8       13.4
+//    200 x  4096 x  4096             15.7        14.1      13.1      17.0       15.8       13.4      19.3
+//    128 x  4096 x  4096                                   13.2      17.3                  13.4      10.9
+//     32 x 28672 x  4096                                   36.0      24.2                  26.2      24.0
+//    200 x   512 x 14336                                   31.2      44.9                  34.3      10.8
 // A row's sums are whole numbers: its bits do not depend on the choice.
 struct TileShape {
   int bn, cg;
@@ -1037,18 +1039,19 @@ template <int EPI>
 cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   constexpr bool kGlu = EPI == EPI_SWIGLU, kDeep = kGlu || EPI == EPI_BIAS_GELU;
   const int kbs = (g.K + KB - 1) / KB;
+  const double load_us = (double)g.N * g.K / 6.2e6 + 2.0;  // (few rows: W's way from memory)
   const TileShape* pick = nullptr;
   double best = 1e30;
   for (const TileShape& t : kShapes) {
     if ((t.cg == 2 && sms < 2) || (kGlu && t.bn != 256)) continue;
     const long long tiles = (long long)((g.M + TM * t.cg - 1) / (TM * t.cg)) * ((g.N + t.bn - 1) / t.bn), workers = sms / t.cg;
-    const double us = (double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor) + 4.8;
+    const double us = std::max((double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor), load_us) + 4.8;
     if (us < best) {
       best = us;
       pick = &t;
     }
   }
-  if (g.N <= 65535 * SN && (g.M <= TM || split_us(g.M, g.N, kbs, sms) < best)) return launch_split(stream, g, sms);
+  if (g.N <= 65535 * SN && split_us(g.M, g.N, kbs, sms, load_us) < best) return launch_split(stream, g, sms);
   TileArgs a{};
   a.xs = g.x_scales;
   a.ws = g.w_scales;
