@@ -1,6 +1,6 @@
 // Scores of given tokens from logits: log softmax of a token, its rank, the entropy of the row and the first tokens of the order (logit descending, id ascending).
 //
-// One pass over a row, read once: every thread keeps the running maximum m of its entries, S = sum e^(x - m) and U = sum (x - m) e^(x - m), so that at the end
+// One pass over a row, read once: every thread keeps an m near the maximum of its entries, S = sum e^(x - m) and U = sum (x - m) e^(x - m), so that at the end
 //   log softmax(x_t) = x_t - m - log S,   entropy = log S - U / S.
 // A thread also remembers the step in which it met its maximum, and the largest of its other steps' maxima.  The n-th best of the threads' maxima bounds what may be among
 // the row's first n: n threads have such entries, and list those of that step; the few whose other steps reach the bound too are looked through once more (from L2).  Places in the
@@ -55,32 +55,19 @@ __device__ __forceinline__ float at_least(float a, float b) {  // 1 or 0
 struct Sums {
   float m, s, u;
 };
-// S and U of two parts brought to the larger maximum
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m);
-  Sums r{m, 0.f, 0.f};
-  auto add = [&](const Sums& p) {
-    const float d = p.m == m ? 0.f : p.m - m;
-    const float w = d < -200.f ? 0.f : exp2_fast(d * kLog2e);  // (nothing is left of it below e^-200: and no infinity times 0)
-    if (w > 0.f || p.s != p.s) {
-      r.s = fmaf(w, p.s, r.s);
-      r.u += w * fmaf(d < -200.f ? 0.f : d, p.s, p.u);
-    }
-  };
-  add(a);
-  add(b);
-  if (a.s != a.s || b.s != b.s) r.s = __uint_as_float(0x7fffffffu);
-  return r;
-}
-
-__device__ __forceinline__ Sums join_lanes(Sums my, int lanes) {  // of the first `lanes` lanes (a power of two), known to all of these afterwards
+// The sums of the first `lanes` lanes (a power of two) brought to the largest m and added, known to all of these afterwards
+__device__ __forceinline__ Sums join_lanes(const Sums& my, int lanes) {
+  const float m = value_of(__reduce_max_sync(0xffffffffu, ordered(my.m)));
+  const float d = my.m == m ? 0.f : my.m - m;  // (no infinity less itself)
+  const float w = exp2_fast(d * kLog2e);
+  Sums r{m, w * my.s, w > 0.f ? w * fmaf(d, my.s, my.u) : 0.f};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     if (o < lanes) {
-      const Sums other{__shfl_xor_sync(0xffffffffu, my.m, o), __shfl_xor_sync(0xffffffffu, my.s, o), __shfl_xor_sync(0xffffffffu, my.u, o)};
-      my = threadIdx.x & o ? join(other, my) : join(my, other);
+      r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+      r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
     }
-  return my;
+  return r;
 }
 
 struct Shared {
@@ -88,7 +75,7 @@ struct Shared {
   u64 best[kThreads];  // the threads' earliest places; a block's first tokens
   u64 bound;
   int step[kThreads];  // with a thread's maximum
-  int candidate[kMost], candidates;
+  int candidate[kMost], candidates, ahead[kMost];
   Sums warp_sums[kWarps];
   int warp_before[kWarps];
   Sums sums;
@@ -176,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenSc
 
   Sums my{-INFINITY, 0.f, 0.f};
   int first_at = mine;  // the step with the thread's maximum
-  float second = -INFINITY;  // the largest of its other steps
+  float best = -INFINITY, second = -INFINITY;  // that, and the largest of its other steps
   uint64_t before2 = f2_pack(0.f, 0.f);  // (whole numbers below 2^24)
   int equals = 0;
   auto values_of = [&](const uint4& u, const uint4& v, float(&f)[E]) {
@@ -213,17 +200,16 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenSc
 #pragma unroll
     for (int e = 1; e + 1 < E; e += 2) top = max3(top, f[e], f[e + 1]);
     top = fmaxf(top, f[E - 1]);
-    if (top > my.m) {
+    second = fmaxf(second, fminf(best, top));
+    first_at = top > best ? i : first_at;
+    best = fmaxf(best, top);
+    if (best - my.m > 8.f) {  // (m need not be the maximum: it follows when it is left far behind)
       if (my.m > -INFINITY) {
-        const float d = my.m - top, w = exp2_fast(d * kLog2e);
+        const float d = my.m - best, w = exp2_fast(d * kLog2e);
         my.u = w > 0.f ? w * fmaf(d, my.s, my.u) : 0.f;
         my.s *= w;
       }
-      second = my.m;
-      my.m = top;
-      first_at = i;
-    } else {
-      second = fmaxf(second, top);
+      my.m = best;
     }
     const float m = my.m > -INFINITY ? my.m : 0.f;
     const uint64_t off = f2_pack(-m, -m), log2e = f2_pack(kLog2e, kLog2e);
@@ -265,73 +251,78 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenSc
     int i = first_at;
     for (; i < end; i += kStep) {  // (where its maximum is -inf, the first that is no NaN may lie further on)
       entries_at(i, f);
+      int at = E;
 #pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (id_of(i, e) < end && f[e] == my.m) first = place_of(f[e], id_of(i, e));
-      if (first) break;
+      for (int e = E - 1; e >= 0; --e) at = f[e] == best ? e : at;
+      if (at < E && id_of(i, at) < end) {
+        first = place_of(best, id_of(i, at));
+        break;
+      }
     }
     sh.best[tid] = first;
     if (tid == 0) sh.candidates = 0;
     __syncthreads();
-    if (warp == 0) {  // the n-th of them, bit by bit: of the values, and where these tie of the ids
-      u64 theirs[kThreads / 32];
-      uint32_t high = 0, low = ~0u;
+    if (warp == 0) {  // the n-th of them by value, two bits at a time
+      uint32_t theirs[kThreads / 32], high = 0, low = ~0u;
       int live = 0;
 #pragma unroll
       for (int k = 0; k < kThreads / 32; ++k) {
-        theirs[k] = sh.best[k * 32 + lane];
-        high = max(high, (uint32_t)(theirs[k] >> 32));
-        low = min(low, (uint32_t)(theirs[k] >> 32));
+        theirs[k] = (uint32_t)(sh.best[k * 32 + lane] >> 32);
+        high = max(high, theirs[k]);
+        low = min(low, theirs[k]);
         live += theirs[k] != 0;
       }
-      u64 at = 0;
+      u64 bound = 0;
       if (__reduce_add_sync(0xffffffffu, live) > n) {
         high = __reduce_max_sync(0xffffffffu, high);
         low = __reduce_min_sync(0xffffffffu, low);
-        int bit = high == low ? -1 : 31 - __clz(high ^ low);
-        uint32_t key = bit < 0 ? high : bit == 31 ? 0 : high & ~((2u << bit) - 1);
-        int c = 0;
-        for (; bit >= 0; --bit) {
-          const uint32_t trial = key | 1u << bit;
-          int above = 0;
+        int bit = high == low ? -2 : (31 - __clz(high ^ low)) & ~1;  // (of the upper one of a pair's two)
+        uint32_t key = bit < 0 ? high : bit == 30 ? 0 : high & ~((4u << bit) - 1);
+        int c = kThreads;
+        for (; bit >= 0 && c != n; bit -= 2) {
+          uint32_t counts = 0;  // of those at or above key + 1, 2, 3 units of the pair, ten bits each
 #pragma unroll
-          for (int k = 0; k < kThreads / 32; ++k) above += (uint32_t)(theirs[k] >> 32) >= trial;
-          above = __reduce_add_sync(0xffffffffu, above);
-          if (above >= n) {
-            key = trial;
-            c = above;
-            if (c == n) break;
+          for (int k = 0; k < kThreads / 32; ++k)
+            counts += (theirs[k] >= key + (1u << bit) ? 1u : 0u) + (theirs[k] >= key + (2u << bit) ? 1u << 10 : 0u) + (theirs[k] >= key + (3u << bit) ? 1u << 20 : 0u);
+          counts = __reduce_add_sync(0xffffffffu, counts);
+          const int units = (counts & 1023) >= (uint32_t)n ? (counts >> 10 & 1023) >= (uint32_t)n ? (counts >> 20) >= (uint32_t)n ? 3 : 2 : 1 : 0;
+          if (units) {
+            key += (uint32_t)units << bit;
+            c = counts >> (10 * (units - 1)) & 1023;
           }
         }
-        at = (u64)key << 32;
-        if (c != n)
+        u64 at = (u64)key << 32;
+        if (c > kMost) {  // more tie than may list theirs: the n-th by its id too
           for (bit = 31; bit >= 0; --bit) {
             const u64 trial = at | 1ull << bit;
             int above = 0;
-#pragma unroll
-            for (int k = 0; k < kThreads / 32; ++k) above += theirs[k] >= trial;
+            for (int k = 0; k < kThreads / 32; ++k) above += sh.best[k * 32 + lane] >= trial;
             above = __reduce_add_sync(0xffffffffu, above);
             if (above >= n) {
               at = trial;
               if (above == n) break;
             }
           }
+        }
+        bound = at - 1;
       }
-      if (lane == 0) sh.bound = at ? at - 1 : 0;
+      if (lane == 0) sh.bound = bound;
     }
     __syncthreads();
     u64 bound = sh.bound;  // what is listed lies above it
+    const float line = value_of((uint32_t)((bound + 1) >> 32));  // (what is no less may lie above the bound; a NaN for none: so all do)
     auto list = [&](const float(&f)[E], int i) {  // those of a thread's entries of a step
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const u64 place = id_of(i, e) < end ? place_of(f[e], id_of(i, e)) : 0ull;
-        if (place > bound) {
-          const int to = atomicAdd(&sh.count, 1);
-          if (to < kList) sh.list[to] = place;
+      for (int e = 0; e < E; ++e)
+        if (!(f[e] < line) && id_of(i, e) < end) {
+          const u64 place = place_of(f[e], id_of(i, e));
+          if (place > bound) {
+            const int to = atomicAdd(&sh.count, 1);
+            if (to < kList) sh.list[to] = place;
+          }
         }
-      }
     };
-    if (first > bound) {  // (n threads at most)
+    if (first > bound) {  // (kMost threads at most)
       list(f, i);
       if (ordered(second) >= (uint32_t)(bound >> 32)) sh.candidate[atomicAdd(&sh.candidates, 1)] = tid;
     }
@@ -392,37 +383,48 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenSc
   if constexpr (NC > 1) {
     __syncthreads();
     cluster_sync_all();
-    if (part == 0) {
-      all = join_lanes(*cluster_ptr<NC>(&sh.sums, lane % NC), NC);
-      n_before = __reduce_add_sync(0xffffffffu, lane < NC ? *cluster_ptr<NC>(&sh.before, lane % NC) : 0);
-      if constexpr (TOP) {
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        for (int k = tid; k < NC * kMost; k += kThreads) {  // (places enough for all)
-          const u64 p = k % kMost < a.n_top ? *cluster_ptr<NC>(&sh.best[k % kMost], k / kMost) : 0ull;
-          if (p) sh.list[atomicAdd(&sh.count, 1)] = p;
-        }
-        __syncthreads();
-      }
-    }
-    __syncwarp();
-    cluster_sync_all();  // the others may leave
-    if (part != 0) return;
-    if constexpr (TOP) thin_out(sh, a.n_top);
+    all = join_lanes(*cluster_ptr<NC>(&sh.sums, lane % NC), NC);
+    n_before = __reduce_add_sync(0xffffffffu, lane < NC ? *cluster_ptr<NC>(&sh.before, lane % NC) : 0);
   }
   const bool none = all.s == 0.f;  // nothing but -inf
   const float log_s = logf(all.s), lse = none ? INFINITY : all.m + log_s;
-  if (tid == 0) {
+  if (part == 0 && tid == 0) {
     if (a.lp) a.lp[t] = has ? xt - lse : -INFINITY;
     if (a.rank) a.rank[t] = has && xt == xt ? n_before : -1;
     if (a.entropy) a.entropy[t] = none ? 0.f : log_s - all.u / all.s;
   }
   if constexpr (TOP) {
-    for (int j = tid; j < a.n_top; j += kThreads) {
-      const u64 p = j < sh.count ? sh.list[j] : 0ull;
-      a.top_ids[(size_t)t * a.n_top + j] = p ? (int)~(uint32_t)p : -1;
-      if (a.top_lp) a.top_lp[(size_t)t * a.n_top + j] = p ? value_of((uint32_t)(p >> 32)) - lse : __uint_as_float(0x7fffffffu);
+    const int n = a.n_top;
+    auto write = [&](int to, u64 place) {
+      a.top_ids[(size_t)t * n + to] = place ? (int)~(uint32_t)place : -1;
+      if (a.top_lp) a.top_lp[(size_t)t * n + to] = place ? value_of((uint32_t)(place >> 32)) - lse : __uint_as_float(0x7fffffffu);
+    };
+    if constexpr (NC == 1) {
+      for (int j = tid; j < n; j += kThreads) write(j, j < sh.count ? sh.list[j] : 0ull);
+    } else {
+      // every block sees all blocks' first tokens, and writes its own to where they stand among these
+      for (int k = tid; k < NC * kMost; k += kThreads) sh.list[k] = k % kMost < n ? *cluster_ptr<NC>(&sh.best[k % kMost], k / kMost) : 0ull;
+      if (tid < kMost) sh.ahead[tid] = 0;
+      int live = 0;
+      for (int k = 0; k < NC * kMost; k += kThreads) live += __syncthreads_count(k + tid < NC * kMost && sh.list[min(k + tid, NC * kMost - 1)] != 0);
+      for (int k = tid; k < n * NC; k += kThreads) {
+        const u64 place = sh.best[k / NC];
+        const u64* other = sh.list + k % NC * kMost;
+        int ahead = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) ahead += other[j] > place;
+        if (ahead) atomicAdd(&sh.ahead[k / NC], ahead);
+      }
+      __syncthreads();
+      if (tid < n) {
+        if (sh.best[tid] && sh.ahead[tid] < n) write(sh.ahead[tid], sh.best[tid]);
+        if (part == 0 && tid >= live) write(tid, 0ull);
+      }
     }
+  }
+  if constexpr (NC > 1) {
+    __syncwarp();
+    cluster_sync_all();  // others may still read this block's
   }
 }
 
@@ -450,9 +452,9 @@ cudaError_t launch_nc(cudaStream_t stream, const TokenScoresArgs& a) {
 }
 template <bool F32, bool TOP>
 cudaError_t launch_top(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
-  // blocks per row: twice as many while not all SMs have their four and a block keeps some steps
+  // blocks per row: twice as many while not all SMs have one and a block keeps some steps (32 rows of 128256 in fp32: four blocks 15.7 us, eight 17.4)
   int nc = 1;
-  while (nc < 8 && (long long)a.T * nc * 2 <= 4LL * sms && a.V >= nc * 2 * kThreads * kEntries<F32>) nc *= 2;
+  while (nc < 8 && (long long)a.T * nc * 2 <= sms && a.V >= nc * 2 * kThreads * kEntries<F32>) nc *= 2;
   switch (nc) {
     case 1: return launch_nc<F32, 1, TOP>(stream, a);
     case 2: return launch_nc<F32, 2, TOP>(stream, a);
