@@ -429,14 +429,17 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_kernel(const TokenSc
 }
 
 template <bool F32, int NC, bool TOP>
-cudaError_t launch_nc(cudaStream_t stream, const TokenScoresArgs& a) {
+cudaError_t launch_nc(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.T * NC);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (pdl_enabled()) {
+  // Blocks that start beside the last ones of a kernel before take what room there is, and lie unevenly: worth it only where all have room, or many rounds follow
+  // (300 rows of 128256 in fp32 45.8 us that way, 37.3 without; 400 in bf16 41.3, 34.8)
+  const long long blocks = (long long)a.T * NC;
+  if (pdl_enabled() && (blocks <= 2 * sms || blocks > 8 * sms)) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
@@ -462,10 +465,10 @@ cudaError_t launch_top(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
   };
   while (nc < 8 && more(nc * 2)) nc *= 2;
   switch (nc) {
-    case 1: return launch_nc<F32, 1, TOP>(stream, a);
-    case 2: return launch_nc<F32, 2, TOP>(stream, a);
-    case 4: return launch_nc<F32, 4, TOP>(stream, a);
-    default: return launch_nc<F32, 8, TOP>(stream, a);
+    case 1: return launch_nc<F32, 1, TOP>(stream, a, sms);
+    case 2: return launch_nc<F32, 2, TOP>(stream, a, sms);
+    case 4: return launch_nc<F32, 4, TOP>(stream, a, sms);
+    default: return launch_nc<F32, 8, TOP>(stream, a, sms);
   }
 }
 
