@@ -7,7 +7,9 @@
 // tiles' so that one tile's epilogue lies behind the next one's products.
 //   Scores: thread = row, so that a row's running maximum m, S = sum e^(z - m) and U = sum (z - m) e^(z - m) need no other thread; a tile leaves three numbers per row and 128 (64)
 //   columns instead of its logits, and join_scores_kernel puts them together: lp = z_t - m - log S, entropy = log S - U / S.
-// split_kernel: few tiles.  The blocks of a cluster share K and add their whole numbers through distributed shared memory; a block's X has only as many rows as there are.
+//   few_scores_kernel: up to 64 rows, W's rows the 128 of a product and X's its columns, so that none of the products is for nothing; a lane has a column of logits.
+// split_kernel: few tiles.  The blocks of a cluster share K and add their whole numbers through distributed shared memory.  W's rows are the 128 of a product there and X's its
+//   columns, as many as there are: products of rows that nobody wants would take power, and with it clock.
 //
 // Waits are bounded (q8_wait_cycles): one that runs out ends the kernel with NaN in place of what it was for, and q8_status says so.
 #include <math.h>
@@ -256,6 +258,13 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       tmem_relinquish();
     }
     pdl_launch_dependents();  // (launch.h)
+  }
+  if constexpr (CG == 1) {
+    // rows of X that are not loaded are zeros: their products take less of the power that the card's clock goes by (32 rows of a bf16 head, run for seconds: 202 -> 191 us)
+    const int fill = (TM - a.box_rows) * (KB / 16);
+    for (int i = threadIdx.x; i < STAGES * fill; i += C::THREADS)
+      *reinterpret_cast<uint4*>(smem_x + i / fill * C::X_BYTES + a.box_rows * KB + i % fill * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   if constexpr (CG == 2) cluster_sync_all(); else __syncthreads();
@@ -700,7 +709,7 @@ struct SplitArgs {
   const bf16 *bias, *r;
   void* out;
   int ldo, ldr, M, N, kbs, epi;
-  int box_rows, stages;
+  int box_rows, columns, stages;  // rows of X that are loaded (a multiple of 16), columns of tensor memory for them
   long long wait_cycles;
 };
 
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   __shared__ float s_xs[TM], s_ws[SN], s_bias[SN];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
   const int x_bytes = a.box_rows * KB, stages = a.stages;
-  uint8_t* smem_w = smem + stages * x_bytes;  // (products read 128 rows of X whatever was loaded: what lies behind goes into rows that nobody reads)
+  uint8_t* smem_w = smem + stages * x_bytes;
   int* dump = reinterpret_cast<int*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int parts = gridDim.x, part = blockIdx.x;
@@ -733,7 +742,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_at, SN);
+    tmem_alloc(&tmem_at, a.columns);
     tmem_relinquish();
     pdl_launch_dependents();  // (launch.h)
   }
@@ -762,7 +771,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
     }
   } else if (warp == 1) {
     const bool elected = elect_one_sync();
-    constexpr uint32_t idesc = umma_idesc_i8(TM, SN);
+    const uint32_t idesc = umma_idesc_i8(SN, a.box_rows);
     int s = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
@@ -771,7 +780,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
       const uint32_t xa = smem_u32(smem + s * x_bytes), wa = smem_u32(smem_w + s * SN * KB);
       if (elected) {
 #pragma unroll
-        for (int k = 0; k < KB; k += 32) umma_i8_ss(tmem, umma_desc_kmajor_sw128(xa + k), umma_desc_kmajor_sw128(wa + k), idesc, kb > kb0 || k != 0);
+        for (int k = 0; k < KB; k += 32) umma_i8_ss(tmem, umma_desc_kmajor_sw128(wa + k), umma_desc_kmajor_sw128(xa + k), idesc, kb > kb0 || k != 0);
         umma_commit(&empty[s]);
       }
       if (++s == stages) { s = 0; phase ^= 1; }
@@ -787,18 +796,15 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
       else s_bias[j] = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
     }
     ok = wait_turn(&sums_full, 0, a.wait_cycles);
-    const int q = warp & 3, row = q * 32 + lane, c0 = warp < 6 ? 0 : SN / 2;
-    if (ok && q * 32 < a.box_rows) {  // (all operands have been read: their room takes the sums)
+    const int q = warp & 3;
+    if (ok) {  // (all operands have been read: their room takes the sums, a row of X after the other)
       tc_fence_after();
-#pragma unroll
-      for (int c = c0; c < c0 + SN / 2; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
+      for (int c = warp < 6 ? 0 : 16; c < a.box_rows; c += 32) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
         tmem_ld_wait();
-        if (row < a.box_rows) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(dump + row * kDump + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
+        for (int j = 0; j < 16; ++j) dump[(c + j) * kDump + q * 32 + lane] = (int)v[j];
       }
     }
   }
@@ -885,7 +891,231 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, SN);
+    tmem_dealloc(tmem, a.columns);
+  }
+}
+
+// ------------------------------------------------------------------ scores of few rows
+constexpr int kFewRows = 64, kFewThreads = 64 + 4 * 128, kFewSmem = 200 * 1024;  // (the kernel that joins the sums finds room beside it)
+
+struct FewArgs {
+  const float *xs, *ws;
+  int T, V, kbs;
+  int box_rows, columns, stages;  // as in SplitArgs; the columns hold two tiles' sums
+  const int32_t* targets;
+  float *part, *at;
+  float scale;
+  Cap cap;
+  long long wait_cycles;
+};
+
+template <bool I8>
+__global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[12], empty[12], sums_full[2], sums_empty[2], all_done;
+  __shared__ uint32_t tmem_at;
+  __shared__ __align__(16) float s_xs[kFewRows];
+  __shared__ __align__(16) int s_targets[kFewRows];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);
+  const int x_bytes = a.box_rows * KB, stages = a.stages;
+  uint8_t* smem_w = smem + stages * x_bytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = (a.V + SN - 1) / SN, groups = a.box_rows / 16;  // sixteen rows of X for each group of four warps
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_w);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sums_full[i], 1);
+      mbar_init(&sums_empty[i], 4 * groups);
+    }
+    mbar_init(&all_done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_at, a.columns);
+    tmem_relinquish();
+    pdl_launch_dependents();  // (launch.h)
+  }
+  pdl_wait();
+  if (threadIdx.x < kFewRows) {
+    const int t = threadIdx.x;
+    s_xs[t] = t < a.T ? (I8 ? __ldg(a.xs + t) : 1.f) * a.scale : 0.f;
+    s_targets[t] = t < a.T && a.targets ? __ldg(a.targets + t) : -1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0);
+
+  bool ok = true;
+  int issued = 0;
+  if (warp == 0) {
+    const bool elected = elect_one_sync();
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+      for (int kb = 0; kb < a.kbs; ++kb) {
+        if (!(ok = wait_turn(&empty[s], phase ^ 1, a.wait_cycles))) break;
+        if (elected) {
+          mbar_arrive_expect_tx(&full[s], x_bytes + SN * KB);
+          tma_load_2d(smem_w + s * SN * KB, &map_w, &full[s], k_at<I8>(kb), t * SN);
+          tma_load_2d(smem + s * x_bytes, &map_x, &full[s], k_at<I8>(kb), 0);
+        }
+        ++issued;
+        if (++s == stages) { s = 0; phase ^= 1; }
+      }
+  } else if (warp == 1) {
+    const bool elected = elect_one_sync();
+    const uint32_t idesc = I8 ? umma_idesc_i8(SN, a.box_rows) : umma_idesc_bf16(SN, a.box_rows);
+    int s = 0, it = 0;
+    uint32_t phase = 0, d = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+      for (int kb = 0; kb < a.kbs; ++kb) {
+        const bool first = I8 ? kb == 0 : kb % kPiece == 0;
+        if (first) {
+          if (!(ok = wait_turn(&sums_empty[it & 1], ((it >> 1) & 1) ^ 1, a.wait_cycles))) break;
+          tc_fence_after();
+          d = tmem + (it & 1) * a.box_rows;
+        }
+        if (!(ok = wait_turn(&full[s], phase, a.wait_cycles))) break;
+        tc_fence_after();
+        const uint32_t xa = smem_u32(smem + s * x_bytes), wa = smem_u32(smem_w + s * SN * KB);
+        if (elected) {
+#pragma unroll
+          for (int k = 0; k < KB; k += 32) {
+            const uint64_t dw = umma_desc_kmajor_sw128(wa + k), dx = umma_desc_kmajor_sw128(xa + k);
+            if constexpr (I8) umma_i8_ss(d, dw, dx, idesc, !first || k != 0);
+            else umma_f16_ss(d, dw, dx, idesc, !first || k != 0);
+          }
+          umma_commit(&empty[s]);
+        }
+        if (++s == stages) { s = 0; phase ^= 1; }
+        if (kb + 1 == a.kbs || (!I8 && kb % kPiece == kPiece - 1)) {
+          if (elected) umma_commit(&sums_full[it & 1]);
+          ++it;
+        }
+      }
+    __syncwarp();
+  } else if ((warp - 2) >> 2 < groups) {
+    // a lane has a column of logits, its sixteen rows' sums go on through the block's tiles
+    const int q = warp & 3, r0 = ((warp - 2) >> 2) * 16;
+    float m[16], S[16], U[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      m[j] = -INFINITY;
+      S[j] = U[j] = 0.f;
+    }
+    int it = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int n = t * SN + q * 32 + lane;
+      float z[16];
+      auto take = [&] {  // the next sums of this warp's lanes
+        ok = wait_turn(&sums_full[it & 1], (it >> 1) & 1, a.wait_cycles);
+        if (!ok) return;
+        tc_fence_after();
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + (it & 1) * a.box_rows + r0, v);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sums_empty[it & 1]);
+        ++it;
+        const float w = I8 && n < a.V ? __ldg(a.ws + n) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if constexpr (I8) z[j] = __fmul_rn((float)(int)v[j], w);
+          else z[j] += __uint_as_float(v[j]);
+        }
+      };
+      if constexpr (I8) {
+        take();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) z[j] = 0.f;
+        for (int k0 = 0; k0 < a.kbs && ok; k0 += kPiece) take();
+      }
+      if (!ok || n >= a.V) continue;
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(s_xs + r0 + j);
+        z[j] = __fmul_rn(z[j], x.x);
+        z[j + 1] = __fmul_rn(z[j + 1], x.y);
+        z[j + 2] = __fmul_rn(z[j + 2], x.z);
+        z[j + 3] = __fmul_rn(z[j + 3], x.w);
+      }
+      if (a.cap.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) cap2(a.cap, z[j], z[j + 1]);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (s_targets[r0 + j] == n) a.at[r0 + j] = z[j];
+        if (z[j] - m[j] > 8.f) {  // (m need not be the maximum: it follows when it is left far behind)
+          if (m[j] > -INFINITY) {
+            const float d = m[j] - z[j], w = exp2_fast(d * kLog2e);
+            U[j] = w > 0.f ? w * fmaf(d, S[j], U[j]) : 0.f;
+            S[j] *= w;
+          }
+          m[j] = z[j];
+        }
+        const float d = z[j] - (m[j] > -INFINITY ? m[j] : 0.f), w = exp2_fast(d * kLog2e);
+        S[j] += w;
+        U[j] = fmaf(w, d, U[j]);
+      }
+    }
+    // the lanes' sums: each row's brought to one m, then half of the rows to each half of the lanes, and so on
+    const int j0 = lane >> 1;  // the row that this lane ends up with
+    float mine = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t u = __float_as_uint(m[j]);
+      const uint32_t key = __reduce_max_sync(0xffffffffu, u & 0x80000000u ? ~u : u | 0x80000000u);
+      const float top = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+      const float d = m[j] == top ? 0.f : m[j] - top, w = exp2_fast(d * kLog2e);  // (no infinity less itself)
+      U[j] = w > 0.f ? w * fmaf(d, S[j], U[j]) : 0.f;
+      S[j] *= w;
+      mine = j == j0 ? top : mine;
+    }
+#pragma unroll
+    for (int half = 8; half > 0; half >>= 1) {
+      const bool upper = lane & 2 * half;
+#pragma unroll
+      for (int j = 0; j < half; ++j) {
+        const float s = upper ? S[j] : S[j + half], u = upper ? U[j] : U[j + half];
+        S[j] = (upper ? S[j + half] : S[j]) + __shfl_xor_sync(0xffffffffu, s, 2 * half);
+        U[j] = (upper ? U[j + half] : U[j]) + __shfl_xor_sync(0xffffffffu, u, 2 * half);
+      }
+    }
+    S[0] += __shfl_xor_sync(0xffffffffu, S[0], 1);
+    U[0] += __shfl_xor_sync(0xffffffffu, U[0], 1);
+    if (!(lane & 1) && r0 + j0 < a.T) {
+      float* p = a.part + (size_t)(blockIdx.x * 4 + q) * 3 * a.T + r0 + j0;
+      p[0] = mine;
+      p[a.T] = S[0];
+      p[2 * a.T] = U[0];
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  if (__syncthreads_or(!ok)) {
+    if (warp == 0)
+      for (int i = max(0, issued - stages); i < issued; ++i) wait_turn(&full[i % stages], (i / stages) & 1, HB_WAIT_TIMEOUT_CYCLES);
+    if (warp == 1) {
+      if (elect_one_sync()) umma_commit(&all_done);
+      __syncwarp();
+      wait_turn(&all_done, 0, HB_WAIT_TIMEOUT_CYCLES);
+    }
+    for (int i = threadIdx.x; i < 4 * a.T; i += kFewThreads) a.part[(size_t)(blockIdx.x * 4 + i / a.T) * 3 * a.T + a.T + i % a.T] = __uint_as_float(0x7fffffffu);
+    if (threadIdx.x == 0) wait_ran_out = 1;
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, a.columns);
   }
 }
 
@@ -983,13 +1213,29 @@ cudaError_t launch_tiles(cudaStream_t stream, TileArgs a, const Operand& x, cons
   return cudaLaunchKernelEx(&l.cfg, tile_kernel<I8, BN, CG, EPI>, mx, mw, mc, a);
 }
 
+template <bool I8>
+cudaError_t launch_few(cudaStream_t stream, const HeadScoresArgs& g, const TileArgs& t, int sms, int* slots) {
+  static std::atomic<uint64_t> asked{0};
+  cudaError_t e = ask_smem(few_scores_kernel<I8>, kFewSmem, asked);
+  if (e != cudaSuccess) return e;
+  const int box = (g.T + 15) / 16 * 16, stage = (box + SN) * KB, stages = std::min(12, (kFewSmem - 1024) / stage);
+  CUtensorMap mx, mw;
+  if (!operand_map<I8>(&mx, {g.x, g.ldx, g.T}, g.H, box) || !operand_map<I8>(&mw, {g.w, g.ldw, g.V}, g.H, SN)) return cudaErrorInvalidValue;
+  const FewArgs a{g.x_scales, g.w_scales, g.T, g.V, ((I8 ? g.H : 2 * g.H) + KB - 1) / KB, box, 2 * box <= 32 ? 32 : 2 * box <= 64 ? 64 : 128, stages, t.targets, t.part, t.at, t.scale, t.cap,
+                  wait_limit.load(std::memory_order_relaxed)};
+  const int workers = std::min((g.V + SN - 1) / SN, sms);
+  *slots = workers * 4;
+  Launch l(dim3(workers), kFewThreads, stages * stage + 1024, stream, 1);
+  return cudaLaunchKernelEx(&l.cfg, few_scores_kernel<I8>, mx, mw, a);
+}
+
 // K in parts: the blocks of a cluster.  More parts while all clusters are resident at once: with two blocks per SM (up to 64 rows of X, 108 KB) some 260 blocks, with one some 130,
 // as a cluster lies within one group of SMs (us in 4 | 5 | 6 parts, 1 x 6144 x 4096: 8.7 | 8.9 | 13.9, 300 x 1024 x 8192: 12.1 | 11.1 | 17.1), and four blocks of K are left for each.
 struct SplitPlan {
   int parts, stages, smem, rounds;
 };
 SplitPlan split_plan(int M, int N, int kbs, int sms) {
-  const int box = std::min(TM, (M + 7) / 8 * 8);
+  const int box = std::min(TM, (M + 15) / 16 * 16);
   const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = (long long)((box <= 64 ? 2 : 1) * 0.88 * sms);
   int parts = 1;
   while (parts < 8 && tiles * (parts + 1) <= room && kbs >= 4 * (parts + 1)) ++parts;
@@ -1006,11 +1252,11 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   static std::atomic<uint64_t> asked{0};
   cudaError_t e = ask_smem(split_kernel, 220 * 1024, asked);
   if (e != cudaSuccess) return e;
-  const int kbs = (g.K + KB - 1) / KB, box = std::min(TM, (g.M + 7) / 8 * 8);
+  const int kbs = (g.K + KB - 1) / KB, box = std::min(TM, (g.M + 15) / 16 * 16);
   const SplitPlan p = split_plan(g.M, g.N, kbs, sms);
   CUtensorMap mx, mw;
   if (!operand_map<true>(&mx, {g.x, g.ldx, g.M}, g.K, box) || !operand_map<true>(&mw, {g.w, g.ldw, g.N}, g.K, 64)) return cudaErrorInvalidValue;
-  const SplitArgs a{g.x_scales, g.w_scales, has_bias(g.epi) ? g.bias : nullptr, has_resid(g.epi) ? g.r : nullptr, g.out, g.ldo, g.ldr, g.M, g.N, kbs, (int)g.epi, box, p.stages,
+  const SplitArgs a{g.x_scales, g.w_scales, has_bias(g.epi) ? g.bias : nullptr, has_resid(g.epi) ? g.r : nullptr, g.out, g.ldo, g.ldr, g.M, g.N, kbs, (int)g.epi, box, box <= 32 ? 32 : box <= 64 ? 64 : 128, p.stages,
                     wait_limit.load(std::memory_order_relaxed)};
   Launch l(dim3(p.parts, (g.N + SN - 1) / SN, (g.M + TM - 1) / TM), kSplitThreads, p.smem, stream, p.parts);
   return cudaLaunchKernelEx(&l.cfg, split_kernel, mx, mw, a);
@@ -1151,7 +1397,8 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   if (sms < 2) return cudaErrorInvalidConfiguration;
   cudaError_t e;
   int slots = 0;
-  if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
+  if (g.T <= kFewRows) e = i8 ? launch_few<true>(stream, g, a, sms, &slots) : launch_few<false>(stream, g, a, sms, &slots);
+  else if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   if (e != cudaSuccess) return e;
   // (few threads find room beside the kernel before, and wait there for its end)
