@@ -3,10 +3,10 @@
 // The sums are whole numbers of 32 bits on the tensor cores (tcgen05 kind::i8): exact in any order, so parts of K add up to the same bits however they are cut.  Both operands
 // lie in rows along K and come as blocks of 128 bytes of 128 or 256 rows, TMA's 128-byte swizzle: 128 codes, or 64 entries of bf16 where the head's scores take those.
 //
-// tile_kernel: persistent, one block (or a pair of blocks, cta_group::2) per SM; warp 0 loads, warp 1 multiplies, eight warps take the sums from tensor memory, which holds two
-// tiles' so that one tile's epilogue lies behind the next one's products.
-//   Scores: thread = row, so that a row's running maximum m, S = sum e^(z - m) and U = sum (z - m) e^(z - m) need no other thread; a tile leaves three numbers per row and 128 (64)
-//   columns instead of its logits, and join_scores_kernel puts them together: lp = z_t - m - log S, entropy = log S - U / S.
+// tile_kernel: persistent, one block (or a pair of blocks, cta_group::2) per SM; warp 0 loads, warp 1 multiplies, sixteen warps (eight for bf16) take the sums from tensor memory,
+// which holds two tiles' so that one tile's epilogue lies behind the next one's products.
+//   Scores: thread = row, so that a row's running maximum m, S = sum e^(z - m) and U = sum (z - m) e^(z - m) need no other thread; tiles leave three numbers per row
+//   and group of columns instead of its logits, and join_scores_kernel puts them together: lp = z_t - m - log S, entropy = log S - U / S.
 //   few_scores_kernel: up to 64 rows, W's rows the 128 of a product and X's its columns, so that none of the products is for nothing; a lane has a column of logits.
 // split_kernel: few tiles.  The blocks of a cluster share K and add their whole numbers through distributed shared memory.  W's rows are the 128 of a product there and X's its
 //   columns, as many as there are: products of rows that nobody wants would take power, and with it clock.
@@ -62,6 +62,7 @@ __device__ __forceinline__ bool all_of(uint32_t id, uint32_t nthreads, bool mine
 __device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -95,7 +96,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 struct Cap {
-  float cap, inv;  // 0: none
+  float cap, inv;  // cap 0: none
 };
 // cap tanh(x / cap) for two values: 1 - 2 / (e^2y + 1), and where that cancels (|y| < 1/4) the series, whose next term is 2^-26 of it
 __device__ __forceinline__ void cap2(const Cap& c, float& x0, float& x1) {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void cap2(const Cap& c, float& x0, float& x1) {
   float a0, a1, u0, u1, s0, s1;
   f2_unpack(f2_mul(y, c2(2.f * kLog2e)), a0, a1);
   f2_unpack(f2_add(f2_pack(exp2_fast(a0), exp2_fast(a1)), c2(1.f)), a0, a1);
-  f2_unpack(f2_fma(f2_pack(rcp_fast(a0), rcp_fast(a1)), c2(-2.f * c.cap), c2(c.cap)), a0, a1);
+  f2_unpack(f2_mul(f2_fma(f2_pack(rcp_fast(a0), rcp_fast(a1)), c2(-2.f), c2(1.f)), c2(c.cap)), a0, a1);
   uint64_t p = f2_fma(u, c2(62.f / 2835.f), c2(-17.f / 315.f));
   p = f2_fma(p, u, c2(2.f / 15.f));
   p = f2_mul(f2_fma(p, u, c2(-1.f / 3.f)), u);
@@ -411,7 +412,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 #pragma unroll
             for (int j = 0; j < 32; j += 2) cap2(a.cap, f[j], f[j + 1]);
           }
-          if ((unsigned)(target - n0) < 32u) {
+          if ((unsigned)target - (unsigned)n0 < 32u) {
             float z = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) z = target - n0 == j ? f[j] : z;
@@ -488,8 +489,16 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           S = U = 0.f;
         }
       } else {
-        if (!sums_there()) break;
         const int n_out0 = ni * OUT_BN, n_out = kGlu ? a.N / 2 : a.N;
+        // what the columns are multiplied by and what is added is on its way while the tile's products are made
+        for (int c = team; c < NCHUNK; c += EG / 2) {
+          const int col = c * CHUNK + half * (CHUNK / 2), n0 = ni * BN + col;
+          if (lane == 0 && n0 < a.N) prefetch_l1(a.ws + n0);
+          if (kGlu && lane == 1) prefetch_l1(a.ws + n0 + 128);
+          if (has_bias(EPI) && lane == 2 && n0 < a.N) prefetch_l1(a.bias + n0);
+          if (has_resid(EPI) && live && n0 < n_out) prefetch_l2_line(a.r + (size_t)row_g * a.ldr + n0);
+        }
+        if (!sums_there()) break;
 #pragma unroll 1
         for (int c = team; c < NCHUNK; c += EG / 2) {
           const bool last = c + EG / 2 >= NCHUNK;
@@ -1038,34 +1047,37 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid
         for (int j = 0; j < 16; ++j) z[j] = 0.f;
         for (int k0 = 0; k0 < a.kbs && ok; k0 += kPiece) take();
       }
-      if (!ok || n >= a.V) continue;
+      __syncwarp();
+      if (ok && n < a.V) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(s_xs + r0 + j);
-        z[j] = __fmul_rn(z[j], x.x);
-        z[j + 1] = __fmul_rn(z[j + 1], x.y);
-        z[j + 2] = __fmul_rn(z[j + 2], x.z);
-        z[j + 3] = __fmul_rn(z[j + 3], x.w);
-      }
-      if (a.cap.cap > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) cap2(a.cap, z[j], z[j + 1]);
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (s_targets[r0 + j] == n) a.at[r0 + j] = z[j];
-        if (z[j] - m[j] > 8.f) {  // (m need not be the maximum: it follows when it is left far behind)
-          if (m[j] > -INFINITY) {
-            const float d = m[j] - z[j], w = exp2_fast(d * kLog2e);
-            U[j] = w > 0.f ? w * fmaf(d, S[j], U[j]) : 0.f;
-            S[j] *= w;
-          }
-          m[j] = z[j];
+        for (int j = 0; j < 16; j += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(s_xs + r0 + j);
+          z[j] = __fmul_rn(z[j], x.x);
+          z[j + 1] = __fmul_rn(z[j + 1], x.y);
+          z[j + 2] = __fmul_rn(z[j + 2], x.z);
+          z[j + 3] = __fmul_rn(z[j + 3], x.w);
         }
-        const float d = z[j] - (m[j] > -INFINITY ? m[j] : 0.f), w = exp2_fast(d * kLog2e);
-        S[j] += w;
-        U[j] = fmaf(w, d, U[j]);
+        if (a.cap.cap > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) cap2(a.cap, z[j], z[j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (s_targets[r0 + j] == n) a.at[r0 + j] = z[j];
+          if (z[j] - m[j] > 8.f) {  // (m need not be the maximum: it follows when it is left far behind)
+            if (m[j] > -INFINITY) {
+              const float d = m[j] - z[j], w = exp2_fast(d * kLog2e);
+              U[j] = w > 0.f ? w * fmaf(d, S[j], U[j]) : 0.f;
+              S[j] *= w;
+            }
+            m[j] = z[j];
+          }
+          const float d = z[j] - (m[j] > -INFINITY ? m[j] : 0.f), w = exp2_fast(d * kLog2e);
+          S[j] += w;
+          U[j] = fmaf(w, d, U[j]);
+        }
       }
+      __syncwarp();
     }
     // the lanes' sums: each row's brought to one m, then half of the rows to each half of the lanes, and so on
     const int j0 = lane >> 1;  // the row that this lane ends up with
@@ -1265,13 +1277,13 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
 // Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile, the least that a round takes (what follows the products, plain | gelu and gated
 // units) and the part that does not depend on sizes, fitted to runs (us):
 //                            256 x 256 pair  192 pair  128 pair  128 x 256  128 x 192  128 x 128  parts of K
-//   8192 x 28672 x  4096            586         652       806       660        746        896
-//   1100 x  4096 x 14336 (R)         76          63        89        52         80         68
-//    512 x  2048 x  8192             24.6        21.6      20.9      28.4       26.5       22.1
-//   5000 x  2304 x   768 (bias)      18.4        19.4      17.1      17.1       18.2       16.5
-//    777 x  8960 x  1536 (gelu)      20.2        22.0      21.2      19.3       21.2       21.5
-//    200 x  4096 x  4096             15.7        14.1      13.1      17.0       15.8       13.4      19.3
-//    128 x  4096 x  4096                                   13.2      17.3                  13.4      10.9
+//   8192 x 28672 x  4096            575         639       796       651        736        889
+//   1100 x  4096 x 14336 (R)         73.8        62.9      86.8      52.3       79.8       67.5
+//    512 x  2048 x  8192             24.4        21.5      20.4      28.0       26.3       22.0
+//   5000 x  2304 x   768 (bias)      16.9        17.9      16.2      15.9       17.1       16.0
+//    777 x  8960 x  1536 (gelu)      19.5        20.9      21.1      18.8       21.1       21.3
+//    200 x  4096 x  4096             15.4        14.0      13.1      16.8       15.6       13.4      19.3
+//    128 x  4096 x  4096                                   13.2      17.3                  13.4      10.7
 //     32 x 28672 x  4096                                   36.0      24.2                  26.2      24.0
 //    200 x   512 x 14336                                   31.2      44.9                  34.3      10.8
 // A row's sums are whole numbers: its bits do not depend on the choice.
@@ -1279,7 +1291,7 @@ struct TileShape {
   int bn, cg;
   double kb, floor, deep_floor;
 };
-constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.5, 7.0}, {192, 2, 0.311, 3.6, 5.4}, {128, 2, 0.258, 2.4, 3.8}, {256, 1, 0.418, 4.2, 7.0}, {192, 1, 0.356, 3.4, 5.3}, {128, 1, 0.287, 2.4, 3.8}};
+constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.0, 7.3}, {192, 2, 0.311, 3.3, 5.4}, {128, 2, 0.258, 2.3, 4.1}, {256, 1, 0.418, 3.7, 7.0}, {192, 1, 0.356, 3.1, 5.4}, {128, 1, 0.287, 2.2, 4.1}};
 
 template <int EPI>
 cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
@@ -1297,7 +1309,7 @@ cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
       pick = &t;
     }
   }
-  if (g.N <= 65535 * SN && split_us(g.M, g.N, kbs, sms, load_us) < best) return launch_split(stream, g, sms);
+  if (g.N <= 65535 * SN && g.M <= 65535 * TM && split_us(g.M, g.N, kbs, sms, load_us) < best) return launch_split(stream, g, sms);
   TileArgs a{};
   a.xs = g.x_scales;
   a.ws = g.w_scales;
@@ -1344,7 +1356,7 @@ cudaError_t q8_status() {
 
 cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& g) {
   const bool f32 = g.epi == EPI_F32, glu = g.epi == EPI_SWIGLU;
-  if (g.epi < EPI_NONE || g.epi > EPI_F32 || g.M < 0 || g.N < 1 || g.K < 1 || g.K > kMostK || (glu && g.N % 256)) return cudaErrorInvalidValue;
+  if (g.epi < EPI_NONE || g.epi > EPI_F32 || g.M < 0 || g.M > (1 << 30) || g.N < 1 || g.N > (1 << 30) || g.K < 1 || g.K > kMostK || (glu && g.N % 256)) return cudaErrorInvalidValue;
   if (g.M == 0) return cudaSuccess;
   if (!g.x || ((uintptr_t)g.x & 15) || g.ldx < g.K || g.ldx % 16 || !g.w || ((uintptr_t)g.w & 15) || g.ldw < g.K || g.ldw % 16) return cudaErrorInvalidValue;
   if (!g.x_scales || ((uintptr_t)g.x_scales & 3) || !g.w_scales || ((uintptr_t)g.w_scales & 15)) return cudaErrorInvalidValue;
@@ -1392,7 +1404,7 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   a.part = g.workspace;
   a.at = g.workspace + 3 * (size_t)score_slots(g.T, g.V) * g.T;
   a.scale = g.scale;
-  a.cap = {g.softcap, 1.f / g.softcap};
+  a.cap = {g.softcap, std::min(1.f / g.softcap, 3.4028235e38f)};  // (a logit of 0 stays 0 under the smallest caps)
   const Operand x{g.x, g.ldx, g.T}, w{g.w, g.ldw, g.V};
   if (sms < 2) return cudaErrorInvalidConfiguration;
   cudaError_t e;

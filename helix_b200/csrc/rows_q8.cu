@@ -263,7 +263,7 @@ cudaError_t launch_rows(cudaStream_t stream, const RowsQ8Args& a, int sms) {
 }  // namespace
 
 cudaError_t rows_q8(cudaStream_t stream, const RowsQ8Args& a) {
-  if (a.T < 0 || a.K < 1 || a.K > INT32_MAX - 65536) return cudaErrorInvalidValue;  // (steps past the last entry stay within 32 bits)
+  if (a.T < 0 || a.T > (1 << 30) || a.K < 1 || a.K > (1 << 30)) return cudaErrorInvalidValue;
   if (a.T == 0) return cudaSuccess;
   if (!a.x || ((uintptr_t)a.x & 15) || a.ldx < a.K || a.ldx % 8 || !a.codes || ((uintptr_t)a.codes & 15) || a.ldc < a.K || a.ldc % 16 || !a.scales || ((uintptr_t)a.scales & 3) ||
       (a.seen && (((uintptr_t)a.seen & 15) || a.lds < a.K || a.lds % 8)))

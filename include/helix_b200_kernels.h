@@ -157,22 +157,23 @@ int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, cons
 
 /* ---- products in 8-bit whole numbers with a scale for each token and each channel, and scores of given tokens.  A row of codes c in -127..127 with a scale s
  * stands for s c.  These calls take the stream they run on (NULL: the legacy default stream), allocate nothing, never wait, and can be captured into a graph; a call's
- * buffers are on the current device, and outputs overlap no input but where it is said.  Row strides count entries; codes lie on 16 bytes in rows of a multiple of 16.
+ * buffers are on the current device, and outputs overlap no input but where it is said.  Row strides count entries; codes, weight scales, biases, matrices of bf16 and fp32 lie
+ * on 16 bytes, strides of codes are multiples of 16, others of 8 (fp32 out of a product: 4).  Rows, columns and logits of a row up to 2^30 (scored rows 2^28).
  *
- * Rows x [T][K] (bf16, or fp32 where x_f32; on 16 bytes, ldx a multiple of 8 and 4) to codes [T][ldc >= K] and scales [T]: s = max |x| / 127 rounded to fp32, c the
- * whole number nearest to x / s (exactly: of two equally near ones the even one).  A row of zeros has scale 0 and codes 0, as has one whose s rounds to 0; a row with
- * an infinity or a NaN has scale NaN and codes 0.  seen [T][lds >= K] (or NULL; on 16 bytes, lds a multiple of 8; may be x itself where that is bf16): s c in
- * bf16, what products in 16 bits take if they shall see what products of the codes do.  Columns from K on are left as they are.  Weights are coded by the same call. */
+ * Rows x [T][ldx >= K] (bf16, or fp32 where x_f32) to codes [T][ldc >= K] and scales [T]: s = max |x| / 127 rounded to fp32, c the whole number nearest to x / s (exactly: of
+ * two equally near ones the even one).  A row of zeros has scale 0 and codes 0, as has one whose s rounds to 0; a row with an infinity or a NaN has scale NaN and codes 0.
+ * seen [T][lds >= K] (or NULL; may be x itself where that is bf16, with its stride): s c in bf16, what products in 16 bits take if they shall see what products of the codes
+ * do.  Columns from K on are left as they are.  Weights are coded by the same call, a channel per row. */
 int hbk_rows_q8(const void* x, int x_f32, int ldx, void* codes, int ldc, float* scales, void* seen, int lds, int T, int K, void* stream);
-/* out[M, N] = (X W^T)[m, n] x_scales[m] w_scales[n] of codes X [M][K], W [N][K]: sums in 32-bit whole numbers, exact for K up to 131056 (more is refused); epi as in
- * hbk_gemm, 0 to 6 (5: W rows packed [128 gate|128 up] per 256, out has N/2 columns; the erf of 2 is good to 1.5e-7).  out and R are bf16 (6: out fp32) on 16 bytes
- * with strides of a multiple of 8 (6: 4), R may be out itself; bias [N] bf16.  Any M and N >= 1. */
+/* out[M, N] = (X W^T)[m, n] x_scales[m] w_scales[n] of codes X [M][K], W [N][K] (any signed bytes): sums in 32-bit whole numbers, exact for K up to 131056 (more is refused), so
+ * that a row's bits depend on nothing but its operands; epi as in hbk_gemm, 0 to 6 (5: W rows packed [128 gate|128 up] per 256, out has N/2 columns; the erf of 2 is good to
+ * 1.5e-7).  out and R are bf16 (6: out fp32), R may be out itself; bias [N] bf16. */
 int hbk_gemm_q8(const void* X, int ldx, const float* x_scales, const void* W, int ldw, const float* w_scales, void* out, int ldo, const void* R, int ldr,
                 const void* bias, int M, int N, int K, int epi, void* stream);
 /* Scores of given tokens straight from the head's product, whose logits are never stored: with z[t][v] = scale (X W^T)[t, v] (softcap > 0: softcap tanh(z / softcap)),
- * lp[t] = log softmax(z[t])[targets[t]] (-inf where that is none of 0..V-1) and entropy[t] in nats.  X [T][H], W [V][H] in bf16 (both scales NULL; on 16 bytes,
- * strides multiples of 8, any H), or codes with x_scales [T] and w_scales [V] (H up to 131056).  targets and lp, or entropy, may be NULL.  A row with an infinite or
- * NaN logit has NaN.  workspace: hbk_head_scores_workspace_floats(T, V) floats; launches that may run at the same time need one each. */
+ * lp[t] = log softmax(z[t])[targets[t]] (-inf where that is none of 0..V-1) and entropy[t] in nats.  X [T][H], W [V][H] in bf16 (both scales NULL), or codes with x_scales
+ * [T] and w_scales [V] (H up to 131056).  targets and lp, or entropy, may be NULL.  A row with an infinite or NaN logit has NaN.  workspace:
+ * hbk_head_scores_workspace_floats(T, V) floats; launches that may run at the same time need one each. */
 int hbk_head_scores(const void* X, int ldx, const float* x_scales, const void* W, int ldw, const float* w_scales, const int32_t* targets, float* lp,
                     float* entropy, float* workspace, int T, int V, int H, float scale, float softcap, void* stream);
 size_t hbk_head_scores_workspace_floats(int T, int V); /* 0: refused sizes */
@@ -182,9 +183,9 @@ size_t hbk_head_scores_workspace_floats(int T, int V); /* 0: refused sizes */
 int hbk_q8_status(void);
 /* cycles after which such a wait is given up by the calls that follow (below 0: at once), of the whole process; returns the former */
 long long hbk_q8_wait_cycles(long long cycles);
-/* Scores of given tokens from logits [T][V] (fp32 where f32, else bf16; on 16 bytes, ldl a multiple of 8): lp[t] = log softmax of targets[t], rank[t] = how many tokens come
- * before it in the order (logit descending, id ascending), entropy[t] in nats, and the first n_top (0..64, at most V) of that order: top_ids, top_lp [T][n_top].
- * Any of lp, rank, entropy, top_lp may be NULL (and targets where lp and rank are; top_ids only with n_top 0).  A target that is none of 0..V-1: lp -inf, rank -1.  Masked
+/* Scores of given tokens from logits [T][ldl >= V] (fp32 where f32, else bf16): lp[t] = log softmax of targets[t], rank[t] = how many tokens come before it in the
+ * order (logit descending, id ascending), entropy[t] in nats, and the first n_top (0..64, at most V) of that order: top_ids, top_lp [T][n_top].  Any of lp, rank,
+ * entropy, top_lp may be NULL (and targets where lp and rank are; top_ids only with n_top 0).  A target that is none of 0..V-1: lp -inf, rank -1.  Masked
  * entries are -inf or as low as the type goes; a row of nothing but -inf has lp -inf and entropy 0.  With a NaN or +inf in a row its lp and entropy are NaN; a NaN is never
  * picked and before no token (a NaN target has rank -1), and ids are -1 where nothing is left to pick. */
 int hbk_token_scores(const void* logits, int f32, int ldl, const int32_t* targets, int T, int V, int n_top, float* lp, int32_t* rank, float* entropy,

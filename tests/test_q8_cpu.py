@@ -13,7 +13,7 @@ def rows(x=OK, f32=0, ldx=256, codes=OK, ldc=256, scales=OK, seen=None, lds=0, T
 
 @pytest.mark.parametrize("kw", [dict(x=None), dict(codes=None), dict(scales=None), dict(x=OK + 8), dict(codes=OK + 8), dict(scales=OK + 2), dict(ldx=248), dict(ldx=260), dict(ldc=248), dict(ldc=264),
                                 dict(f32=1, ldx=252), dict(f32=1, x=OK + 4), dict(f32=1, ldx=260), dict(seen=OK, lds=248), dict(seen=OK, lds=260), dict(seen=OK + 2, lds=256), dict(T=-1), dict(K=0),
-                                dict(K=-1), dict(K=2 ** 31 - 16, ldx=2 ** 31 - 8, ldc=2 ** 31 - 16)])
+                                dict(K=-1), dict(K=2 ** 30 + 1, ldx=2 ** 31 - 8, ldc=2 ** 31 - 16), dict(T=2 ** 30 + 1)])
 def test_rows_refusals(kw):
     assert rows(**kw) == 1 and b"invalid argument" in L.hbk_last_error()
 
@@ -25,7 +25,7 @@ def gemm(x=OK, ldx=256, xs=OK, w=OK, ldw=256, ws=OK, out=OK, ldo=64, r=None, ldr
 @pytest.mark.parametrize("kw", [dict(x=None), dict(xs=None), dict(w=None), dict(ws=None), dict(out=None), dict(x=OK + 8), dict(xs=OK + 2), dict(w=OK + 8), dict(ws=OK + 4), dict(out=OK + 8), dict(ldx=240),
                                 dict(ldx=264), dict(ldw=240), dict(ldw=264), dict(ldo=56), dict(ldo=68), dict(ldo=66, epi=6), dict(M=-1), dict(N=0), dict(K=0), dict(K=131057, ldx=131072, ldw=131072),
                                 dict(epi=-1), dict(epi=7), dict(epi=8), dict(epi=1), dict(epi=2), dict(epi=3), dict(epi=4, bias=OK), dict(epi=4, r=OK, ldr=64), dict(epi=3, r=OK, ldr=56),
-                                dict(epi=3, r=OK, ldr=68), dict(epi=3, r=OK + 8, ldr=64), dict(epi=1, bias=OK + 2), dict(epi=5), dict(epi=5, N=320), dict(epi=5, N=256, ldo=120)])
+                                dict(epi=3, r=OK, ldr=68), dict(epi=3, r=OK + 8, ldr=64), dict(epi=1, bias=OK + 2), dict(epi=5), dict(epi=5, N=320), dict(epi=5, N=256, ldo=120), dict(M=2 ** 30 + 1), dict(N=2 ** 30 + 1, ldo=2 ** 31 - 8)])
 def test_product_refusals(kw):
     assert gemm(**kw) == 1
 

@@ -328,7 +328,7 @@ def check_head(lp, entropy, x, xs, w, ws, targets, H, scale=1.0, cap=0.0):
         off = 5 * 2.0 ** -24 * z.abs()
     if cap > 0:
         z = cap * torch.tanh(z / cap)
-        off = off + 2.0 ** -21 * z.abs()
+        off = off + 2.0 ** -20 * z.abs()  # (1 - 2 / (e^2y + 1) with two approximate functions is off by 2^-22, and 1/4 at least)
     worst = off.max(-1).values
     a, b = exact_scores(z, targets if targets is not None else torch.zeros(T, dtype=torch.int32, device=DEV))
     sums = 2.0 ** -18 + 2.0 ** -23 * z.abs().max(-1).values  # (up to 300 terms one after the other, each off by 2^-22 and by its exponent's rounding)
@@ -408,6 +408,19 @@ def test_head_flat_and_steep_rows(L, T, scale):
     check_head(lp, entropy, x, None, w, None, targets, H, scale=scale)
     if scale < 1:
         assert (lp + math.log(V)).abs().max() < 1e-5 and (entropy - math.log(V)).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("T", [4, 100, 300])
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 1e-30, 0.01, 0.3, 5.0, 1e4, 1e30, 3.4e38])
+def test_head_caps_of_any_size(L, T, cap):
+    V, H = 3000, 128
+    x, w = randn(1, T, H).to(BF), (randn(2, V, H) * 0.3).to(BF)
+    x[2] = 0  # logits of 0 stay 0
+    targets = torch.randint(0, V, (T,), generator=gen(3), device=DEV).int()
+    cap = torch.tensor(cap, dtype=torch.float32).item()  # (as the call takes it)
+    lp, entropy = head(L, x, None, w, None, targets, H, cap=cap)
+    check_head(lp, entropy, x, None, w, None, targets, H, cap=cap)
+    assert (lp[2] + math.log(V)).abs() < 1e-5
 
 
 def test_head_again_is_the_same(L):
