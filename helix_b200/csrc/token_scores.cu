@@ -455,14 +455,13 @@ cudaError_t launch_nc(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
 }
 template <bool F32, bool TOP>
 cudaError_t launch_top(cudaStream_t stream, const TokenScoresArgs& a, int sms) {
-  // Blocks per row: twice as many while not all SMs have one (up to four per row: two, where each keeps twelve steps) and a block keeps seven steps.  us with 1 | 2 | 4 | 8 blocks
-  // per row: 8 x 128256 fp32 20.0 | 14.5 | 11.1 | 10.6, 32 rows 21.3 | 16.2 | 13.3 | 14.7, 64 rows 21.7 | 16.9 | 14.9 | 20.1; 100 x 32768 9.9 | 10.7 | 11.7 | 20.6.  Blocks of twice
-  // the threads, or that fetch eight steps ahead, where few blocks run: the same within a tenth either way
+  // Blocks per row: twice as many while a block keeps seven steps and not all SMs have one (up to four per row: some three, where a row has 24 steps).  us with 1 | 2 | 4 | 8
+  // blocks per row: 8 x 128256 fp32 20.0 | 14.5 | 11.1 | 10.6, 32 rows 21.3 | 16.2 | 13.3 | 14.7, 64 rows 21.7 | 16.9 | 14.9 | 20.1, 100 rows 21.9 | 19.8 | 18.6, 150 rows
+  // 26.5 | 24.0 | 28.2, 250 rows 29.2 | 31.0 | 36.2; 100 x 32768 9.8 | 10.7 | 11.0 | 20.6.  Blocks of twice the threads, or that fetch eight steps ahead, where few blocks run:
+  // the same within a tenth either way
   int nc = 1;
-  auto more = [&](int to) {
-    const long long step = (long long)to * kThreads * kEntries<F32>;
-    return a.V >= 7 * step && (long long)a.T * to <= (to <= 4 && a.V >= 12 * step ? 2LL * sms : sms);
-  };
+  constexpr long long kStepOf = (long long)kThreads * kEntries<F32>;
+  auto more = [&](int to) { return a.V >= 7 * to * kStepOf && (long long)a.T * to <= (to <= 4 && a.V >= 24 * kStepOf ? 11LL * sms / 4 : sms); };
   while (nc < 8 && more(nc * 2)) nc *= 2;
   switch (nc) {
     case 1: return launch_nc<F32, 1, TOP>(stream, a, sms);
