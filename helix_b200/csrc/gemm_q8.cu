@@ -120,7 +120,7 @@ __host__ __device__ constexpr bool has_bias(int epi) { return epi == EPI_BIAS ||
 __host__ __device__ constexpr bool has_resid(int epi) { return epi == EPI_RESID || epi == EPI_BIAS_RESID; }
 
 struct TileArgs {
-  const float *xs, *ws;       // scales of rows and columns (NULL: bf16 operands)
+  const float *xs, *ws;       // scales of rows and columns (codes)
   const bf16* bias;
   const bf16* r;
   void* out;
@@ -168,25 +168,20 @@ __device__ __forceinline__ void tile_at(const TileArgs& a, int t, int num_m, int
   ni = a.group_n ? x : y;
 }
 
-// NC sums of a row to values: the whole numbers times both scales, or the fp32 sums themselves
-template <bool I8, int NC>
+// NC whole numbers of a row times both scales
+template <int NC>
 __device__ __forceinline__ void values_of(const uint32_t (&v)[NC], const TileArgs& a, float sx, int n0, float (&f)[NC]) {
-  if constexpr (I8) {
-    if (n0 + NC <= a.N) {
-      const uint64_t s2 = f2_pack(sx, sx);
+  if (n0 + NC <= a.N) {
+    const uint64_t s2 = f2_pack(sx, sx);
 #pragma unroll
-      for (int j = 0; j < NC; j += 4) {
-        const float4 w = __ldg(reinterpret_cast<const float4*>(a.ws + n0 + j));
-        f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j], (float)(int)v[j + 1]), f2_pack(w.x, w.y)), s2), f[j], f[j + 1]);
-        f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j + 2], (float)(int)v[j + 3]), f2_pack(w.z, w.w)), s2), f[j + 2], f[j + 3]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NC; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
+    for (int j = 0; j < NC; j += 4) {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(a.ws + n0 + j));
+      f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j], (float)(int)v[j + 1]), f2_pack(w.x, w.y)), s2), f[j], f[j + 1]);
+      f2_unpack(f2_mul(f2_mul(f2_pack((float)(int)v[j + 2], (float)(int)v[j + 3]), f2_pack(w.z, w.w)), s2), f[j + 2], f[j + 3]);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) f[j] = __uint_as_float(v[j]);
+    for (int j = 0; j < NC; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
   }
 }
 // 32 bf16 values of a row (of which `left` are there) added
@@ -466,7 +461,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             tmem_ld_32x32b_x32(t_row + grp * MINE + c, v);
             tmem_ld_wait();
             if (c + 32 == MINE) release();
-            values_of<I8>(v, a, sx, n_first + c, f);
+            values_of(v, a, sx, n_first + c, f);
             take(f, n_first + c);
           }
         } else {
@@ -510,7 +505,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             tmem_ld_32x32b_x16(t_row + col, v);
             tmem_ld_wait();
             if (last) release();
-            values_of<I8>(v, a, sx, n_out0 + col, f);
+            values_of(v, a, sx, n_out0 + col, f);
             bar_sync(1 + team, TEAM);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -527,8 +522,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 tmem_ld_32x32b_x16(t_row + 128 + col + h, u);
                 tmem_ld_wait();
                 if (h == 16 && last) release();
-                values_of<I8>(v, a, sx, ni * BN + col + h, g);
-                values_of<I8>(u, a, sx, ni * BN + 128 + col + h, x);
+                values_of(v, a, sx, ni * BN + col + h, g);
+                values_of(u, a, sx, ni * BN + 128 + col + h, x);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) f[h + j] = silu(g[j]) * x[j];
               }
@@ -537,7 +532,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
               tmem_ld_32x32b_x32(t_row + col, v);
               tmem_ld_wait();
               if (last) release();
-              values_of<I8>(v, a, sx, n0, f);
+              values_of(v, a, sx, n0, f);
             }
             if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
             if constexpr (EPI == EPI_BIAS_GELU) {
