@@ -393,6 +393,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             release();
           }
         } else {
+          const int n0 = ni * BN + grp * MINE + lane * 32;
+          if (lane < MINE / 32 && n0 < a.N) prefetch_l1(a.ws + n0);  // (on its way while the tile's products are made)
           sums_there();
         }
         if (!ok) break;
