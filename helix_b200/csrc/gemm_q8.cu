@@ -755,6 +755,15 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0);
+  // W is on its way into L2 (nothing of it is read) while the kernel before ends: 13 x 4096 x 14336 15.1 -> 13.9 us back to back, 32 x 28672 x 4096 gated 23.2 -> 21.3; with more rows
+  // of X these come late behind the others (128 x 4096 x 4096 10.7 -> 10.9)
+  if (a.box_rows <= 64 && warp == 0 && elect_one_sync()) {
+    for (int kb = kb0; kb < min(kb1, kb0 + stages); ++kb) {
+      tma_prefetch_l2_2d(&map_w, kb * KB, w0);
+      tma_prefetch_l2_2d(&map_w, kb * KB, w1);
+    }
+  }
+  __syncwarp();
   pdl_wait();
 
   bool ok = true;
@@ -901,7 +910,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------ scores of few rows
-constexpr int kFewRows = 64, kFewThreads = 64 + 4 * 128, kFewSmem = 200 * 1024;  // (the kernel that joins the sums finds room beside it)
+constexpr int kFewRows = 64, kFewThreads = 64 + 4 * 128, kFewSmem = 184 * 1024;  // (us of 32 | 16 rows of a 1 GB head with 100, 130, 165, 200, 225 KB: 181, 171, 166, 165, 173 | 176, 168, 164, 168, 174)
 
 struct FewArgs {
   const float *xs, *ws;
@@ -945,6 +954,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid
     tmem_relinquish();
     pdl_launch_dependents();  // (launch.h)
   }
+  if (warp == 2 && elect_one_sync())  // W is on its way into L2 (nothing of it is read) while the kernel before ends
+    for (int kb = 0; kb < min(a.kbs, stages); ++kb) tma_prefetch_l2_2d(&map_w, k_at<I8>(kb), blockIdx.x * SN);
+  __syncwarp();
   pdl_wait();
   if (threadIdx.x < kFewRows) {
     const int t = threadIdx.x;
@@ -1409,10 +1421,12 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   else if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   if (e != cudaSuccess) return e;
-  // Few sums: small blocks, which find room beside the kernel before and wait there for its end, and many threads per row (a row of a head of 151936 x 1536 in codes 51.5 -> 47.8 us)
+  // Few sums: many threads per row (a row of a head of 151936 x 1536 in codes 51.5 -> 47.8 us).  Blocks that wait beside the kernel before for its end cost it more than their start
+  // is worth once there are more than a few (us started early | behind it: 4 rows of a 1 GB head 187.9 | 189.9, 16 rows 195.8 | 188.5, 128 rows 196.9 | 191.8)
+  const bool early = g.T <= 8;
   if (slots <= 600)
-    return launch_k(join_scores_kernel<128, 2>, dim3((g.T + 1) / 2), dim3(128), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
-  return launch_k(join_scores_kernel<512, 8>, dim3((g.T + 7) / 8), dim3(512), 0, stream, true, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
+    return launch_k(join_scores_kernel<128, 2>, dim3((g.T + 1) / 2), dim3(128), 0, stream, early, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
+  return launch_k(join_scores_kernel<512, 8>, dim3((g.T + 7) / 8), dim3(512), 0, stream, early, (const float*)a.part, (const float*)a.at, g.targets, g.lp, g.entropy, slots, g.T, g.V);
 }
 
 }  // namespace hb
