@@ -152,7 +152,9 @@ struct Cfg {
   static constexpr int THREADS = 64 + EG * 128;
   static constexpr int X_BYTES = TM * KB, W_BYTES = BN / CG * KB;
   static constexpr int STAGE = X_BYTES + W_BYTES;
-  static constexpr int STAGING = EPI == EPI_SCORES ? 0 : 2 * kStaging;
+  // Products: teams of groups, a staging buffer each, take chunks of 128 bytes per row in turn: two teams of two groups, or three of one where there are three chunks (192 columns)
+  static constexpr int TEAMS = EPI == EPI_SCORES ? EG : BN == 192 && EPI != EPI_F32 ? 3 : 2, MEMBERS = EPI == EPI_SCORES || TEAMS == 3 ? 1 : 2;
+  static constexpr int STAGING = EPI == EPI_SCORES ? 0 : TEAMS * kStaging;
   static constexpr int FIXED = STAGING + 1024 + 512;  // alignment, barriers
   static constexpr int RAW = (227 * 1024 - FIXED) / STAGE;
   static constexpr int STAGES = RAW > 10 ? 10 : RAW;
@@ -240,7 +242,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sums_full[i], 1);
-      mbar_init(&sums_empty[i], 4 * EG * CG);
+      mbar_init(&sums_empty[i], 4 * C::TEAMS * C::MEMBERS * CG);
     }
     mbar_init(all_done, 1);
     fence_barrier_init();
@@ -335,12 +337,12 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
       }
     }
-  } else {
+  } else if ((warp - 2) >> 2 < C::TEAMS * C::MEMBERS) {
     const int q = warp & 3, row = q * 32 + lane;  // row of the block's 128, lane of tensor memory
     const int grp = (warp - 2) >> 2;
-    // products: two groups share a chunk of 128 bytes per row, half each; scores: each has its columns
-    constexpr int TEAM = kScores ? 128 : 256;
-    const int team = kScores ? grp : grp >> 1, half = grp & 1;
+    // products: a team's groups share a chunk, half each; scores: each group has its columns
+    constexpr int TEAMS = C::TEAMS, MEMBERS = C::MEMBERS, TEAM = 128 * MEMBERS;
+    const int team = grp / MEMBERS, half0 = MEMBERS == 2 ? grp & 1 : 0, half1 = MEMBERS == 2 ? half0 + 1 : 2;  // halves of a chunk that are this group's
     const bool leader = (threadIdx.x - 64) % TEAM == 0;
     uint8_t* const buf = staging + team * kStaging;
     uint8_t* const my_row = buf + row * 128;
@@ -488,8 +490,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       } else {
         const int n_out0 = ni * OUT_BN, n_out = kGlu ? a.N / 2 : a.N;
         // what the columns are multiplied by and what is added is on its way while the tile's products are made
-        for (int c = team; c < NCHUNK; c += EG / 2) {
-          const int col = c * CHUNK + half * (CHUNK / 2), n0 = ni * BN + col;
+        for (int c = team; c < NCHUNK; c += TEAMS) {
+          const int col = c * CHUNK + half0 * (CHUNK / 2), n0 = ni * BN + col;
           if (lane == 0 && n0 < a.N) prefetch_l1(a.ws + n0);
           if (kGlu && lane == 1) prefetch_l1(a.ws + n0 + 128);
           if (has_bias(EPI) && lane == 2 && n0 < a.N) prefetch_l1(a.bias + n0);
@@ -497,11 +499,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
         if (!sums_there()) break;
 #pragma unroll 1
-        for (int c = team; c < NCHUNK; c += EG / 2) {
-          const bool last = c + EG / 2 >= NCHUNK;
+        for (int c = team; c < NCHUNK; c += TEAMS) {
+          const bool last = c + TEAMS >= NCHUNK;
           if (leader) tma_store_wait_read<0>();  // the team's store before has read `buf`
           if constexpr (kF32) {
-            const int col = c * 32 + half * 16;
+            const int col = c * 32 + half0 * 16;
             uint32_t v[16];
             float f[16];
             tmem_ld_32x32b_x16(t_row + col, v);
@@ -511,54 +513,57 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             bar_sync(1 + team, TEAM);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(my_row + (((half * 4 + j) ^ (row & 7)) << 4)) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+              *reinterpret_cast<float4*>(my_row + (((half0 * 4 + j) ^ (row & 7)) << 4)) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
           } else {
-            const int col = c * 64 + half * 32, n0 = n_out0 + col;
-            float f[32];
-            if constexpr (kGlu) {
+#pragma unroll 1
+            for (int half = half0; half < half1; ++half) {
+              const int col = c * 64 + half * 32, n0 = n_out0 + col;
+              float f[32];
+              if constexpr (kGlu) {
 #pragma unroll
-              for (int h = 0; h < 32; h += 16) {
-                uint32_t v[16], u[16];
-                float g[16], x[16];
-                tmem_ld_32x32b_x16(t_row + col + h, v);
-                tmem_ld_32x32b_x16(t_row + 128 + col + h, u);
+                for (int h = 0; h < 32; h += 16) {
+                  uint32_t v[16], u[16];
+                  float g[16], x[16];
+                  tmem_ld_32x32b_x16(t_row + col + h, v);
+                  tmem_ld_32x32b_x16(t_row + 128 + col + h, u);
+                  tmem_ld_wait();
+                  if (h == 16 && last && half + 1 == half1) release();
+                  values_of(v, a, sx, ni * BN + col + h, g);
+                  values_of(u, a, sx, ni * BN + 128 + col + h, x);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) f[h + j] = silu(g[j]) * x[j];
+                }
+              } else {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(t_row + col, v);
                 tmem_ld_wait();
-                if (h == 16 && last) release();
-                values_of(v, a, sx, ni * BN + col + h, g);
-                values_of(u, a, sx, ni * BN + 128 + col + h, x);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) f[h + j] = silu(g[j]) * x[j];
+                if (last && half + 1 == half1) release();
+                values_of(v, a, sx, n0, f);
               }
-            } else {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(t_row + col, v);
-              tmem_ld_wait();
-              if (last) release();
-              values_of(v, a, sx, n0, f);
-            }
-            if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
-            if constexpr (EPI == EPI_BIAS_GELU) {
+              if constexpr (has_bias(EPI)) add_32(a.bias + n0, n_out - n0, f);
+              if constexpr (EPI == EPI_BIAS_GELU) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) gelu_erf2(f[j], f[j + 1]);
-            }
-            if constexpr (has_resid(EPI)) {
-              if (live) add_32(a.r + (size_t)row_g * a.ldr + n0, n_out - n0, f);
-            }
-            bar_sync(1 + team, TEAM);
+                for (int j = 0; j < 32; j += 2) gelu_erf2(f[j], f[j + 1]);
+              }
+              if constexpr (has_resid(EPI)) {
+                if (live) add_32(a.r + (size_t)row_g * a.ldr + n0, n_out - n0, f);
+              }
+              if (half == half0) bar_sync(1 + team, TEAM);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4 o;
-              o.x = pack_bf16x2(f[8 * j], f[8 * j + 1]);
-              o.y = pack_bf16x2(f[8 * j + 2], f[8 * j + 3]);
-              o.z = pack_bf16x2(f[8 * j + 4], f[8 * j + 5]);
-              o.w = pack_bf16x2(f[8 * j + 6], f[8 * j + 7]);
-              *reinterpret_cast<uint4*>(my_row + (((half * 4 + j) ^ (row & 7)) << 4)) = o;
+              for (int j = 0; j < 4; ++j) {
+                uint4 o;
+                o.x = pack_bf16x2(f[8 * j], f[8 * j + 1]);
+                o.y = pack_bf16x2(f[8 * j + 2], f[8 * j + 3]);
+                o.z = pack_bf16x2(f[8 * j + 4], f[8 * j + 5]);
+                o.w = pack_bf16x2(f[8 * j + 6], f[8 * j + 7]);
+                *reinterpret_cast<uint4*>(my_row + (((half * 4 + j) ^ (row & 7)) << 4)) = o;
+              }
             }
           }
           const int n0 = n_out0 + c * CHUNK;
           if (n0 + CHUNK > n_out && n_out % (kF32 ? 4 : 8) != 0) {  // (a copy ends on 16 bytes: it would write zeros behind the last column)
             if (live) {
-              for (int j = half * (CHUNK / 2); j < (half + 1) * (CHUNK / 2) && n0 + j < n_out; ++j) {
+              for (int j = half0 * (CHUNK / 2); j < half1 * (CHUNK / 2) && n0 + j < n_out; ++j) {
                 const int at = ((j / (kF32 ? 4 : 8)) ^ (row & 7)) << 4, in = j % (kF32 ? 4 : 8);
                 if constexpr (kF32) static_cast<float*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const float*>(my_row + at)[in];
                 else static_cast<bf16*>(a.out)[(size_t)row_g * a.ldo + n0 + j] = reinterpret_cast<const bf16*>(my_row + at)[in];
@@ -1282,28 +1287,30 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   return cudaLaunchKernelEx(&l.cfg, split_kernel, mx, mw, a);
 }
 
-// Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile, the least that a round takes (what follows the products, plain | gelu and gated
-// units) and the part that does not depend on sizes, fitted to runs (us):
+// Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile and the least that a round takes (what follows the products: plain | gelu, gated
+// units and residuals); 4.8 beside them (and 2.5 for the last tile's, of the latter kind), fitted to runs (us):
 //                            256 x 256 pair  192 pair  128 pair  128 x 256  128 x 192  128 x 128  parts of K
 //   8192 x 28672 x  4096            575         639       796       651        736        889
-//   1100 x  4096 x 14336 (R)         73.8        62.9      86.8      52.3       79.8       67.5
-//    512 x  2048 x  8192             24.4        21.5      20.4      28.0       26.3       22.0
-//   5000 x  2304 x   768 (bias)      16.9        17.9      16.2      15.9       17.1       16.0
-//    777 x  8960 x  1536 (gelu)      19.5        20.9      21.1      18.8       21.1       21.3
+//   1100 x  4096 x 14336 (R)         73.9        63.0      86.5      53.4       79.8       67.9
+//    512 x  2048 x  8192             24.3        21.6      20.6      28.2       26.6       22.0
+//  13800 x  2304 x   768 (bias)      32.8        29.5      33.7      31.3       30.6       34.7
+//  13800 x   768 x   768 (R)         25.5        20.8      22.5      25.1       21.0       22.3
+//  13800 x  2304 x   768 (gelu)      47.0        42.6      44.8      43.0       42.9       45.2
+//    777 x  8960 x  1536 (gelu)      19.9        20.4      21.4      19.1       21.0       21.7
 //    200 x  4096 x  4096             15.4        14.0      13.1      16.8       15.6       13.4      19.3
 //    128 x  4096 x  4096                                   13.2      17.3                  13.4      10.7
-//     32 x 28672 x  4096                                   36.0      24.2                  26.2      24.0
+//     32 x 28672 x  4096                                   36.0      24.2                  26.2      22.6
 //    200 x   512 x 14336                                   31.2      44.9                  34.3      10.8
 // A row's sums are whole numbers: its bits do not depend on the choice.
 struct TileShape {
   int bn, cg;
   double kb, floor, deep_floor;
 };
-constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.0, 7.3}, {192, 2, 0.311, 3.3, 5.4}, {128, 2, 0.258, 2.3, 4.1}, {256, 1, 0.418, 3.7, 7.0}, {192, 1, 0.356, 3.1, 5.4}, {128, 1, 0.287, 2.2, 4.1}};
+constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.0, 6.0}, {192, 2, 0.311, 2.8, 4.2}, {128, 2, 0.258, 2.1, 2.9}, {256, 1, 0.418, 3.8, 5.5}, {192, 1, 0.356, 2.9, 4.2}, {128, 1, 0.287, 2.1, 2.9}};
 
 template <int EPI>
 cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
-  constexpr bool kGlu = EPI == EPI_SWIGLU, kDeep = kGlu || EPI == EPI_BIAS_GELU;
+  constexpr bool kGlu = EPI == EPI_SWIGLU, kDeep = kGlu || EPI == EPI_BIAS_GELU || has_resid(EPI);
   const int kbs = (g.K + KB - 1) / KB;
   const double load_us = (double)g.N * g.K / 6.2e6 + 2.0;  // (few rows: W's way from memory)
   const TileShape* pick = nullptr;
@@ -1311,7 +1318,7 @@ cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   for (const TileShape& t : kShapes) {
     if ((t.cg == 2 && sms < 2) || (kGlu && t.bn != 256)) continue;
     const long long tiles = (long long)((g.M + TM * t.cg - 1) / (TM * t.cg)) * ((g.N + t.bn - 1) / t.bn), workers = sms / t.cg;
-    const double us = std::max((double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor), load_us) + 4.8;
+    const double us = std::max((double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor), load_us) + (kDeep ? 7.3 : 4.8);
     if (us < best) {
       best = us;
       pick = &t;
