@@ -1268,9 +1268,9 @@ SplitPlan split_plan(int M, int N, int kbs, int sms) {
   const int stages = std::min(std::min(most, 12), (box <= 64 ? 108 : 216) * 1024 / stage);
   return {parts, stages, std::max(stages * stage, box * kDump * 4) + 1024, (int)std::min<long long>((tiles * parts + room - 1) / room, INT32_MAX)};
 }
-double split_us(int M, int N, int kbs, int sms, double load_us) {  // (fitted as below)
+double split_us(int M, int N, int kbs, int sms, double load_us, bool resid) {  // (fitted as below)
   const SplitPlan p = split_plan(M, N, kbs, sms);
-  return std::max(p.rounds * ((kbs + p.parts - 1) / p.parts * 0.287 + std::min(M, TM) / 16.0 / p.parts), load_us) + 4.4 + std::min(M, TM) / 100.0;
+  return std::max(p.rounds * ((kbs + p.parts - 1) / p.parts * 0.26 + std::min(M, TM) * (resid ? 0.076 : 0.034) / p.parts), load_us) + 3.5 + std::min(M, TM) / 40.0;
 }
 
 cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
@@ -1287,8 +1287,9 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   return cudaLaunchKernelEx(&l.cfg, split_kernel, mx, mw, a);
 }
 
-// Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile and the least that a round takes (what follows the products: plain | gelu, gated
-// units and residuals); 4.8 beside them (and 2.5 for the last tile's, of the latter kind), fitted to runs (us):
+// Which kernel, which tiles: the one whose rounds end first.  Per shape: us per block of K of one tile, the least that a round takes (what follows the products: plain | gelu, gated
+// units and residuals), what a launch takes beside them (a pair starts later, a wide last tile is longer on its way out); 3.6 (4.8 for the latter kind) for all.  Fitted to 1690 runs of
+// 283 products, 1 x 2048 x 2048 to 13800 x 2304 x 768: what it chooses takes 0.3% more than the fastest there on the mean.  Some of these (us):
 //                            256 x 256 pair  192 pair  128 pair  128 x 256  128 x 192  128 x 128  parts of K
 //   8192 x 28672 x  4096            575         639       796       651        736        889
 //   1100 x  4096 x 14336 (R)         73.9        63.0      86.5      53.4       79.8       67.9
@@ -1304,27 +1305,27 @@ cudaError_t launch_split(cudaStream_t stream, const GemmQ8Args& g, int sms) {
 // A row's sums are whole numbers: its bits do not depend on the choice.
 struct TileShape {
   int bn, cg;
-  double kb, floor, deep_floor;
+  double kb, floor, deep_floor, beside;
 };
-constexpr TileShape kShapes[] = {{256, 2, 0.370, 4.0, 6.0}, {192, 2, 0.311, 2.8, 4.2}, {128, 2, 0.258, 2.1, 2.9}, {256, 1, 0.418, 3.8, 5.5}, {192, 1, 0.356, 2.9, 4.2}, {128, 1, 0.287, 2.1, 2.9}};
+constexpr TileShape kShapes[] = {{256, 2, 0.352, 3.6, 6.2, 2.05}, {192, 2, 0.295, 2.75, 4.15, 1.9}, {128, 2, 0.239, 2.1, 2.7, 1.75}, {256, 1, 0.439, 4.0, 5.9, 0.65}, {192, 1, 0.414, 3.2, 4.4, 0.5}, {128, 1, 0.317, 2.35, 3.1, 0.35}};
 
 template <int EPI>
 cudaError_t launch_product(cudaStream_t stream, const GemmQ8Args& g, int sms) {
   constexpr bool kGlu = EPI == EPI_SWIGLU, kDeep = kGlu || EPI == EPI_BIAS_GELU || has_resid(EPI);
   const int kbs = (g.K + KB - 1) / KB;
-  const double load_us = (double)g.N * g.K / 6.2e6 + 2.0;  // (few rows: W's way from memory)
+  const double load_us = (double)g.N * g.K / 6.2e6 + 0.9;  // (few rows: W's way from memory)
   const TileShape* pick = nullptr;
   double best = 1e30;
   for (const TileShape& t : kShapes) {
     if ((t.cg == 2 && sms < 2) || (kGlu && t.bn != 256)) continue;
     const long long tiles = (long long)((g.M + TM * t.cg - 1) / (TM * t.cg)) * ((g.N + t.bn - 1) / t.bn), workers = sms / t.cg;
-    const double us = std::max((double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor), load_us) + (kDeep ? 7.3 : 4.8);
+    const double us = std::max((double)((tiles + workers - 1) / workers) * std::max(kbs * t.kb, kDeep ? t.deep_floor : t.floor), load_us) + t.beside + (kDeep ? 4.8 : 3.6);
     if (us < best) {
       best = us;
       pick = &t;
     }
   }
-  if (g.N <= 65535 * SN && g.M <= 65535 * TM && split_us(g.M, g.N, kbs, sms, load_us) < best) return launch_split(stream, g, sms);
+  if (g.N <= 65535 * SN && g.M <= 65535 * TM && split_us(g.M, g.N, kbs, sms, load_us, has_resid(EPI)) < best) return launch_split(stream, g, sms);
   TileArgs a{};
   a.xs = g.x_scales;
   a.ws = g.w_scales;
