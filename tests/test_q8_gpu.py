@@ -207,7 +207,8 @@ SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 96), (5, 130, 4096), (7, 1000, 160), (
          (33, 48, 320), (64, 96, 1025), (65, 129, 31), (100, 70, 544), (128, 1000, 3000), (1, 30000, 64),  # a cluster shares K
          (129, 256, 300), (256, 50, 96), (300, 2000, 500), (1000, 100, 9000),                             # and so with more rows
          (400, 6000, 100), (400, 6003, 300), (1000, 4005, 40), (1300, 1500, 1000), (2049, 520, 272),   # tiles of one block
-         (2600, 2304, 272), (2570, 2100, 1100), (5000, 4101, 130)]                                        # tiles of pairs
+         (2600, 2304, 272), (2570, 2100, 1100), (5000, 4101, 130),                                        # tiles of pairs
+         (154, 2722, 3033), (4194, 131, 3548), (6877, 260, 1948), (6546, 390, 1441), (6327, 392, 101), (6672, 397, 2840)]  # every shape of tile, plain and with more behind the products
 
 
 @pytest.mark.parametrize("epi", [0, 1, 2, 3, 4, 6])
