@@ -137,9 +137,11 @@ struct TileArgs {
   long long wait_cycles;
 };
 
-// Sums of bf16 products lose their last bits each time that more are added to them on the tensor cores: after so many blocks (512 terms) they are taken out and added in fp32.
-// (H = 4096: scores off by 3e-6 of themselves in one piece, 4e-7 in eight.)  Whole numbers lose nothing.
-constexpr int kPiece = 8;
+// Sums of bf16 products lose their last bits each time that more are added to them on the tensor cores (they are cut off, not rounded): after so many blocks they are taken out and
+// added in fp32.  In one piece scores of H = 4096 are off by 3e-6 of themselves, in pieces of 512 terms by 2.2e-7 (entropies 3.6e-7), of 256 by 1.1e-7 (1.6e-7), of 128 by 7e-8.
+// Up to 128 rows the weights' way from memory takes longer than either (us in pieces of 512 | 256 | 128, a 1 GB head: 1 row 167 | 167 | 171, 64 rows 175 | 178 | 193, 100 rows
+// 176 | 177 | 186), above it does not (2048 rows 1422 | 1488 | 1657, 1000 rows of 30522 x 768 41.6 | 48.3 | 60.4).  Whole numbers lose nothing.
+constexpr int kPiece = 8, kFewPiece = 4;  // blocks of 64 terms: above 128 rows, up to them
 
 template <bool I8>
 __device__ __forceinline__ int k_at(int kb) {  // a block's first entry
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(Cfg<I8, BN, CG, EPI>::THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
             const __grid_constant__ TileArgs a) {
   using C = Cfg<I8, BN, CG, EPI>;
-  constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG;
+  constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG, PIECE = CG == 1 ? kFewPiece : kPiece;
   constexpr bool kScores = EPI == EPI_SCORES, kGlu = EPI == EPI_SWIGLU, kF32 = EPI == EPI_F32;
   constexpr int OUT_BN = kGlu ? BN / 2 : BN, CHUNK = kF32 ? 32 : 64, NCHUNK = OUT_BN / CHUNK;
   static_assert(!kGlu || BN == 256, "[128 gate|128 up]");
@@ -306,7 +308,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       for (int t = worker; t < tiles && ok; t += workers) {
         uint32_t d = 0;
         for (int kb = 0; kb < a.kbs; ++kb) {
-          const bool first = I8 ? kb == 0 : kb % kPiece == 0;
+          const bool first = I8 ? kb == 0 : kb % PIECE == 0;
           if (first) {
             if (!(ok = wait_turn(&sums_empty[it & 1], ((it >> 1) & 1) ^ 1, a.wait_cycles))) break;
             tc_fence_after();
@@ -328,7 +330,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             if constexpr (CG == 2) umma_commit_2sm_mc(&empty[s], 0x3); else umma_commit(&empty[s]);
           }
           if (++s == STAGES) { s = 0; phase ^= 1; }
-          if (kb + 1 == a.kbs || (!I8 && kb % kPiece == kPiece - 1)) {
+          if (kb + 1 == a.kbs || (!I8 && kb % PIECE == PIECE - 1)) {
             if (elected) {
               if constexpr (CG == 2) umma_commit_2sm_mc(&sums_full[it & 1], 0x3); else umma_commit(&sums_full[it & 1]);
             }
@@ -382,7 +384,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         if constexpr (!I8) {
 #pragma unroll
           for (int j = 0; j < MINE; ++j) sums[j] = 0.f;
-          for (int k0 = 0; k0 < a.kbs; k0 += kPiece) {
+          for (int k0 = 0; k0 < a.kbs; k0 += PIECE) {
             if (!sums_there()) break;
 #pragma unroll
             for (int c = 0; c < MINE; c += 32) {
@@ -997,7 +999,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid
     uint32_t phase = 0, d = 0;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
       for (int kb = 0; kb < a.kbs; ++kb) {
-        const bool first = I8 ? kb == 0 : kb % kPiece == 0;
+        const bool first = I8 ? kb == 0 : kb % kFewPiece == 0;
         if (first) {
           if (!(ok = wait_turn(&sums_empty[it & 1], ((it >> 1) & 1) ^ 1, a.wait_cycles))) break;
           tc_fence_after();
@@ -1016,7 +1018,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid
           umma_commit(&empty[s]);
         }
         if (++s == stages) { s = 0; phase ^= 1; }
-        if (kb + 1 == a.kbs || (!I8 && kb % kPiece == kPiece - 1)) {
+        if (kb + 1 == a.kbs || (!I8 && kb % kFewPiece == kFewPiece - 1)) {
           if (elected) umma_commit(&sums_full[it & 1]);
           ++it;
         }
@@ -1058,7 +1060,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_scores_kernel(const __grid
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) z[j] = 0.f;
-        for (int k0 = 0; k0 < a.kbs && ok; k0 += kPiece) take();
+        for (int k0 = 0; k0 < a.kbs && ok; k0 += kFewPiece) take();
       }
       __syncwarp();
       if (ok && n < a.V) {
