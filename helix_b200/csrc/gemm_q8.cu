@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(Cfg<I8, BN, CG, EPI>::THREADS, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
             const __grid_constant__ TileArgs a) {
   using C = Cfg<I8, BN, CG, EPI>;
-  constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG, PIECE = CG == 1 ? kFewPiece : kPiece;
+  constexpr int STAGES = C::STAGES, EG = C::EG, TILE_M = TM * CG, PIECE = BN == 128 ? kFewPiece : kPiece;
   constexpr bool kScores = EPI == EPI_SCORES, kGlu = EPI == EPI_SWIGLU, kF32 = EPI == EPI_F32;
   constexpr int OUT_BN = kGlu ? BN / 2 : BN, CHUNK = kF32 ? 32 : 64, NCHUNK = OUT_BN / CHUNK;
   static_assert(!kGlu || BN == 256, "[128 gate|128 up]");
@@ -355,7 +355,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       int mi, ni;
       tile_at(a, t, num_m, num_n, mi, ni);
       const int m0 = mi * TILE_M + (int)rank * TM, row_g = m0 + row;
-      const bool live = row_g < a.M;
+      const bool live = row_g < a.M, any = m0 + q * 32 < a.M;  // this row, one of the warp's is there
       float sx = 1.f;
       if constexpr (I8) sx = live ? __ldg(a.xs + row_g) : 0.f;
       int target = -1;
@@ -386,13 +386,15 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           for (int j = 0; j < MINE; ++j) sums[j] = 0.f;
           for (int k0 = 0; k0 < a.kbs; k0 += PIECE) {
             if (!sums_there()) break;
+            if (any) {
 #pragma unroll
-            for (int c = 0; c < MINE; c += 32) {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(t_row + grp * MINE + c, v);
-              tmem_ld_wait();
+              for (int c = 0; c < MINE; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(t_row + grp * MINE + c, v);
+                tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sums[c + j] += __uint_as_float(v[j]);
+                for (int j = 0; j < 32; ++j) sums[c + j] += __uint_as_float(v[j]);
+              }
             }
             release();
           }
@@ -459,7 +461,9 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           U += lo + hi;
         };
         const int n_first = ni * BN + grp * MINE;
-        if constexpr (I8) {
+        if (!any) {
+          if constexpr (I8) release();
+        } else if constexpr (I8) {
 #pragma unroll 1
           for (int c = 0; c < MINE; c += 32) {
             uint32_t v[32];
@@ -1396,6 +1400,16 @@ cudaError_t gemm_q8(cudaStream_t stream, const GemmQ8Args& g) {
 
 namespace {
 bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
+// Above 128 rows: pairs' tiles of 256 rows or blocks' of 128, whichever rounds end first: us per block of K, the least of a round (what follows the products), the pair's later start,
+// as in kShapes.  (us of pairs | blocks: 200 x 128256 x 4096 in bf16 210 | 231, 300 rows 353 | 322, 300 rows of codes, H = 1536, with a cap 84 | 73, 384 x 30522 x 768 in bf16 28.0 | 24.8,
+// 512 x 50000 x 2048 78 | 88, 1000 x 128256 x 1536 268 | 296, 1100 x 30522 x 768 50.8 | 48.8.)
+bool pairs_score(int T, int V, int kbs, bool i8, bool cap, int sms) {
+  const long long wide = (V + 255) / 256, pairs = sms / 2;
+  const double least = (i8 ? 3.2 : 4.9) + (cap ? 2.3 : 0.0);
+  const double two = (double)((wide * ((T + 255) / 256) + pairs - 1) / pairs) * std::max(kbs * 0.37, least) + 1.4;
+  const double one = (double)((wide * ((T + 127) / 128) + sms - 1) / sms) * std::max(kbs * 0.46, least);
+  return two <= one;
+}
 int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 4 : (V + 255) / 256 * 4; }  // at most
 }  // namespace
 
@@ -1429,7 +1443,10 @@ cudaError_t head_scores(cudaStream_t stream, const HeadScoresArgs& g) {
   int slots = 0;
   if (g.T <= kFewRows) e = i8 ? launch_few<true>(stream, g, a, sms, &slots) : launch_few<false>(stream, g, a, sms, &slots);
   else if (g.T <= TM) e = i8 ? launch_tiles<true, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 128, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
-  else e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
+  else if (pairs_score(g.T, g.V, ((i8 ? 1 : 2) * g.H + KB - 1) / KB, i8, g.softcap > 0.f, sms))
+    e = i8 ? launch_tiles<true, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 2, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
+  else
+    e = i8 ? launch_tiles<true, 256, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots) : launch_tiles<false, 256, 1, EPI_SCORES>(stream, a, x, w, g.H, sms, &slots);
   if (e != cudaSuccess) return e;
   // Few sums: many threads per row (a row of a head of 151936 x 1536 in codes 51.5 -> 47.8 us).  Blocks that wait beside the kernel before for its end cost it more than their start
   // is worth once there are more than a few (us started early | behind it: 4 rows of a 1 GB head 187.9 | 189.9, 16 rows 195.8 | 188.5, 128 rows 196.9 | 191.8)

@@ -343,7 +343,8 @@ def check_head(lp, entropy, x, xs, w, ws, targets, H, scale=1.0, cap=0.0):
 
 
 HEADS = [(1, 1, 8), (1, 2, 1), (3, 127, 64), (7, 1000, 100), (32, 5003, 256), (64, 129, 4096), (127, 300, 72), (128, 20000, 128), (129, 255, 64), (200, 30522, 768), (256, 4000, 500), (257, 1001, 264),
-         (600, 5003, 1000), (1100, 257, 33)]
+         (600, 5003, 1000), (1100, 257, 33),                        # blocks' tiles
+         (250, 9500, 2100), (500, 20100, 2100), (700, 18900, 2100)]  # pairs'
 
 
 @pytest.mark.parametrize("q8", [False, True])
