@@ -1402,12 +1402,12 @@ namespace {
 bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
 // Above 128 rows: pairs' tiles of 256 rows or blocks' of 128, whichever rounds end first: us per block of K, the least of a round (what follows the products), the pair's later start,
 // as in kShapes.  (us of pairs | blocks: 200 x 128256 x 4096 in bf16 210 | 231, 300 rows 353 | 322, 300 rows of codes, H = 1536, with a cap 84 | 73, 384 x 30522 x 768 in bf16 28.0 | 24.8,
-// 512 x 50000 x 2048 78 | 88, 1000 x 128256 x 1536 268 | 296, 1100 x 30522 x 768 50.8 | 48.8.)
+// 512 x 50000 x 2048 78 | 88, 1000 x 128256 x 1536 268 | 296, 1100 x 30522 x 768 50.8 | 48.8, 700 x 151936 x 1536 of codes with a cap 146 | 151.)
 bool pairs_score(int T, int V, int kbs, bool i8, bool cap, int sms) {
   const long long wide = (V + 255) / 256, pairs = sms / 2;
   const double least = (i8 ? 3.2 : 4.9) + (cap ? 2.3 : 0.0);
   const double two = (double)((wide * ((T + 255) / 256) + pairs - 1) / pairs) * std::max(kbs * 0.37, least) + 1.4;
-  const double one = (double)((wide * ((T + 127) / 128) + sms - 1) / sms) * std::max(kbs * 0.46, least);
+  const double one = (double)((wide * ((T + 127) / 128) + sms - 1) / sms) * std::max(kbs * 0.46, least + kbs * 0.03);
   return two <= one;
 }
 int score_slots(int T, int V) { return T <= TM ? (V + 127) / 128 * 4 : (V + 255) / 256 * 4; }  // at most
