@@ -663,10 +663,9 @@ def test_calls_on_two_streams_at_once(L):
         check_head(lp, en, x, xs, w, ws, t, K, 0.05)
 
 
-@pytest.mark.parametrize("M,N", [(5, 300), (300, 1000), (400, 6000), (2600, 2304)])
-def test_waits_that_run_out_end_the_call_and_are_said(L, M, N):
+@pytest.mark.parametrize("M,N,K", [(5, 300, 512), (300, 1000, 512), (400, 6000, 512), (2600, 2304, 512), (250, 9500, 2100), (6877, 260, 1948), (6672, 397, 2840)])
+def test_waits_that_run_out_end_the_call_and_are_said(L, M, N, K):
     """With a limit below 0 every wait is given up at once."""
-    K = 512
     (x, xs), (w, ws) = any_codes(1, M, K), any_codes(2, N, K)
     t = torch.zeros(M, dtype=torch.int32, device=DEV)
     lp, en, work = torch.zeros(M, device=DEV), torch.zeros(M, device=DEV), torch.empty(L.hbk_head_scores_workspace_floats(M, N), device=DEV)
