@@ -438,10 +438,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             }
             m = top;
           }
-          const float base = m > -INFINITY ? m : 0.f;
-          if (left < 32) {  // (0 times what is no infinity)
+          float base = m > -INFINITY ? m : 0.f;
+          if (left < 32) {  // (0 times what is no infinity: the distance itself, as a large m less 1e4 is m again)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = j < left ? f[j] : base - 1e4f;
+            for (int j = 0; j < 32; ++j) f[j] = j < left ? f[j] - base : -1e4f;
+            base = 0.f;
           }
           const uint64_t off = f2_pack(-base, -base), log2e = f2_pack(kLog2e, kLog2e);
           uint64_t s2 = f2_pack(0.f, 0.f), u2 = s2;  // two at a time

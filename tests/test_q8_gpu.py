@@ -434,6 +434,33 @@ def test_head_again_is_the_same(L):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def plain_head(w0, T, H, q8, scale=1.0):
+    """A head whose logits are scale times w0 [V], whole numbers of seven bits, in every row, through the call."""
+    V = len(w0)
+    x, w = torch.zeros(T, up(H, 16), dtype=torch.int8, device=DEV), torch.zeros(V, up(H, 16), dtype=torch.int8, device=DEV)
+    x[:, 0], w[:, 0] = 1, w0
+    ones = torch.ones(max(T, V), device=DEV)
+    z = scale * w0.double()[None].expand(T, V)
+    return (x, ones[:T], w, ones[:V], z) if q8 else (x.to(BF), None, w.to(BF), None, z)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("w0,last", [(1, 2), (-3, -1)])
+@pytest.mark.parametrize("T,V", [(9, 1001), (100, 1001), (100, 30522), (300, 1001), (300, 30522), (700, 33), (2100, 30522)])
+def test_head_of_very_large_logits(L, T, V, w0, last, q8):
+    """Logits 1e13 apart, the two largest the last: what is not there (columns from V on) has no weight however large the others are."""
+    H = 64
+    logits = torch.full((V,), w0, dtype=torch.int8, device=DEV)
+    logits[-2:] = last
+    x, xs, w, ws, z = plain_head(logits, T, H, q8, 1e13)
+    targets = torch.full((T,), V - 1, dtype=torch.int32, device=DEV)
+    targets[1::2] = 0
+    lp, entropy = head(L, x, xs, w, ws, targets, H, scale=1e13)
+    a, b = exact_scores(z - z.max(), targets)  # (whole numbers of 1e13: exact)
+    # two weights of 1 and their logarithm: four roundings of numbers below 2; a far token's score is its distance, rounded with both logits
+    assert ((lp.double() - a).abs() <= 2.0 ** -21 + 2.0 ** -21 * a.abs()).all() and (entropy.double() - b).abs().max() <= 2.0 ** -21
+
+
 # ------------------------------------------------------------------ scores from logits
 def scores(L, x, targets, top, V, want=("lp", "rank", "entropy", "top_lp")):
     T = x.shape[0]
