@@ -172,8 +172,8 @@ int hbk_gemm_q8(const void* X, int ldx, const float* x_scales, const void* W, in
                 const void* bias, int M, int N, int K, int epi, void* stream);
 /* Scores of given tokens straight from the head's product, whose logits are never stored: with z[t][v] = scale (X W^T)[t, v] (softcap > 0: softcap tanh(z / softcap)),
  * lp[t] = log softmax(z[t])[targets[t]] (-inf where that is none of 0..V-1) and entropy[t] in nats.  X [T][H], W [V][H] in bf16 (both scales NULL), or codes with x_scales
- * [T] and w_scales [V] (H up to 131056).  targets and lp, or entropy, may be NULL.  A row with an infinite or NaN logit has NaN.  workspace:
- * hbk_head_scores_workspace_floats(T, V) floats; launches that may run at the same time need one each. */
+ * [T] and w_scales [V] (H up to 131056).  targets and lp, or entropy, may be NULL.  A z of -inf has no weight (a row of nothing but these: lp -inf, entropy 0); a row with
+ * one of +inf or NaN has NaN.  workspace: hbk_head_scores_workspace_floats(T, V) floats; launches that may run at the same time need one each. */
 int hbk_head_scores(const void* X, int ldx, const float* x_scales, const void* W, int ldw, const float* w_scales, const int32_t* targets, float* lp,
                     float* entropy, float* workspace, int T, int V, int H, float scale, float softcap, void* stream);
 size_t hbk_head_scores_workspace_floats(int T, int V); /* 0: refused sizes */

@@ -461,6 +461,69 @@ def test_head_of_very_large_logits(L, T, V, w0, last, q8):
     assert ((lp.double() - a).abs() <= 2.0 ** -21 + 2.0 ** -21 * a.abs()).all() and (entropy.double() - b).abs().max() <= 2.0 ** -21
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("T,V", [(9, 1000), (9, 3), (64, 40001), (100, 1000), (300, 1001), (400, 3), (2100, 30522)])
+def test_head_logits_that_are_minus_infinity(L, T, V, cap, q8):
+    """Beside others a token whose logit is -inf has no weight (a cap makes it -cap): first, last, between others, and in a group of columns alone."""
+    H = 72
+    none = sorted({0, V // 2, *range(32, min(V - 1, 64)), *range(128, min(V - 1, 384)), V - 1} - {1})
+    if q8:
+        (x, xs), (w, ws) = any_codes(T, T, H), any_codes(V + 9, V, H)
+        xs, ws = xs * 3, ws * H ** -0.5
+        x[:, :H] = x[:, :H].abs().clamp(min=1)
+        w[none, :H] = -w[none, :H].abs().clamp(min=1)
+        ws[none] = INF
+        z = (x[:, :H].double() @ w[:, :H].double().T) * xs.double()[:, None] * ws.double()
+    else:
+        x, w, xs, ws = randn(T, T, up(H, 8)).abs().to(BF) + 0.5, (randn(V, V, up(H, 8)) * 2.5 * H ** -0.5).to(BF), None, None
+        w[none, 7] = -INF
+        z = x[:, :H].double() @ w[:, :H].double().T
+    assert torch.equal(torch.isinf(z), torch.isin(torch.arange(V, device=DEV), torch.tensor(none, device=DEV))[None].expand(T, V)) and (z < INF).all()
+    targets = torch.randint(0, V, (T,), generator=gen(T), device=DEV).int()
+    targets[0], targets[1], targets[2] = V // 2, V - 1, 1
+    lp, entropy = head(L, x, xs, w, ws, targets, H, cap=cap)
+    if cap:
+        z = cap * torch.tanh(z / cap)
+    a, b = exact_scores(z, targets)
+    seen = ~torch.isinf(z[0])
+    # (as check_head, of the logits that there are)
+    if q8:
+        off = (5 * 2.0 ** -24 + 2.0 ** -20) * z.abs().nan_to_num(posinf=0.0)
+    else:
+        off = ((x[:, :H].double().abs() @ w[:, :H].double().abs().nan_to_num(posinf=0.0).T) * (H / 16 + 4) * 2.0 ** -22 + 2.0 ** -20 * z.abs().nan_to_num(posinf=0.0))
+    worst, sums = off[:, seen].max(-1).values, 2.0 ** -18 + 2.0 ** -23 * z[:, seen].abs().max(-1).values
+    assert torch.equal(torch.isinf(lp), torch.isinf(a)) and not torch.isnan(lp).any()
+    assert ((lp.double() - a).abs() <= 2 * worst + sums)[~torch.isinf(a)].all()
+    assert ((entropy.double() - b).abs() <= 2 * (worst + sums) * (1 + math.log(V))).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("T,V", [(5, 1000), (100, 1000), (300, 1000), (300, 2001)])
+def test_head_of_nothing_but_minus_infinity(L, T, V, q8):
+    H = 64
+    x, xs, w, ws, _ = plain_head(torch.full((V,), -1, dtype=torch.int8, device=DEV), T, H, q8)
+    if q8:
+        ws = torch.full((V,), INF, device=DEV)
+    else:
+        w[:, 0] = -INF
+    lp, entropy = head(L, x, xs, w, ws, torch.zeros(T, dtype=torch.int32, device=DEV), H)
+    assert (lp == -INF).all() and (entropy == 0).all()
+
+
+@pytest.mark.parametrize("T", [5, 100, 300])
+def test_head_logits_whose_distance_has_no_number(L, T):
+    """Finite logits at both ends of fp32: the lowest have no weight."""
+    V, H = 1001, 64
+    x, w = torch.zeros(T, H, dtype=BF, device=DEV), torch.zeros(V, H, dtype=BF, device=DEV)
+    x[:, 0] = 1
+    w[:, 0] = -3e38
+    w[500, 0] = w[V - 1, 0] = 3e38
+    targets = torch.full((T,), 500, dtype=torch.int32, device=DEV)
+    lp, entropy = head(L, x, None, w, None, targets, H)
+    assert (lp + math.log(2)).abs().max() <= 2.0 ** -21 and (entropy - math.log(2)).abs().max() <= 2.0 ** -21
+
+
 # ------------------------------------------------------------------ scores from logits
 def scores(L, x, targets, top, V, want=("lp", "rank", "entropy", "top_lp")):
     T = x.shape[0]
