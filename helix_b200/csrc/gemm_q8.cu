@@ -904,13 +904,19 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
       for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(silu(__fmul_rn(__fmul_rn((float)acc[e], s_ws[c + e]), sx)), __fmul_rn(__fmul_rn((float)up[e], s_ws[64 + c + e]), sx));
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(__fmul_rn(__fmul_rn((float)acc[e], s_ws[c + e]), sx), s_bias[c + e]);  // (roundings as in tile_kernel)
+      for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn((float)acc[e], s_ws[c + e]), sx);  // (roundings as in tile_kernel, nothing added where that adds nothing: zeros keep their signs)
+      if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(f[e], s_bias[c + e]);
+      }
       if (a.epi == EPI_BIAS_GELU) {
         gelu_erf2(f[0], f[1]);
         gelu_erf2(f[2], f[3]);
       }
+      if (a.r) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(f[e], resid[e]);
+        for (int e = 0; e < 4; ++e) f[e] = __fadd_rn(f[e], resid[e]);
+      }
     }
     if (bad) f[0] = f[1] = f[2] = f[3] = __uint_as_float(0x7fffffffu);
     if (a.epi == EPI_F32) {

@@ -257,6 +257,24 @@ def test_product_bits_do_not_depend_on_the_other_rows(L, epi):
         assert torch.equal(part[:-1], whole[rows])
 
 
+@pytest.mark.parametrize("epi", [0, 1, 3, 4, 6])
+def test_product_zeros_have_the_same_sign_in_every_kernel(L, epi):
+    """Scales below 0, and such that products of them have no number: -0 as 0 times those is, whatever the other rows."""
+    M, N, K = 2600, 2304, 100
+    (x, xs), (w, ws) = any_codes(3, M, K), any_codes(4, N, K)
+    x[::3] = 0
+    xs[:2000], ws[::2] = -xs[:2000], -ws[::2]
+    xs[1000:], ws[1::4] = xs[1000:] * 1e-22, ws[1::4] * 1e-23
+    bias = torch.full((N,), -0.0, dtype=BF, device=DEV) if epi in (1, 4) else None
+    r = torch.full((M, N), -0.0, dtype=BF, device=DEV) if epi in (3, 4) else None
+    bits = torch.int32 if epi == 6 else torch.int16
+    whole = product(L, x, xs, w, ws, K, epi, r=r, bias=bias)[:M, :N].contiguous().view(bits)
+    assert (whole == torch.iinfo(bits).min).sum() > 1000  # -0
+    for rows in (slice(0, 3), slice(1000, 1030), slice(1900, 2028), slice(2000, 2500)):
+        part = product(L, x[rows], xs[rows].contiguous(), w, ws, K, epi, r=r[rows] if r is not None else None, bias=bias)
+        assert torch.equal(part[:-1, :N].contiguous().view(bits), whole[rows])
+
+
 @pytest.mark.parametrize("M", [3, 130, 2600])
 @pytest.mark.parametrize("a,b", [(-128, -128), (-128, 127), (127, 127)])
 def test_product_of_the_largest_sums(L, M, a, b):
