@@ -185,7 +185,7 @@ __device__ __forceinline__ void values_of(const uint32_t (&v)[NC], const TileArg
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) f[j] = (float)(int)v[j] * (n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f) * sx;
+    for (int j = 0; j < NC; ++j) f[j] = __fmul_rn(__fmul_rn((float)(int)v[j], n0 + j < a.N ? __ldg(a.ws + n0 + j) : 0.f), sx);  // (each rounded, as above and in split_kernel)
   }
 }
 // 32 bf16 values of a row (of which `left` are there) added
@@ -201,7 +201,7 @@ __device__ __forceinline__ void add_32(const bf16* p, int left, float (&f)[32]) 
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < left) f[j] += __bfloat162float(p[j]);
+      if (j < left) f[j] = __fadd_rn(f[j], __bfloat162float(p[j]));
   }
 }
 

@@ -257,6 +257,20 @@ def test_product_bits_do_not_depend_on_the_other_rows(L, epi):
         assert torch.equal(part[:-1], whole[rows])
 
 
+@pytest.mark.parametrize("epi", [0, 1, 2, 3, 4, 6])
+@pytest.mark.parametrize("N", [2284, 2305, 2335])
+def test_product_bits_do_not_depend_on_the_other_rows_in_the_last_columns(L, N, epi):
+    """Nor do they in the columns of a last group that is not whole."""
+    K = 1000
+    (x, xs), (w, ws) = any_codes(3, 2600, K), any_codes(4, N, K)
+    bias = randn(1, up(N, 8)).to(BF)[:N] if epi in (1, 2, 4) else None
+    r = randn(2, 2600, up(N, 8)).to(BF)[:, :N] if epi in (3, 4) else None
+    whole = product(L, x, xs, w, ws, K, epi, r=r, bias=bias)[:2600, :N]
+    for rows in (slice(0, 1), slice(70, 100), slice(1000, 1300), slice(2000, 2500)):
+        part = product(L, x[rows], xs[rows].contiguous(), w, ws, K, epi, r=r[rows] if r is not None else None, bias=bias)
+        assert torch.equal(part[:-1, :N], whole[rows])
+
+
 @pytest.mark.parametrize("epi", [0, 1, 3, 4, 6])
 def test_product_zeros_have_the_same_sign_in_every_kernel(L, epi):
     """Scales below 0, and such that products of them have no number: -0 as 0 times those is, whatever the other rows."""
