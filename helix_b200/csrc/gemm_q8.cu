@@ -1288,7 +1288,7 @@ struct SplitPlan {
 };
 SplitPlan split_plan(int M, int N, int kbs, int sms) {
   const int box = std::min(TM, (M + 15) / 16 * 16);
-  const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = (long long)((box <= 64 ? 2 : 1) * 0.88 * sms);
+  const long long tiles = (long long)((M + TM - 1) / TM) * ((N + SN - 1) / SN), room = std::max(1LL, (long long)((box <= 64 ? 2 : 1) * 0.88 * sms));
   int parts = 1;
   while (parts < 8 && tiles * (parts + 1) <= room && kbs >= 4 * (parts + 1)) ++parts;
   const int stage = box * KB + SN * KB, most = (kbs + parts - 1) / parts;

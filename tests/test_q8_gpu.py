@@ -1,4 +1,5 @@
 """Rows coded in 8 bits, products of such rows, and scores of given tokens (from a head's product and from logits), each against plain 64-bit forms, and together."""
+import ctypes
 import math
 
 import pytest
@@ -323,6 +324,22 @@ def test_product_of_many_columns(L):
         check_product(out[:M, cols], x, xs, w[cols], ws[cols], K, 0)
     one = product(L, x[:1], xs[:1], w, ws, K, 0)
     assert torch.equal(one[0, :N], out[0, :N])
+
+
+@pytest.mark.parametrize("sms", [1, 2, 3])
+def test_product_within_few_sms(L, sms):
+    """A caller's share of the SMs (hb::sm_limit, of its thread) may be as small as one."""
+    limit = L._ZN2hb8sm_limitEv
+    limit.restype = ctypes.POINTER(ctypes.c_int)
+    try:
+        for M, N, K in ((5, 300, 700), (100, 300, 700), (300, 515, 300)):
+            (x, xs), (w, ws) = any_codes(1, M, K), any_codes(2, N, K)
+            limit()[0] = sms
+            out = product(L, x, xs, w, ws, K, 0)
+            limit()[0] = 0
+            check_product(out[:M, :N], x, xs, w, ws, K, 0)
+    finally:
+        limit()[0] = 0
 
 
 # ------------------------------------------------------------------ scores from a head's product
