@@ -140,6 +140,19 @@ def test_rows_that_have_no_scale(L):
         assert (codes[:6] == 0).all() and (scales[[0, 1, 5]] == 0).all() and torch.isnan(scales[2:5]).all() and torch.isnan(seen[2:5]).all() and (codes[6] != 0).any()
 
 
+@pytest.mark.parametrize("T,K", [(600, 9000), (901, 8193), (1300, 10240), (1200, 12287), (1250, 14336), (1301, 16381), (1190, 16384)])
+def test_long_rows_one_after_the_other(L, T, K):
+    """fp32 rows of 8193 to 16384 entries, more than the SMs take at a time: a block has several, the next on its way while it works on one."""
+    x = randn(K, T, up(K, 8) + 8) * torch.exp(3 * randn(T, T, 1))
+    x[T // 2, :] = 0
+    x[T // 2 + 1, K - 1] = NAN
+    x[T // 3, 5] = -INF
+    x[T - 1, K - 1] = 1e5
+    x = x[:, :K]
+    check_codes(x, *code(L, x))
+    check_codes(x, *code(L, x, seen=None))
+
+
 def test_rows_beyond_32_bit_offsets(L):
     K, ld = 3000, 2 ** 30 + 16
     x = torch.empty(2 * ld + up(K, 8), dtype=BF, device=DEV)
