@@ -586,6 +586,39 @@ def test_head_logits_whose_distance_has_no_number(L, T):
     assert (lp + math.log(2)).abs().max() <= 2.0 ** -21 and (entropy - math.log(2)).abs().max() <= 2.0 ** -21
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("T,V,H", [(1, 151936, 72), (16, 40000, 256), (33, 58000, 100), (64, 128256, 64)])
+def test_head_of_few_rows_with_many_tiles_for_each_block(L, T, V, H, q8):
+    targets = torch.randint(0, V, (T,), generator=gen(T), device=DEV).int()
+    targets[::5] = V - 1
+    if q8:
+        (x, xs), (w, ws) = any_codes(T, T, H), any_codes(V + 9, V, H)
+        xs, ws = xs * 3, ws * H ** -0.5
+    else:
+        x, w = randn(T, T, up(H, 8) + 8).to(BF), (randn(V, V, up(H, 8) + 8) * 2.5 * H ** -0.5).to(BF)
+        xs = ws = None
+    for scale, cap in ((1.0, 0.0), (0.5, 2.0)):
+        lp, entropy = head(L, x, xs, w, ws, targets, H, scale, cap)
+        check_head(lp, entropy, x, xs, w, ws, targets, H, scale, cap)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("way", ["rising", "falling", "up and down", "at the end"])
+@pytest.mark.parametrize("T", [1, 20, 64, 100, 300])
+def test_head_of_logits_that_change_from_tile_to_tile(L, T, way, q8):
+    """Logits of one tile lie far from those of the next that its block takes: sums are brought to another maximum on the way, or are not."""
+    V, H = 110001, 64
+    step = torch.arange(V, device=DEV) // 10000  # (148 blocks take 18944 columns at a time)
+    by = {"rising": 11 * step, "falling": 110 - 11 * step, "up and down": 30 * (step // 2 % 2), "at the end": 100 * (torch.arange(V, device=DEV) >= V - 3)}[way]
+    x, xs, w, ws, _ = plain_head(by.to(torch.int8), T, H, q8)
+    x[:, 1:] = torch.randint(-1, 2, (T, H - 1), generator=gen(1), device=DEV).to(x.dtype)
+    w[:, 1:] = (torch.rand(V, H - 1, generator=gen(2), device=DEV) < 0.06).to(w.dtype)
+    targets = torch.randint(0, V, (T,), generator=gen(T), device=DEV).int()
+    targets[0] = V - 1
+    lp, entropy = head(L, x, xs, w, ws, targets, H)
+    check_head(lp, entropy, x, xs, w, ws, targets, H)
+
+
 # ------------------------------------------------------------------ scores from logits
 def scores(L, x, targets, top, V, want=("lp", "rank", "entropy", "top_lp")):
     T = x.shape[0]
