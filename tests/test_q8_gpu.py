@@ -619,6 +619,34 @@ def test_head_of_logits_that_change_from_tile_to_tile(L, T, way, q8):
     check_head(lp, entropy, x, xs, w, ws, targets, H)
 
 
+@pytest.mark.parametrize("T,piece", [(48, 256), (120, 256), (512, 512)])
+def test_head_of_bf16_is_as_near_as_its_pieces_make_it(L, T, piece):
+    """Sixteen products at a time are added to a sum, which is cut off at its last place (2^-23 of it at most, half of that on the average) each time, until a piece of K is full; the pieces are
+    added in fp32.  A score is off by its token's logit and by the weighted mean of all: 2e-5 and less.  (In one piece of 4096 older and larger sums are cut off: some 4e-5.)"""
+    V, H = 3000, 4096
+    x, w = randn(T, T, H).to(BF), (randn(V, V, H) * 2.5 * H ** -0.5).to(BF)
+    targets = torch.randint(0, V, (T,), generator=gen(T), device=DEV).int()
+    xd, wd = x.double(), w.double()
+    z, off, bound = torch.zeros(T, V, dtype=torch.float64, device=DEV), torch.zeros(T, V, dtype=torch.float64, device=DEV), {}
+    for k0 in range(0, H, piece):
+        part = torch.zeros_like(z)
+        for k in range(k0, k0 + piece, 16):
+            part += xd[:, k:k + 16] @ wd[:, k:k + 16].T
+            off += 2.0 ** -24 * part.abs()
+        z += part
+        off += 2.0 ** -24 * z.abs()
+    lp, entropy = head(L, x, None, w, None, targets, H)
+    a, b = exact_scores(z, targets)
+    q = torch.exp(z - torch.logsumexp(z, -1, keepdim=True))
+    tol = off.gather(1, targets.long()[:, None])[:, 0] + (q * off).sum(-1) + 2.0 ** -22 * (1 + a.abs())  # (and the sums of exponentials: 2^-22 of theirs on the average)
+    err = lp.double() - a
+    assert err.square().mean().sqrt() <= tol.square().mean().sqrt() and err.mean().abs() <= tol.mean(), (err.square().mean().sqrt().item(), tol.square().mean().sqrt().item())
+    assert tol.square().mean().sqrt() < 3e-5
+    mean = ((q * (z - (q * z).sum(-1, keepdim=True))).abs() * off).sum(-1) + 2.0 ** -21 * (1 + math.log(V))  # (an entropy's slope: a weight times its distance from the mean)
+    gone = entropy.double() - b
+    assert gone.square().mean().sqrt() <= mean.square().mean().sqrt(), (gone.square().mean().sqrt().item(), mean.square().mean().sqrt().item())
+
+
 # ------------------------------------------------------------------ scores from logits
 def scores(L, x, targets, top, V, want=("lp", "rank", "entropy", "top_lp")):
     T = x.shape[0]
