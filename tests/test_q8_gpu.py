@@ -898,3 +898,45 @@ def test_waits_that_run_out_end_the_call_and_are_said(L, M, N, K):
     torch.cuda.synchronize()
     assert L.hbk_q8_status() == 0
     check_product(out[:, :N], x, xs, w, ws, K, 6)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 20000), (60, 40000, 2048), (100, 5000, 2048), (128, 768, 9000), (300, 1000, 512), (400, 6000, 512), (2600, 2304, 512), (250, 9500, 9000), (6877, 260, 1948),
+                                   (6672, 397, 2840)])
+def test_waits_that_run_out_half_way_end_the_call_and_are_said(L, M, N, K):
+    """With short limits waits are given up while copies and products are on their way: the call ends, what it says it lost is NaN, the rest is as it is without a limit."""
+    (x, xs), (w, ws) = any_codes(1, M, K), any_codes(2, N, K)
+    xb, wb = x[:, :up(K, 16)].to(BF), w[:, :up(K, 16)].to(BF)
+    t = torch.randint(0, N, (M,), generator=gen(3), device=DEV).int()
+    work = torch.empty(L.hbk_head_scores_workspace_floats(M, N), device=DEV)
+    out, lp, en = torch.zeros(M, up(N, 8), device=DEV), torch.zeros(M, device=DEV), torch.zeros(M, device=DEV)
+
+    said = 0
+
+    def calls():
+        yield lambda: L.hbk_gemm_q8(p(x), x.stride(0), p(xs), p(w), w.stride(0), p(ws), p(out), out.stride(0), None, 0, None, M, N, K, 6, here()), [out]
+        yield lambda: L.hbk_head_scores(p(x), x.stride(0), p(xs), p(w), w.stride(0), p(ws), p(t), p(lp), p(en), p(work), M, N, K, 1e-3, 0.0, here()), [lp, en]
+        yield lambda: L.hbk_head_scores(p(xb), xb.stride(0), None, p(wb), wb.stride(0), None, p(t), p(lp), p(en), p(work), M, N, K, 1e-6, 0.0, here()), [lp, en]
+
+    for call, outs in calls():
+        ck(L, call())
+        torch.cuda.synchronize()
+        good = [o.clone() for o in outs]
+        assert L.hbk_q8_status() == 0 and all(torch.isfinite(o).all() for o in good)
+        for limit in (1, 200, 700, 1500, 3000, 6000, 12000, 25000):
+            former = L.hbk_q8_wait_cycles(limit)
+            try:
+                ck(L, call())
+                torch.cuda.synchronize()
+            finally:
+                L.hbk_q8_wait_cycles(former)
+            status = L.hbk_q8_status()
+            assert status in (0, 702)
+            said += status == 702
+            lost = [torch.isnan(o) for o in outs]
+            assert any(n.any() for n in lost) == (status == 702)
+            for o, n, g in zip(outs, lost, good):
+                assert torch.equal(o[~n], g[~n])
+        ck(L, call())
+        torch.cuda.synchronize()
+        assert L.hbk_q8_status() == 0 and all(torch.equal(o, g) for o, g in zip(outs, good))
+    assert said or K < 9000  # (a wait for the products of long rows takes longer than one look at it)
