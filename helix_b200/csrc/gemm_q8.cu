@@ -942,7 +942,9 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __grid_const
 }
 
 // ------------------------------------------------------------------ scores of few rows
-constexpr int kFewRows = 64, kFewThreads = 64 + 4 * 128, kFewSmem = 184 * 1024;  // (us of 32 | 16 rows of a 1 GB head with 100, 130, 165, 200, 225 KB: 181, 171, 166, 165, 173 | 176, 168, 164, 168, 174)
+// Shared memory: us of 1 | 16 | 32 | 64 rows of a 1 GB head with 130 KB 167 | 169 | 173 | 180, 165 KB 163 | 164 | 167 | 176, 184 KB 164 | 166 | 166 | 173, 200 KB 166 | 168 | 165 | 171 (32 | 16 rows
+// with 100 KB 181 | 176, 225 KB 173 | 174)
+constexpr int kFewRows = 64, kFewThreads = 64 + 4 * 128, kFewSmem = 184 * 1024;
 
 struct FewArgs {
   const float *xs, *ws;
@@ -1423,7 +1425,8 @@ namespace {
 bool score_sizes_ok(int T, int V) { return T >= 0 && T <= (1 << 28) && V >= 1 && V <= (1 << 30); }
 // Above 128 rows: pairs' tiles of 256 rows or blocks' of 128, whichever rounds end first: us per block of K, the least of a round (what follows the products), the pair's later start,
 // as in kShapes.  (us of pairs | blocks: 200 x 128256 x 4096 in bf16 210 | 231, 300 rows 353 | 322, 300 rows of codes, H = 1536, with a cap 84 | 73, 384 x 30522 x 768 in bf16 28.0 | 24.8,
-// 512 x 50000 x 2048 78 | 88, 1000 x 128256 x 1536 268 | 296, 1100 x 30522 x 768 50.8 | 48.8, 700 x 151936 x 1536 of codes with a cap 146 | 151.)
+// 512 x 50000 x 2048 78 | 88, 1000 x 128256 x 1536 268 | 296, 1100 x 30522 x 768 50.8 | 48.8, 700 x 151936 x 1536 of codes with a cap 146 | 151: what follows the products of a block takes a
+// little longer the more of them there are beside it, 0.03 us per block of K by these runs.)
 bool pairs_score(int T, int V, int kbs, bool i8, bool cap, int sms) {
   const long long wide = (V + 255) / 256, pairs = sms / 2;
   const double least = (i8 ? 3.2 : 4.9) + (cap ? 2.3 : 0.0);

@@ -161,7 +161,8 @@ int hbk_gemm_q4(const void* X, int ldx, const void* W4, void* out, int ldo, cons
  * on 16 bytes, strides of codes are multiples of 16, others of 8 (fp32 out of a product: 4).  Rows, columns and logits of a row up to 2^30 (scored rows 2^28).
  *
  * Rows x [T][ldx >= K] (bf16, or fp32 where x_f32) to codes [T][ldc >= K] and scales [T]: s = max |x| / 127 rounded to fp32, c the whole number nearest to x / s (exactly: of
- * two equally near ones the even one).  A row of zeros has scale 0 and codes 0, as has one whose s rounds to 0; a row with an infinity or a NaN has scale NaN and codes 0.
+ * two equally near ones the even one; where the largest |x| is below 3e-41, s may round down so far that x / s passes 127.5: c stays 127).  A row of zeros has scale 0 and
+ * codes 0, as has one whose s rounds to 0; a row with an infinity or a NaN has scale NaN and codes 0.
  * seen [T][lds >= K] (or NULL; may be x itself where that is bf16, with its stride): s c in bf16, what products in 16 bits take if they shall see what products of the codes
  * do.  Columns from K on are left as they are.  Weights are coded by the same call, a channel per row. */
 int hbk_rows_q8(const void* x, int x_f32, int ldx, void* codes, int ldc, float* scales, void* seen, int lds, int T, int K, void* stream);

@@ -622,7 +622,7 @@ def test_head_of_logits_that_change_from_tile_to_tile(L, T, way, q8):
 @pytest.mark.parametrize("T,piece", [(48, 256), (120, 256), (512, 512)])
 def test_head_of_bf16_is_as_near_as_its_pieces_make_it(L, T, piece):
     """Sixteen products at a time are added to a sum, which is cut off at its last place (2^-23 of it at most, half of that on the average) each time, until a piece of K is full; the pieces are
-    added in fp32.  A score is off by its token's logit and by the weighted mean of all: 2e-5 and less.  (In one piece of 4096 older and larger sums are cut off: some 4e-5.)"""
+    added in fp32.  A score is off by its token's logit and by the weighted mean of all: 2e-5 and less.  (In one piece of 4096 older and larger sums are cut off: 2.5e-5 and more.)"""
     V, H = 3000, 4096
     x, w = randn(T, T, H).to(BF), (randn(V, V, H) * 2.5 * H ** -0.5).to(BF)
     targets = torch.randint(0, V, (T,), generator=gen(T), device=DEV).int()
